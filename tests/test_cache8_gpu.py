@@ -1,0 +1,365 @@
+"""Append to an 8-bit cache (store8.hip) and attention over it (attention8.hip) against their formulas in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from plain_cache8 import attention, store
+from vosti_amd.kernels import KernelError, kernels_for
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def host(t):
+    return None if t is None else t.detach().to(torch.float64).cpu().numpy()
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def tables(rng, keys, P, spare=3, width=None):
+    """Pages of every sequence in any order, and a table that holds page numbers of nothing behind them."""
+    used = [-(-k // P) for k in keys]
+    order = rng.permutation(sum(used) + spare)
+    W = max(max(used, default=0), 1) if width is None else width
+    table, at = np.full((len(keys), W), 10 ** 9), 0
+    for s, n in enumerate(used):
+        table[s, :n] = order[at:at + n]
+        at += n
+    return table, sum(used) + spare
+
+
+def rotation(places, half, dtype):
+    angle = torch.arange(places, dtype=torch.float64)[:, None] * 1e4 ** (-torch.arange(half, dtype=torch.float64) / half)
+    return torch.cos(angle).to(dtype).cuda(), torch.sin(angle).to(dtype).cuda()
+
+
+def filled(rng, pages, nkv, P, d, low=-9, high=-4):
+    """A cache whose entries use their range, NaN in none."""
+    def entries(*shape):
+        return torch.from_numpy(np.clip(rng.standard_normal(shape) * 90, -448, 448)).to(torch.float32).to(E4M3).cuda()
+    scales = torch.from_numpy(2.0 ** rng.integers(low, high, (pages, nkv, 2))).to(torch.float32).cuda()
+    return entries(pages, nkv, P, d), entries(pages, nkv, d, P), scales
+
+
+STORES = [
+    # (type, rows, keys, nq, nkv, d, P, norm, rotated entries)
+    ("bf16", [1], [1], 2, 1, 16, 16, True, 16),
+    ("bf16", [1, 1, 1], [64, 65, 100], 8, 2, 128, 64, True, 128),
+    ("bf16", [130], [130], 4, 2, 128, 64, True, 128),
+    ("bf16", [5, 0, 200, 1, 17], [70, 9, 200, 128, 33], 6, 2, 64, 32, True, 64),
+    ("bf16", [40, 3], [50, 259], 3, 3, 80, 16, False, 40),
+    ("bf16", [300, 2], [301, 5], 2, 1, 256, 256, True, 256),
+    ("bf16", [33], [40], 5, 1, 192, 128, True, 96),
+    ("bf16", [7] * 70, [7 + 3 * i for i in range(70)], 2, 1, 32, 16, True, 20),
+    ("f32", [1, 1], [16, 17], 4, 2, 64, 16, True, 64),
+    ("f32", [90, 0, 31], [95, 0, 64], 4, 4, 96, 32, True, 48),
+    ("f32", [21, 300], [21, 300], 2, 2, 256, 128, False, 0),
+    ("f32", [5], [300], 2, 1, 16, 256, True, 8),
+]
+
+
+@pytest.mark.parametrize("case", range(len(STORES)))
+def test_append_is_the_formula(case):
+    """Entries and scales to the bit (they are computed in 64 bits and rounded once); q off by its rounding and a few 32-bit ones, of sums of d squares and two products:
+    half a step of the type and 2^-24 (d / 64 + 12) of the two entries that a rotation mixes."""
+    name, rows, keys, nq, nkv, d, P, norm, turned = STORES[case]
+    dtype, k = TYPES[name], kernels_for(name)
+    rng = np.random.default_rng(case)
+    T = sum(rows) + 2                                          # two rows behind the last sequence
+    qkv = torch.from_numpy(rng.standard_normal((T, (nq + 2 * nkv) * d)) * 2.0 ** rng.integers(-3, 4, (T, 1))).to(dtype).cuda()
+    table, pages = tables(rng, keys, P)
+    kc, vc, scales = filled(rng, pages, nkv, P, d)
+    q_w = k_w = cos = sin = None
+    if norm:
+        q_w, k_w = (torch.from_numpy(rng.uniform(0.5, 1.5, d)).to(dtype).cuda() for _ in range(2))
+    if turned:
+        cos, sin = rotation(max(keys) + 3, turned // 2, dtype)
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    want_k, want_v, want_s = host(kc), host(vc), host(scales)
+    want = store(host(qkv), nq, nkv, d, want_k, want_v, want_s, host(q_w), host(k_w), 1e-5, host(cos), host(sin), table, cu, keys)
+    out = torch.full((T, nq, d), 77.0, dtype=dtype, device="cuda")
+    got = k.qkv_post8(qkv, nq=nq, nkv=nkv, d=d, k_cache=kc, v_cache=vc, scales=scales, q_w=q_w, k_w=k_w, eps=1e-5, cos=cos, sin=sin, block_table=ints(table),
+                      cu_q=ints(cu), k_len=ints(keys), max_k_len=max(keys), q_out=out)
+    assert got is out
+    assert np.array_equal(host(scales), want_s)
+    assert np.array_equal(host(kc), want_k)
+    assert np.array_equal(host(vc), want_v)
+    got = host(got)
+    assert (got[sum(rows):] == 77.0).all()
+    got, want = got[:sum(rows)], want[:sum(rows)]
+    most = np.abs(want).max(-1, keepdims=True)
+    assert (np.abs(got - want) <= torch.finfo(dtype).eps / 2 * np.abs(want) * (1 + 1e-3) + 2.0 ** -24 * (d / 64 + 12) * most).all()
+
+
+def append(k, x, kc, vc, scales, table, keys, rows=None, d=64, nkv=1):
+    rows = [1] * len(keys) if rows is None else rows
+    k.qkv_post8(x, nq=0, nkv=nkv, d=d, k_cache=kc, v_cache=vc, scales=scales, q_w=None, k_w=None, eps=0.0, cos=None, sin=None, block_table=ints(table),
+                cu_q=ints(np.concatenate([[0], np.cumsum(rows)])), k_len=ints(keys), max_k_len=max(keys))
+
+
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+def test_a_page_appended_token_by_token_is_the_page_appended_at_once(name):
+    """Entries of at least 2^-14 of the largest: whatever order their scale grew in."""
+    k, d, P = kernels_for(name), 64, 32
+    rng = np.random.default_rng(3)
+    x = torch.from_numpy(rng.standard_normal((P, 2 * d)).clip(-3, 3) * 2.0 ** rng.integers(-4, 5, (P, 1))).to(TYPES[name])
+    x = torch.where(x.abs() < 2.0 ** -6, torch.zeros_like(x), x).cuda()
+    one, many = k.empty_cache8(2, 1, P, d), k.empty_cache8(2, 1, P, d)
+    append(k, x, *one, [[1]], [P], [P])
+    for i in range(P):
+        append(k, x[i:i + 1], *many, [[1]], [i + 1])
+    for a, b in zip(one, many):
+        assert np.array_equal(host(a), host(b))
+
+
+def test_what_is_not_finite_is_stored_as_nan_and_does_not_set_the_scale():
+    k, d = kernels_for("bf16"), 64
+    x = torch.ones(3, 2 * d, dtype=torch.bfloat16, device="cuda")
+    x[0, 3], x[1, 5], x[2, d + 7] = float("inf"), float("nan"), -float("inf")
+    kc, vc, scales = k.empty_cache8(1, 1, 16, d)
+    append(k, x, kc, vc, scales, [[0]], [3], [3])
+    assert scales.tolist() == [[[2.0 ** -8, 2.0 ** -8]]]
+    kf, vf = kc[0, 0, :3].float(), vc[0, 0, :, :3].float().T
+    assert torch.isnan(kf).nonzero().tolist() == [[0, 3], [1, 5]] and torch.isnan(vf).nonzero().tolist() == [[2, 7]]
+    assert torch.nan_to_num(kf, nan=256.0).eq(256.0).all() and torch.nan_to_num(vf, nan=256.0).eq(256.0).all()
+
+
+def test_zeros_extremes_and_pages_that_are_none():
+    """A page of zeros has the smallest scale; the largest number of the type fits; -1 and a number beyond the cache keep nothing; a sequence that exceeds the
+    bound is left out."""
+    k, d = kernels_for("f32"), 16
+    kc, vc, scales = k.empty_cache8(4, 1, 16, d)
+    x = torch.zeros(5, 2 * d, device="cuda")
+    x[1] = torch.finfo(torch.float32).max
+    x[2:] = 1.0
+    k.qkv_post8(x, nq=0, nkv=1, d=d, k_cache=kc, v_cache=vc, scales=scales, q_w=None, k_w=None, eps=0.0, cos=None, sin=None,
+                block_table=ints([[0, 9], [1, 9], [-1, 9], [4, 9], [3, 3]]), cu_q=ints([0, 1, 2, 3, 4, 5]), k_len=ints([1, 1, 1, 1, 30]), max_k_len=20)
+    assert scales[0].tolist() == [[2.0 ** -64] * 2] and scales[1].tolist() == [[2.0 ** 120] * 2]
+    assert kc[1, 0, 0].float().tolist() == [256.0] * d          # 2^128 - 2^104 in 2^120, to four digits
+    assert not scales[2:].any() and not kc[2:].float().any() and not vc[2:].float().any()
+
+
+def test_rows_of_a_wider_tensor_and_either_half_alone():
+    k, nq, nkv, d, P = kernels_for("bf16"), 4, 2, 64, 16
+    rng = np.random.default_rng(5)
+    wide = torch.from_numpy(rng.standard_normal((9, (nq + 2 * nkv) * d + 24))).to(torch.bfloat16).cuda()
+    rows = wide[:, 16:16 + (nq + 2 * nkv) * d]
+    cos, sin = rotation(16, d // 2, torch.bfloat16)
+    common = dict(d=d, q_w=None, k_w=None, eps=0.0, cos=cos, sin=sin, block_table=ints([[1]]), cu_q=ints([0, 9]), k_len=ints([9]), max_k_len=9)
+    one, two = k.empty_cache8(2, nkv, P, d), k.empty_cache8(2, nkv, P, d)
+    q = k.qkv_post8(rows, nq=nq, nkv=nkv, k_cache=one[0], v_cache=one[1], scales=one[2], **common)
+    q2 = k.qkv_post8(rows[:, :nq * d], nq=nq, nkv=0, k_cache=None, v_cache=None, scales=None, **common)
+    assert k.qkv_post8(rows[:, nq * d:].contiguous(), nq=0, nkv=nkv, k_cache=two[0], v_cache=two[1], scales=two[2], **common) is None
+    assert torch.equal(q, q2)
+    for a, b in zip(one, two):
+        assert np.array_equal(host(a), host(b))
+
+
+# ------------------------------------------------------------------------------------------------------ attention
+def close(got, plain, name, d):
+    """A result is off by half a step of its type; by the weights' rounding (half a step of sixteen-bit floating point, 2^-11, of the sum of weights times |v|; weights
+    below 2^-24 of the largest by 2^-25 of it); and by the scores', sums of d products in 32 bits: (d + 16) 2^-24 of the largest sum of |q k|, twice (numerator
+    and denominator), and 2^-20 for the exponentials."""
+    out, weighted, most, flushed = plain
+    dtype = TYPES[name]
+    score = 2 * (d + 16) * 2.0 ** -24 * most + 2.0 ** -20
+    weights = 2.0 ** -11 if name == "bf16" else 2.0 ** -20
+    bound = torch.finfo(dtype).eps / 2 * np.abs(out) * 1.01 + weighted * (weights + score) + (2.0 ** -25 if name == "bf16" else 0.0) * flushed + 1e-30
+    got = host(got)
+    assert np.array_equal(np.isnan(got), np.isnan(out)), np.argwhere(np.isnan(got) != np.isnan(out))[:5]
+    fine = ~np.isnan(out)
+    off = np.abs(got - out)[fine] / bound[fine]
+    assert off.size == 0 or off.max() <= 1, (off.max(), got[fine][off.argmax()], out[fine][off.argmax()])
+
+
+def items_of(rows, most):
+    return ints([(s, a) for s, n in enumerate(rows) for a in range(0, n, most)] or np.zeros((0, 2)))
+
+
+def attend(k, q, cache, table, rows, keys, most, window=0, scale=None, max_k_len=None, **kw):
+    return k.paged_attention8(q, *cache, ints(table), ints(np.concatenate([[0], np.cumsum(rows)])), ints(keys), items_of(rows, most), item_rows=most,
+                              scale=q.shape[2] ** -0.5 if scale is None else scale, window=window, max_k_len=max(keys) if max_k_len is None else max_k_len, **kw)
+
+
+ATTENDS = [
+    # (type, rows, keys, nq, nkv, d, P, window, rows of an item)
+    ("bf16", [1], [1], 2, 1, 16, 16, 0, 1),
+    ("bf16", [1, 1, 1, 1], [63, 64, 65, 1030], 8, 2, 128, 64, 0, 1),
+    ("bf16", [1, 1], [300, 2000], 16, 2, 64, 16, 0, 1),
+    ("bf16", [5, 3, 1], [5, 259, 700], 10, 2, 128, 64, 0, 5),
+    ("bf16", [9, 16], [9, 300], 16, 2, 80, 32, 0, 16),
+    ("bf16", [16], [513], 64, 1, 128, 128, 0, 16),
+    ("bf16", [4, 1, 2], [900, 3, 600], 8, 8, 256, 64, 0, 4),
+    ("bf16", [3, 2], [400, 64], 6, 1, 192, 256, 0, 3),
+    ("bf16", [2, 5, 1], [700, 300, 40], 12, 4, 96, 16, 100, 5),
+    ("bf16", [1, 3], [600, 520], 4, 2, 128, 64, 1, 3),
+    ("bf16", [17], [17], 4, 2, 128, 64, 0, 128),
+    ("bf16", [150, 20, 1], [150, 333, 70], 8, 2, 128, 64, 0, 128),
+    ("bf16", [130, 60], [200, 60], 5, 1, 64, 16, 33, 128),
+    ("bf16", [70], [200], 3, 3, 256, 32, 0, 64),
+    ("bf16", [40], [41], 14, 2, 192, 128, 0, 40),
+    ("bf16", [33, 18], [100, 18], 6, 2, 32, 16, 7, 33),
+    ("f32", [1, 1], [64, 515], 8, 2, 64, 16, 0, 1),
+    ("f32", [4, 2], [300, 7], 16, 2, 128, 64, 0, 4),
+    ("f32", [7], [260], 8, 1, 256, 32, 50, 7),
+    ("f32", [3], [70], 2, 2, 192, 16, 0, 3),
+    ("f32", [66, 20], [100, 300], 4, 2, 80, 16, 0, 128),
+    ("f32", [30], [90], 4, 1, 256, 64, 20, 30),
+    ("f32", [140], [140], 2, 1, 64, 64, 0, 128),
+    ("f32", [25], [50], 3, 1, 128, 64, 0, 25),
+]
+
+
+@pytest.mark.parametrize("case", range(len(ATTENDS)))
+def test_attention_is_the_formula(case):
+    name, rows, keys, nq, nkv, d, P, window, most = ATTENDS[case]
+    k = kernels_for(name)
+    rng = np.random.default_rng(100 + case)
+    table, pages = tables(rng, keys, P)
+    cache = filled(rng, pages, nkv, P, d)
+    q = torch.from_numpy(rng.standard_normal((sum(rows), nq, d)) * 1.5).to(TYPES[name]).cuda()
+    got = attend(k, q, cache, table, rows, keys, most, window)
+    close(got, attention(host(q), *map(host, cache), table, np.concatenate([[0], np.cumsum(rows)]), keys, d ** -0.5, window), name, d)
+    # A larger bound changes nothing (the table is wider, the launch covers more keys).
+    wide = np.full((len(keys), table.shape[1] + 9), -1)
+    wide[:, :table.shape[1]] = table
+    assert torch.equal(got, attend(k, q, cache, wide, rows, keys, most, window, max_k_len=wide.shape[1] * P))
+
+
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("most", [6, 40])
+def test_nan_is_seen_where_it_is_visible_and_nowhere_else(name, most):
+    """NaN in keys that only later rows see, in keys before the window, behind the last key and in pages of nobody; in keys and in values."""
+    k, P, d, nkv, nq, window = kernels_for(name), 32, 64, 2, 4, 70
+    rng = np.random.default_rng(8)
+    rows, keys = [most, 3], [100 + most, 80]
+    table, pages = tables(rng, keys, P)
+    kc, vc, scales = filled(rng, pages, nkv, P, d)
+    nan = float("nan")
+    kf, vf = kc.float(), vc.float()
+    kf[table[0, 3], 0, (100 + most // 2) % P] = nan                 # seen by the rows from the middle one on (both fall in the fourth page)
+    vf[table[0, 3], 1, 5, (100 + most // 2) % P] = nan
+    kf[table[0, 0]] = nan                                           # keys 0..31: before every row's window
+    vf[table[0, 0]] = nan
+    vf[table[0, 1], 0, 9, 1] = nan                                  # key 33: seen by the first rows alone
+    last = keys[1] % P                                              # behind sequence 1's last key
+    kf[table[1, 2], :, last:] = nan
+    vf[table[1, 2], :, :, last:] = nan
+    kc, vc = kf.to(E4M3), vf.to(E4M3)
+    q = torch.from_numpy(rng.standard_normal((sum(rows), nq, d))).to(TYPES[name]).cuda()
+    got = attend(k, q, (kc, vc, scales), table, rows, keys, most, window)
+    plain = attention(host(q), host(kc), host(vc), host(scales), table, np.concatenate([[0], np.cumsum(rows)]), keys, d ** -0.5, window)
+    assert np.isnan(plain[0]).any() and not np.isnan(plain[0]).all(axis=(1, 2)).all()
+    close(got, plain, name, d)
+
+
+@pytest.mark.parametrize("most", [1, 20])
+def test_rows_without_keys_are_zero_and_rows_of_no_item_stay(most):
+    k, P, d = kernels_for("bf16"), 16, 64
+    rng = np.random.default_rng(9)
+    rows, keys = [most, most, most], [0, most + 30, most]
+    table, pages = tables(rng, [16, 64, 32], P)
+    table[2] = -1                                                   # pages of nothing: no keys
+    cache = filled(rng, pages, 2, P, d)
+    q = torch.from_numpy(rng.standard_normal((sum(rows) + 2, 4, d))).to(torch.bfloat16).cuda()
+    out = torch.full_like(q, 7.0)
+    cu = ints(np.concatenate([[0], np.cumsum(rows)]))
+    k.paged_attention8(q, *cache, ints(table), cu, ints(keys), ints([(0, 0), (1, 0), (2, 0), (3, 0), (-1, 0), (1, most), (1, -1)]), item_rows=most, scale=0.1, max_k_len=most + 30, out=out)
+    got = host(out)
+    assert (got[:most] == 0).all() and (got[2 * most:3 * most] == 0).all() and (got[3 * most:] == 7).all()
+    close(out[most:2 * most], attention(host(q[most:2 * most]), *map(host, cache), table[1:2], [0, most], keys[1:2], 0.1), "bf16", d)
+
+
+@pytest.mark.parametrize("name,most", [("bf16", 4), ("bf16", 30), ("f32", 4), ("f32", 30)])
+def test_pages_of_very_different_scales(name, most):
+    """Scales 2^-40 to 2^20 beside one another: values relative to their neighbours' lose what lies 2^-24 below the largest page's and less."""
+    k, P, d = kernels_for(name), 16, 64
+    rng = np.random.default_rng(11)
+    rows, keys = [most], [300]
+    table, pages = tables(rng, keys, P)
+    kc, vc, scales = filled(rng, pages, 1, P, d)
+    scales[:, :, 1] = torch.from_numpy(2.0 ** rng.integers(-40, 20, (pages, 1))).to(torch.float32)
+    q = torch.from_numpy(rng.standard_normal((most, 4, d))).to(TYPES[name]).cuda()
+    got = attend(k, q, (kc, vc, scales), table, rows, keys, most)
+    plain = attention(host(q), host(kc), host(vc), host(scales), table, [0, most], keys, d ** -0.5)
+    close(got, plain, name, d)
+
+
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+def test_a_row_is_the_same_bits_in_any_company(name):
+    """Few rows: whatever other sequences, items and bounds are in the call, and on every repetition."""
+    k, P, d, nq, nkv = kernels_for(name), 64, 128, 8, 2
+    rng = np.random.default_rng(12)
+    rows, keys = [3, 1, 3, 2], [1500, 90, 700, 2]
+    table, pages = tables(rng, keys, P)
+    cache = filled(rng, pages, nkv, P, d)
+    q = torch.from_numpy(rng.standard_normal((sum(rows), nq, d))).to(TYPES[name]).cuda()
+    got = attend(k, q, cache, table, rows, keys, 3)
+    assert torch.equal(got, attend(k, q, cache, table, rows, keys, 3))
+    at = 0
+    for s, n in enumerate(rows):
+        alone = attend(k, q[at:at + n].contiguous(), cache, table[s:s + 1], [n], keys[s:s + 1], 3, max_k_len=1500)
+        assert torch.equal(got[at:at + n], alone)
+        at += n
+
+
+def test_offsets_beyond_32_bits():
+    """Pages whose entries lie beyond 4 GiB, written and read."""
+    k, P, d, nkv = kernels_for("bf16"), 64, 128, 8
+    pages = 70000                                                   # 4.6 GB of keys, as much of values
+    kc, vc, scales = k.empty_cache8(pages, nkv, P, d)
+    rng = np.random.default_rng(13)
+    table = np.array([[pages - 1, 3, pages - 7]])
+    x = torch.from_numpy(rng.standard_normal((150, 3 * nkv * d))).to(torch.bfloat16).cuda()
+    q = k.qkv_post8(x, nq=nkv, nkv=nkv, d=d, k_cache=kc, v_cache=vc, scales=scales, q_w=None, k_w=None, eps=0.0, cos=None, sin=None, block_table=ints(table),
+                    cu_q=ints([0, 150]), k_len=ints([150]), max_k_len=150)
+    small = k.empty_cache8(10, nkv, P, d)
+    k.qkv_post8(x, nq=nkv, nkv=nkv, d=d, k_cache=small[0], v_cache=small[1], scales=small[2], q_w=None, k_w=None, eps=0.0, cos=None, sin=None,
+                block_table=ints([[9, 3, 5]]), cu_q=ints([0, 150]), k_len=ints([150]), max_k_len=150)
+    for big, little in zip((kc, vc, scales), small):
+        for a, b in ((pages - 1, 9), (3, 3), (pages - 7, 5)):
+            assert np.array_equal(host(big[a]), host(little[b]))
+    for most in (16, 128):
+        assert torch.equal(attend(k, q, (kc, vc, scales), table, [150], [150], most), attend(k, q, small, [[9, 3, 5]], [150], [150], most))
+
+
+def test_refusals():
+    k = kernels_for("bf16")
+    kc, vc, sc = k.empty_cache8(4, 2, 16, 64)
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(3, 8 * 64, dtype=torch.bfloat16, device="cuda")
+    table, cu, kl, it = ints([[0, 1]]), ints([0, 3]), ints([3]), ints([[0, 0]])
+
+    def att(q=q, kc=kc, vc=vc, sc=sc, table=table, cu=cu, kl=kl, it=it, **kw):
+        return k.paged_attention8(q, kc, vc, sc, table, cu, kl, it, **{**dict(item_rows=3, scale=0.1, max_k_len=32), **kw})
+
+    def put(x=x, **kw):
+        return k.qkv_post8(x, **{**dict(nq=4, nkv=2, d=64, k_cache=kc, v_cache=vc, scales=sc, q_w=None, k_w=None, eps=0.0, cos=None, sin=None, block_table=table, cu_q=cu,
+                                        k_len=kl, max_k_len=32), **kw})
+    att(), put()
+    for bad in (dict(q=q.float()), dict(q=q[:, :, :32]), dict(q=q.cpu()), dict(q=q[:, :3].contiguous()), dict(kc=kc.float()), dict(vc=kc), dict(sc=sc[:, :1]), dict(table=table.long()),
+                dict(cu=ints([0])), dict(kl=ints([3, 3])), dict(it=ints([0, 0])), dict(item_rows=0), dict(item_rows=129), dict(window=-1), dict(max_k_len=33),
+                dict(out=q[:2]), dict(max_k_len=-1)):
+        with pytest.raises(KernelError):
+            att(**bad)
+    small = k.empty_cache8(4, 2, 8, 64), k.empty_cache8(2, 2, 512, 64), k.empty_cache8(2, 2, 48, 64)
+    for c in small:
+        with pytest.raises(KernelError):
+            att(kc=c[0], vc=c[1], sc=c[2])
+        with pytest.raises(KernelError):
+            put(k_cache=c[0], v_cache=c[1], scales=c[2])
+    with pytest.raises(KernelError):                                # scratch too small
+        att(table=ints([list(range(4)) * 10]), max_k_len=600, scratch=torch.empty(8, device="cuda"))
+    cos = torch.zeros(32, 32, dtype=torch.bfloat16, device="cuda")
+    put(cos=cos, sin=cos)
+    for bad in (dict(x=x[:, 1:]), dict(x=x.float()), dict(x=x.t()), dict(nq=3), dict(d=24, x=x[:, :192].contiguous()), dict(cos=cos[:31], sin=cos[:31]), dict(cos=cos, sin=cos.float()),
+                dict(cos=torch.zeros(32, 33, dtype=torch.bfloat16, device="cuda"), sin=torch.zeros(32, 33, dtype=torch.bfloat16, device="cuda")), dict(q_w=x[0, :32]),
+                dict(q_w=x[0, :64].contiguous(), k_w=torch.zeros(64, device="cuda")), dict(max_k_len=33), dict(q_out=q[:2]), dict(k_cache=vc), dict(scales=sc.double())):
+        with pytest.raises(KernelError):
+            put(**bad)
+    unaligned = torch.zeros(3 * 512 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(3, 512)
+    with pytest.raises(KernelError):
+        put(x=unaligned)

@@ -9,15 +9,17 @@ All launches go to torch's current stream.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_int64, c_uint64, c_void_p
+from ctypes import c_double, c_float, c_int, c_int64, c_uint64, c_void_p
 
 import torch
 
 from . import build
 
-ABI_VERSION = 20
+ABI_VERSION = 21
 SEGMENT_KEYS = 256
-ATTN_ITEM_ROWS = 128      # rows of one prompt item of paged_attention
+ATTN_ITEM_ROWS = 128      # rows of one prompt item of paged_attention, and of any item of paged_attention8
+CACHE8_DTYPE = torch.float8_e4m3fn
+CACHE8_PAGES = (16, 256)  # smallest and largest page of an 8-bit cache
 
 _DTYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
 _NAMES = {torch.bfloat16: "bf16", torch.float32: "f32", "bfloat16": "bf16", "float32": "f32", "bf16": "bf16",
@@ -83,6 +85,13 @@ class Kernels:
         lib.vk_attn_segment_keys.restype = c_int
         assert lib.vk_attn_segment_keys() == SEGMENT_KEYS
         lib.vk_attn_item_rows.restype = c_int
+        _sig(lib.vk_qkv_post8, P, L, P, P, P, P, P, P, I, P, P, I, P, I, P, P, I, I, I, I, I, I, I, I, c_double, P)
+        _sig(lib.vk_paged_attention8, P, P, P, P, P, P, I, P, P, P, I, I, P, L, I, I, I, I, I, I, I, I, I, F, P)
+        lib.vk_attn8_scratch_floats.argtypes = [I, I, I, I, I]
+        lib.vk_attn8_scratch_floats.restype = c_int64
+        _sig(lib.vk_verify, P, P, P, P, P, P, P, P, P, P, P, L, I, I, I, I, P)
+        lib.vk_verify_scratch_bytes.argtypes = [I, I, I, I]
+        lib.vk_verify_scratch_bytes.restype = c_int64
         assert lib.vk_attn_item_rows() == ATTN_ITEM_ROWS
         self.lib = lib
 
@@ -379,6 +388,147 @@ class Kernels:
         self._call(self.lib.vk_sample, out.data_ptr(), logits.data_ptr(), tp, up, scratch.data_ptr(), R, V, V,
                    self._stream())
         return out
+
+    # ------------------------------------------------ caches of 8 bits, drafted tokens
+    def _here(self, *tensors) -> None:
+        """The launch goes to the current device: what lies on another one is refused."""
+        here = torch.cuda.current_device()
+        for t in tensors:
+            if t is not None and t.device.index != here:
+                raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{here}")
+
+    def empty_cache8(self, pages: int, nkv: int, page_size: int, d: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Keys [pages, nkv, page_size, d], values [pages, nkv, d, page_size] (both e4m3) and scales [pages, nkv, 2] of an empty 8-bit cache."""
+        return (torch.zeros(pages, nkv, page_size, d, dtype=CACHE8_DTYPE, device="cuda"),
+                torch.zeros(pages, nkv, d, page_size, dtype=CACHE8_DTYPE, device="cuda"),
+                torch.zeros(pages, nkv, 2, dtype=torch.float32, device="cuda"))
+
+    def _cache8(self, k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, nkv: int, d: int) -> tuple[int, int]:
+        """Checks the three tensors; returns (pages, page size)."""
+        self._check(k_cache, "k cache", CACHE8_DTYPE)
+        if k_cache.dim() != 4 or k_cache.shape[1] != nkv or k_cache.shape[3] != d:
+            raise KernelError(f"k cache has shape {tuple(k_cache.shape)}, expected [pages, {nkv}, page size, {d}]")
+        pages, _, P, _ = k_cache.shape
+        if P & (P - 1) or not CACHE8_PAGES[0] <= P <= CACHE8_PAGES[1]:
+            raise KernelError(f"page size {P} of an 8-bit cache is no power of two from {CACHE8_PAGES[0]} to {CACHE8_PAGES[1]}")
+        self._check(v_cache, "v cache", CACHE8_DTYPE, (pages, nkv, d, P))
+        self._check(scales, "scales", torch.float32, (pages, nkv, 2))
+        return pages, P
+
+    def qkv_post8(self, qkv: torch.Tensor, *, nq: int, nkv: int, d: int, k_cache: torch.Tensor | None, v_cache: torch.Tensor | None,
+                  scales: torch.Tensor | None, q_w: torch.Tensor | None, k_w: torch.Tensor | None, eps: float, cos: torch.Tensor | None,
+                  sin: torch.Tensor | None, block_table: torch.Tensor, cu_q: torch.Tensor, k_len: torch.Tensor, max_k_len: int,
+                  q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+        """``qkv_post`` for an 8-bit cache: head norm, rotation and append of a [T, (nq + 2 nkv) d] row tensor (see store8.hip).
+
+        Rows of sequence s are cu_q[s] .. cu_q[s + 1] - 1 and stand at the places before k_len[s] (its keys with them) in the pages of
+        block_table[s]; a page number outside the cache keeps nothing.  ``qkv`` may be a view of rows with a row stride that is a whole number of
+        16-byte vectors.  A page's scales grow with its entries and start anew when a call writes its first place; a page that two sequences of a call write
+        to is undefined.  ``max_k_len``: the host's bound on k_len, which tables and block tables cover; a sequence beyond it is left out.  Rows behind the
+        last sequence's are left as they were."""
+        if qkv.dim() != 2 or nq < 0 or nkv < 0 or qkv.shape[1] != (nq + 2 * nkv) * d:
+            raise KernelError(f"qkv_post8: row tensor {tuple(qkv.shape)} is not [T, (nq + 2 nkv) * d = {(nq + 2 * nkv) * d}]")
+        T, W = qkv.shape
+        if not qkv.is_cuda or qkv.dtype != self.dtype or (W and qkv.stride(1) != 1):
+            raise KernelError("qkv_post8: rows must be a GPU tensor of the element type with a contiguous last axis")
+        if nq:
+            q_out = self.empty(T, nq, d) if q_out is None else q_out
+            self._elem(q_out, "q_out", T, nq, d)
+        wf = 0
+        qwp = kwp = None
+        if q_w is not None:
+            qwp, wf = self._weight(q_w, "q norm weight", d)
+        if k_w is not None:
+            kwp, wf2 = self._weight(k_w, "k norm weight", d)
+            if q_w is not None and wf2 != wf:
+                raise KernelError("qkv_post8: q and k norm weights must have the same type")
+            wf = wf2
+        cp = sp = None
+        half = 0
+        if cos is not None:
+            if cos.dim() != 2 or cos.shape[0] < max_k_len:
+                raise KernelError(f"qkv_post8: tables {tuple(cos.shape)} do not cover {max_k_len} places")
+            half = cos.shape[1]
+            cp, sp = self._elem(cos, "cos", *cos.shape), self._elem(sin, "sin", *cos.shape)
+        S, width = block_table.shape
+        tp = self._i32(block_table, "block table", S, width)
+        cup, klp = self._i32(cu_q, "cu_q", S + 1), self._i32(k_len, "k_len", S)
+        pages, P, kcp, vcp, scp = 0, 0, None, None, None
+        if nkv:
+            pages, P = self._cache8(k_cache, v_cache, scales, nkv, d)
+            kcp, vcp, scp = k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr()
+        self._here(qkv, q_out if nq else None, k_cache, v_cache, scales, q_w, k_w, cos, sin, block_table, cu_q, k_len)
+        self._call(self.lib.vk_qkv_post8, qkv.data_ptr(), qkv.stride(0) if T > 1 else W, q_out.data_ptr() if nq else None, kcp, vcp, scp, qwp, kwp, wf, cp, sp,
+                   half, tp, width, cup, klp, T, S, nq, nkv, d, P, pages, max_k_len, float(eps), self._stream())
+        return q_out if nq else None
+
+    def attn8_scratch_floats(self, items: int, item_rows: int, nq: int, d: int, max_k_len: int) -> int:
+        """float32 elements of scratch that ``paged_attention8`` needs for ``items`` items of up to ``item_rows`` rows."""
+        return int(self.lib.vk_attn8_scratch_floats(items, item_rows, nq, d, max_k_len))
+
+    def paged_attention8(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor,
+                         block_table: torch.Tensor, cu_q: torch.Tensor, k_len: torch.Tensor, items: torch.Tensor,
+                         *, item_rows: int, scale: float, window: int = 0, max_k_len: int, scratch: torch.Tensor | None = None,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the rows named by ``items`` over an 8-bit cache (see attention8.hip).
+
+        items [n, 2] = (sequence, first row): an item is up to ``item_rows`` consecutive rows of its sequence, at most ATTN_ITEM_ROWS.  Items of up
+        to 16 rows (decoded tokens, drafted ones) have their keys split over workgroups, whose sums meet in ``scratch`` (``attn8_scratch_floats``;
+        without it the call takes memory of its own); larger ones are for prompts.  ``max_k_len`` is the host's bound on k_len; the block table must
+        cover it, and keys beyond it may be left out.  Rows that no item names are left as they were."""
+        if q.dim() != 3 or k_cache.dim() != 4:
+            raise KernelError(f"attention8: q {tuple(q.shape)} is not [T, heads, size], or the k cache {tuple(k_cache.shape)} not [pages, kv heads, page size, size]")
+        T, nq, d = q.shape
+        nkv = k_cache.shape[1]
+        self._elem(q, "q", T, nq, d)
+        pages, P = self._cache8(k_cache, v_cache, scales, nkv, d)
+        S, W = block_table.shape
+        tp = self._i32(block_table, "block table", S, W)
+        cup, klp = self._i32(cu_q, "cu_q", S + 1), self._i32(k_len, "k_len", S)
+        n_items = items.shape[0]
+        ip = self._i32(items, "items", n_items, 2)
+        out = torch.empty_like(q) if out is None else out
+        self._elem(out, "out", T, nq, d)
+        need = self.attn8_scratch_floats(n_items, item_rows, nq, d, max_k_len)
+        if need and scratch is None:
+            scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+        self._here(q, k_cache, v_cache, scales, block_table, cu_q, k_len, items, scratch, out)
+        self._call(self.lib.vk_paged_attention8, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), tp, W, cup, klp, ip,
+                   n_items, item_rows, self._f32(scratch, "scratch") if need else None, scratch.numel() if need else 0, T, S, nq, nkv, d, P, pages, max_k_len,
+                   int(window), float(scale), self._stream())
+        return out
+
+    def verify(self, logits: torch.Tensor, draft_ids: torch.Tensor, cu: torch.Tensor, *, draft_logits: torch.Tensor | None = None,
+               temps: torch.Tensor | None = None, accept_uniforms: torch.Tensor | None = None,
+               draw_uniforms: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Which drafted tokens stand against the target's logits, and the token behind them (see verify.hip).
+
+        logits [R, V]: rows cu[s] .. cu[s + 1] - 1 are sequence s's, one more than its drafted tokens; draft_ids [D] are those of all sequences one after
+        the other.  ``draft_logits`` [D, V]: the draft model's, without them a draft is certain.  ``temps`` [S] for both models (without them, and at 0, the
+        maximum alone), with random numbers in [0, 1): ``accept_uniforms`` [D] and ``draw_uniforms`` [S].
+
+        Returns (tokens [R], counts [S], accept [D]): sequence s's rows of ``tokens`` begin with counts[s] tokens (the standing ones and the drawn one) and go on
+        with -1; ``accept`` is min(1, p / q) of every drafted token.  What lies behind the last sequence is not written."""
+        if logits.dim() != 2 or draft_ids.dim() != 1 or cu.dim() != 1 or cu.shape[0] < 1:
+            raise KernelError(f"verify: logits {tuple(logits.shape)}, draft ids {tuple(draft_ids.shape)} and cu {tuple(cu.shape)} are not [R, V], [D], [S + 1]")
+        R, V = logits.shape
+        D, S = draft_ids.shape[0], cu.shape[0] - 1
+        lp, ip, cup = self._elem(logits, "logits", R, V), self._i32(draft_ids, "draft ids", D), self._i32(cu, "cu", S + 1)
+        dp = self._elem(draft_logits, "draft logits", D, V) if draft_logits is not None else None
+        tp = ap = up = None
+        if temps is not None:
+            if accept_uniforms is None or draw_uniforms is None:
+                raise KernelError("verify: temperatures need random numbers")
+            tp, ap, up = self._f32(temps, "temps", S), self._f32(accept_uniforms, "accept uniforms", D), self._f32(draw_uniforms, "draw uniforms", S)
+        self._here(logits, draft_ids, cu, draft_logits, temps, accept_uniforms, draw_uniforms)
+        tokens = torch.empty(R, dtype=torch.int32, device=logits.device)
+        counts = torch.empty(S, dtype=torch.int32, device=logits.device)
+        accept = torch.empty(D, dtype=torch.float32, device=logits.device)
+        need = int(self.lib.vk_verify_scratch_bytes(R, D, S, V))
+        scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        self._call(self.lib.vk_verify, tokens.data_ptr(), counts.data_ptr(), accept.data_ptr(), lp, ip, cup, dp, tp, ap, up, scratch.data_ptr(), need, R, D, S, V,
+                   self._stream())
+        return tokens, counts, accept
 
 
 _CACHE: dict[str, Kernels] = {}
