@@ -34,12 +34,12 @@ def test_append_refuses(kernels, bad):
     assert "qkv_post8" in refused(kernels, *put(kernels, **bad))
 
 
-def att(kernels, out=GOOD, q=GOOD, W=4, n=2, rows=3, scratch=None, floats=0, T=3, S=1, nq=4, nkv=2, d=64, P=16, pages=4, max_k_len=32, window=0):
-    return (kernels.lib.vk_paged_attention8, out, q, GOOD, GOOD, GOOD, GOOD, W, GOOD, GOOD, GOOD, n, rows, scratch, floats, T, S, nq, nkv, d, P, pages, max_k_len, window, 0.125, None)
+def att(kernels, out=GOOD, q=GOOD, W=4, n=2, rows=3, scratch=None, floats=0, T=3, S=1, nq=4, nkv=2, d=64, P=16, pages=4, max_k_len=32, window=0, scale=0.125):
+    return (kernels.lib.vk_paged_attention8, out, q, GOOD, GOOD, GOOD, GOOD, W, GOOD, GOOD, GOOD, n, rows, scratch, floats, T, S, nq, nkv, d, P, pages, max_k_len, window, scale, None)
 
 
 @pytest.mark.parametrize("bad", [dict(T=-1), dict(n=-1), dict(nq=3), dict(nkv=0), dict(d=8), dict(d=100), dict(d=288), dict(P=8), dict(P=24), dict(P=1024), dict(rows=0), dict(rows=129),
-                                 dict(pages=0), dict(W=0), dict(max_k_len=65), dict(max_k_len=-1), dict(window=-1), dict(q=GOOD + 4), dict(out=GOOD + 8),
+                                 dict(pages=0), dict(W=0), dict(max_k_len=65), dict(max_k_len=-1), dict(window=-1), dict(scale=0.0), dict(scale=-0.1), dict(scale=math.nan), dict(scale=math.inf), dict(q=GOOD + 4), dict(out=GOOD + 8),
                                  dict(W=64, max_k_len=1000), dict(W=64, max_k_len=1000, scratch=GOOD, floats=100), dict(W=64, max_k_len=1000, scratch=GOOD + 4, floats=1 << 20),
                                  dict(W=2 ** 30, P=16, max_k_len=32)])
 def test_attention_refuses(kernels, bad):
@@ -48,9 +48,9 @@ def test_attention_refuses(kernels, bad):
 
 def test_scratch_of_attention(kernels):
     f = kernels.attn8_scratch_floats
-    assert f(5, 17, 32, 128, 100000) == 0 and f(5, 4, 32, 128, 256) == 0 and f(0, 1, 32, 128, 5000) == 0
-    assert f(5, 4, 32, 128, 257) == 5 * 4 * 32 * 2 * 130
-    assert f(512, 16, 128, 256, 1 << 20) == 512 * 16 * 128 * 4096 * 258          # beyond 32 bits
+    assert f(5, 17, 32, 128, 100000) == 0 and f(5, 4, 32, 128, 512) == 0 and f(0, 1, 32, 128, 5000) == 0
+    assert f(5, 4, 32, 128, 513) == 5 * 4 * 32 * 2 * 130
+    assert f(512, 16, 128, 256, 1 << 20) == 512 * 16 * 128 * 2048 * 258          # beyond 32 bits
 
 
 def ver(kernels, tokens=GOOD, logits=GOOD, ids=GOOD, temps=None, au=None, du=None, scratch=GOOD, size=1 << 30, R=3, D=2, S=1, V=100):

@@ -20,8 +20,9 @@
 #include "vec.h"
 
 #define A8_TILE 64
-#define A8_SEG_TILES 4           // tiles of a segment: what a workgroup of the few rows' kernel takes, a tile a wave
-#define A8_SEG (A8_TILE * A8_SEG_TILES)
+#define A8_SEG 512               // keys that are summed up apart where a row's keys are split over workgroups
+#define A8_STEP 8.0f             // a column's reference maximum moves where the tile's exceeds it by more (log2)
+#define A8_STAGES 3              // tiles in LDS: one is computed, the next has arrived or is arriving, one is being asked for
 #define A8_ITEM_ROWS 128         // rows of an item, at most
 
 struct A8Args {
@@ -31,7 +32,7 @@ struct A8Args {
   const float* scales;
   const int32_t *table, *cu_q, *k_len, *items;
   float *part_ml, *part_acc;   // per (item, kv head, segment, column): maximum and sum; d sums
-  int W, T, S, nq, nkv, d, P, lp, pages, group, item_rows, cols_max, window, nseg;
+  int W, T, S, nq, nkv, d, P, lp, pages, group, item_rows, cols_max, window, nseg, n_items;
   float scale_log2;
 };
 
@@ -177,305 +178,519 @@ __device__ __forceinline__ void a8_load_q(const A8Args& a, const A8Rows<NT>& c, 
   }
 }
 
-// The page of the 16 keys from `key` on, and whether any of them is there for the wave; a page number outside the cache is no page.
-template <int NT>
-__device__ __forceinline__ int a8_page(const A8Args& a, const A8Rows<NT>& c, int key, bool& there) {
-  there = key <= c.wave_pos && key + 15 >= c.wave_lo && key < a.W << a.lp;
-  const int page = there ? a.table[(int64_t)c.seq * a.W + (key >> a.lp)] : 0;
-  there = there && (unsigned)page < (unsigned)a.pages;
-  return there ? page : 0;
-}
-
-// What a wave reads of a tile, and the scales that go with it.
-template <int DP>
-struct A8Tile {
-  u32x4 k[4][DP / 64], v[DP / 16];
-  float k_scale;             // of the keys that the lane reads
-  int v_exp;                 // of the 16 keys whose values it reads, -256: none of them is there
-};
-
-template <int DP, int NT>
-__device__ __forceinline__ void a8_load(const A8Args& a, const A8Rows<NT>& c, int kb, A8Tile<DP>& t) {
-  bool k_there, v_there;
-  const int kkey = kb + 16 * (c.r >> 2), vkey = kb + 16 * c.g;
-  const int64_t kblock = (int64_t)a8_page(a, c, kkey, k_there) * a.nkv + c.kvh, vblock = (int64_t)a8_page(a, c, vkey, v_there) * a.nkv + c.kvh;
-  const float ks = a.scales[2 * kblock], vs = a.scales[2 * vblock + 1];
-  t.k_scale = k_there ? ks : 1.f;
-  t.v_exp = v_there ? exponent_of(vs) : -256;
-  const uint8_t* kp = a.kc + (kblock * a.P + (kkey & (a.P - 1)) + (c.r & 3)) * a.d + 16 * c.g;
-#pragma unroll
-  for (int s = 0; s < 4; ++s)
-#pragma unroll
-    for (int j = 0; j < DP / 64; ++j)
-      t.k[s][j] = 64 * j + 16 * c.g < a.d ? *reinterpret_cast<const u32x4*>(kp + 4 * s * a.d + 64 * j) : u32x4{0, 0, 0, 0};
-  const uint8_t* vp = a.vc + (vblock * a.d + c.r) * a.P + (vkey & (a.P - 1));
-#pragma unroll
-  for (int dt = 0; dt < DP / 16; ++dt)
-    if (16 * dt < a.d) t.v[dt] = *reinterpret_cast<const u32x4*>(vp + (int64_t)16 * dt * a.P);
-}
-
 // Bytes of four that hold a NaN, as 0x01 each.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u; }
 
-// One tile onto the wave's sums: m, l and acc of a column, acc in units of 2^unit (the same for the wave).  full: every column that stands for a row sees every key.
+// A column's sums: m its reference maximum, l the sum of its weights, acc those of weights times values in units of 2^unit (the same for the wave).
 template <int DP, int NT>
-__device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, int kb, A8Tile<DP>& t, const q_part (&q)[DP / 64][NT][A8_QJ], float (&m)[NT],
-                                        float (&l)[NT], f32x4 (&acc)[NT][DP / 16], int& unit) {
-  const bool full = kb >= c.all_lo && kb + A8_TILE - 1 <= c.all_pos && __all(t.v_exp > -256);
+struct A8Sums {
+  float m[NT], l[NT];
+  f32x4 acc[NT][DP / 16];
+  int unit;
+  __device__ __forceinline__ void clear() {
+    unit = -256;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt) acc[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  __device__ __forceinline__ float scale() const {
+#ifdef VK_BF16
+    return unit > -256 ? pow2f(unit) : 1.f;
+#else
+    return 1.f;
+#endif
+  }
+};
+
+// One tile onto the wave's sums.  src.k(i, j) and src.v(dt): the lane's 16 bytes of K's tile i and of V's entries 16 dt + r; src.k_done() and src.v_done(): they are not asked
+// for again.  k_scale: of the keys whose K the lane reads; v_exp: of the 16 keys whose V it reads, -256: none of them is there.
+//
+// A column's reference maximum follows its maximum only where that is more than 2^8 above: weights are 2^8 at most then (their sums are 32-bit, and 2^8 is nothing to
+// sixteen bits), and the sums are scaled in few tiles.  Which columns move is each column's own business; whether any does is the wave's.
+template <int DP, int NT, typename SRC>
+__device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, int kb, SRC&& src, float k_scale, int v_exp, const q_part (&q)[DP / 64][NT][A8_QJ],
+                                        A8Sums<DP, NT>& o) {
+  const bool there = v_exp > -256;
+  // full: every column that stands for a row sees every key.
+  const bool full = kb >= c.all_lo && kb + A8_TILE - 1 <= c.all_pos && __all(there);
+  // What a product reads is asked for one product ahead, and not further: the scheduler would take all of a tile first, and spill.
   f32x4 s[4][NT];
+  u32x4 next[DP / 64];
+#pragma unroll
+  for (int j = 0; j < DP / 64; ++j) next[j] = src.k(0, j);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    u32x4 k[DP / 64];
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j) {
+      k[j] = next[j];
+      if (i < 3) next[j] = src.k(i + 1, j);
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j) keys_times<NT>(t.k[i][j], t.k_scale, q[j], s[i]);
+    for (int j = 0; j < DP / 64; ++j) keys_times<NT>(k[j], k_scale, q[j], s[i]);
+    asm volatile("" ::: "memory");
+  }
+  src.k_done();
+  const int first = kb + 16 * c.g;
+  float m_tile[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float top = -INFINITY;
+    if (full) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) top = fmaxf(top, s[x / 4][n][x % 4]);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const float v = there && first + x >= c.lo[n] && first + x <= c.pos[n] ? s[x / 4][n][x % 4] : -INFINITY;
+        s[x / 4][n][x % 4] = v;
+        top = fmaxf(top, v);
+      }
+    }
+    m_tile[n] = over_groups_max(top) * a.scale_log2;
+  }
+  bool moves = false;
+  float by[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const bool move = m_tile[n] > o.m[n] + A8_STEP || (o.m[n] == -INFINITY && m_tile[n] > -INFINITY);
+    const float to = move ? m_tile[n] : o.m[n];
+    by[n] = move ? exp2_fast(o.m[n] - to) : 1.f;
+    o.m[n] = to;
+    moves = moves || move;
   }
 #ifdef VK_BF16
   // The unit never falls, so that sums are scaled down only: what a smaller page adds is then in units of a larger one's.
-  float top = over_groups_max((float)t.v_exp);
-  const int unit_now = max(unit, (int)top);
-  const float to_unit = unit_now == unit ? 1.f : unit - unit_now < -126 ? 0.f : pow2f(unit - unit_now);
-  unit = unit_now;
-  const float v_scale = pow2f(max(-126, t.v_exp - unit));
+  const int unit = max(o.unit, __builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp)));
+  const float to_unit = o.unit - unit < -126 ? 0.f : pow2f(o.unit - unit), v_scale = pow2f(max(-126, v_exp - unit));
+  moves = moves || unit != o.unit;
+  o.unit = unit;
 #else
-  const float to_unit = 1.f, v_scale = t.v_exp > -256 ? pow2f(t.v_exp) : 1.f;
+  const float to_unit = 1.f, v_scale = there ? pow2f(v_exp) : 1.f;
 #endif
-  const bool there = t.v_exp > -256;
-  w_part w[NT][A8_WP], seen[NT][A8_WP];
+  if (__any(moves)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      o.l[n] = o.l[n] * by[n];
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt) o.acc[n][dt] = o.acc[n][dt] * (by[n] * to_unit);
+    }
+  }
+  w_part w[NT][A8_WP];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    float p[16], top_s = -INFINITY;
-    const int first = kb + 16 * c.g;
+    const float ref = o.m[n] > -INFINITY ? o.m[n] : 0.f;      // a column that has seen no key: its scores are -infinity, its weights 0
+    float p[16], sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
-      const bool vis = full || (there && first + x >= c.lo[n] && first + x <= c.pos[n]);
-      p[x] = vis ? s[x / 4][n][x % 4] : -INFINITY;
-      top_s = fmaxf(top_s, p[x]);
-    }
-    const float m_new = fmaxf(m[n], over_groups_max(top_s) * a.scale_log2), ref = m_new > -INFINITY ? m_new : 0.f;
-    const float by = exp2_fast(m[n] - ref);
-    float sum = 0.f, ones[16];
-#pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      const bool vis = full || (there && first + x >= c.lo[n] && first + x <= c.pos[n]);
-      ones[x] = vis ? 1.f : 0.f;
-      p[x] = vis ? exp2_fast(__builtin_fmaf(p[x], a.scale_log2, -ref)) : 0.f;
+      p[x] = exp2_fast(__builtin_fmaf(s[x / 4][n][x % 4], a.scale_log2, -ref));
       sum = sum + p[x];
     }
-    l[n] = __builtin_fmaf(l[n], by, over_groups_sum(sum));
-    m[n] = m_new;
+    o.l[n] = o.l[n] + sum;                                     // this lane's keys alone: joined where the sums are used
     set_weights(p, w[n]);
-    set_weights(ones, seen[n]);
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) acc[n][dt] = acc[n][dt] * (by * to_unit);
   }
-  bool nan = false;
+  // Values that no column sees are taken out; so are NaN, which some may not see: those that do get it back through a product of ones.
+  uint32_t keep[4] = {0, 0, 0, 0}, nans = 0;
   if (!full) {
-    // Values that no column sees are taken out; so are NaN, which some may not see.
-    uint32_t keep[4];
-    const int from = c.wave_lo - (kb + 16 * c.g), to = c.wave_pos - (kb + 16 * c.g);
+    const int from = c.wave_lo - first, to = c.wave_pos - first;
 #pragma unroll
-    for (int b = 0; b < 16; ++b) {
-      const uint32_t one = there && b >= from && b <= to ? 0xffu << 8 * (b & 3) : 0u;
-      keep[b / 4] = b % 4 == 0 ? one : keep[b / 4] | one;
-    }
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt)
-      if (16 * dt < a.d) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          t.v[dt][b] &= keep[b];
-          nan = nan || nan_bytes(t.v[dt][b]) != 0;
-        }
-      }
-    nan = __any(nan);
+    for (int b = 0; b < 16; ++b) keep[b / 4] |= there && b >= from && b <= to ? 0xffu << 8 * (b & 3) : 0u;
   }
+  u32x4 ahead = src.v(0);
 #pragma unroll
   for (int dt = 0; dt < DP / 16; ++dt) {
-    if (16 * dt >= a.d) continue;
-    f32x4 o[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) o[n] = acc[n][dt];
-    if (nan) {
-      u32x4 where, clean;
-      f32x4 count[NT];
+    u32x4 v = ahead;
+    if (dt + 1 < DP / 16) ahead = src.v(dt + 1);
+    if (!full) {
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const uint32_t x = nan_bytes(t.v[dt][b]);
-        where[b] = x * 0x38u;                         // 1 in e4m3
-        clean[b] = t.v[dt][b] & ~(x * 0xffu);
+        const uint32_t x = v[b] & keep[b], where = nan_bytes(x);
+        nans |= where;
+        v[b] = x & ~(where * 0xffu);
       }
+    }
+    f32x4 x[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x[n] = o.acc[n][dt];
+    values_times<NT>(v, v_scale, w, x);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o.acc[n][dt] = x[n];
+    asm volatile("" ::: "memory");
+  }
+  if (__any(nans != 0)) {
+    w_part seen[NT][A8_WP];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float one[16];
+#pragma unroll
+      for (int y = 0; y < 16; ++y) one[y] = there && first + y >= c.lo[n] && first + y <= c.pos[n] ? 1.f : 0.f;
+      set_weights(one, seen[n]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) {
+      u32x4 v = src.v(dt);
+      f32x4 count[NT];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) v[b] = nan_bytes(v[b] & keep[b]) * 0x38u;     // 1 in e4m3
 #pragma unroll
       for (int n = 0; n < NT; ++n) count[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-      values_times<NT>(where, 1.f, seen, count);
-      values_times<NT>(clean, v_scale, w, o);
+      values_times<NT>(v, 1.f, seen, count);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] = count[n][i] > 0.f ? NAN : o[n][i];
-    } else {
-      values_times<NT>(t.v[dt], v_scale, w, o);
+        for (int i = 0; i < 4; ++i) o.acc[n][dt][i] = o.acc[n][dt][i] + (count[n][i] > 0.f ? NAN : 0.f);
+      asm volatile("" ::: "memory");
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n][dt] = o[n];
   }
+  src.v_done();
 }
 
-__device__ __forceinline__ float unit_of(int unit) {
-#ifdef VK_BF16
-  return unit > -256 ? pow2f(unit) : 1.f;
-#else
-  return 1.f;
-#endif
+// Where a column's result goes, from its first entry 4 g on.
+template <int NT>
+__device__ __forceinline__ elem_t* a8_out(const A8Args& a, const A8Rows<NT>& c, int col) {
+  const int row = col / a.group;
+  return a.out + ((int64_t)(c.tok0 + row) * a.nq + c.kvh * a.group + col - row * a.group) * a.d + 4 * c.g;
 }
 
-// ---- prompts: a wave takes 16 NT columns of an item through all their keys.
-template <int DP, int NT>
-__global__ __launch_bounds__(256) void a8_prompt_kernel(A8Args a, int blocks_y) {
-  A8Rows<NT> c;
-  const int kvh = blockIdx.y % a.nkv, block = blockIdx.y / a.nkv, wave = threadIdx.x >> 6;
-  if (!a8_rows<NT>(a, blockIdx.x, kvh, (block * 4 + wave) * 16 * NT, c)) return;
-  q_part q[DP / 64][NT][A8_QJ];
-  a8_load_q<DP, NT>(a, c, q);
-  float m[NT], l[NT];
-  f32x4 acc[NT][DP / 16];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) acc[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  int unit = -256;
-  A8Tile<DP> t;
-  for (int kb = c.wave_lo & ~(A8_TILE - 1); kb <= c.wave_pos; kb += A8_TILE) {
-    a8_load<DP, NT>(a, c, kb, t);
-    a8_tile<DP, NT>(a, c, kb, t, q, m, l, acc, unit);
-  }
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int col = c.col0 + 16 * n + c.r;
-    if (col >= c.cols) continue;
-    const int row = col / a.group;
-    elem_t* o = a.out + ((int64_t)(c.tok0 + row) * a.nq + kvh * a.group + col - row * a.group) * a.d + 4 * c.g;
-    const float by = l[n] == 0.f ? 0.f : 1.f / l[n], u = unit_of(unit);
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt)
-      if (16 * dt < a.d) store_elems4(o + 16 * dt, l[n] == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[n][dt] * by * u);
-  }
-}
-
-// ---- few rows: a workgroup takes 16 NT columns through a segment of 256 keys, a wave a tile; segments are joined by a8_join_kernel.
-// The segments that columns col0 .. have keys in; one that has none at all counts the first.
+// Segments: what is summed up apart where a row's keys are split over workgroups.  Those in which the columns of a block have keys; a block that has none at all
+// counts the first.
 __device__ __forceinline__ void a8_segments(int lo, int pos, int& first, int& last) {
   last = max(pos, 0) / A8_SEG;
   first = min(lo / A8_SEG, last);
 }
 
-template <int DP, int NT>
-__global__ __launch_bounds__(256) void a8_few_kernel(A8Args a) {
-  extern __shared__ float sums[];                       // [4 waves][DP / 16][64 lanes][4]
-  __shared__ float maxima[4][16 * NT], totals[4][16 * NT];
-  A8Rows<NT> c;
-  const int kvh = blockIdx.y % a.nkv, block = blockIdx.y / a.nkv, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, seg = blockIdx.z;
-  if (!a8_rows<NT>(a, blockIdx.x, kvh, block * 16 * NT, c)) return;
+// The pages that a workgroup walks, 64 at a time: lane l has number `base + l` of the sequence's.
+struct A8Pages {
+  int base, page;
+  float k_scale;
+  int v_exp;
+  template <int NT>
+  __device__ __forceinline__ void fill(const A8Args& a, const A8Rows<NT>& c, int at, int pos) {
+    base = at;
+    const int i = at + (threadIdx.x & 63);
+    page = i < a.W && i <= pos >> a.lp ? a.table[(int64_t)c.seq * a.W + i] : -1;
+    const bool there = (unsigned)page < (unsigned)a.pages;
+    const float* s = a.scales + ((int64_t)(there ? page : 0) * a.nkv + c.kvh) * 2;
+    const float ks = s[0], vs = s[1];
+    k_scale = there ? ks : 1.f;
+    v_exp = there ? exponent_of(vs) : -256;
+    page = there ? page : 0;
+  }
+};
+
+// ---- up to 16 columns (decoded tokens): a workgroup takes segments of 512 keys one after the other, a wave two of a segment's tiles, every fourth.  They come straight into
+// registers: a tile's keys are asked for when the last tile's have been multiplied, its values when those have, so that there is something under way at any time and no
+// load waits for another (page numbers and scales are read 64 pages ahead; a page number read in turn would wait for all loads before it).  The waves' sums meet in LDS,
+// the segments' in a8_join_kernel.
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void a8_few_kernel(A8Args a, int segs_each) {
+  __shared__ float sums[4][DP / 16][64][4];
+  __shared__ float maxima[4][16], totals[4][16];
+  A8Rows<1> c;
+  const int kvh = blockIdx.x % a.nkv, item = blockIdx.x / a.nkv, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (!a8_rows<1>(a, item, kvh, 0, c)) return;
   int seg_first, seg_last;
   a8_segments(c.wave_lo, c.wave_pos, seg_first, seg_last);
-  if (seg < seg_first || seg > seg_last) return;
-  const int kb = seg * A8_SEG + wave * A8_TILE;
-  float m[NT], l[NT];
-  f32x4 acc[NT][DP / 16];
+  const int seg0 = max(seg_first, (int)blockIdx.y * segs_each), seg1 = min(seg_last, (int)blockIdx.y * segs_each + segs_each - 1);
+  if (seg0 > seg1) return;
+  const int kb0 = seg0 * A8_SEG + wave * A8_TILE, pos = min(c.wave_pos, seg1 * A8_SEG + A8_SEG - 1);
+  A8Pages pages;
+  pages.fill(a, c, seg0 * A8_SEG >> a.lp, pos);
+
+  struct Tile {
+    const A8Args& a;
+    const A8Rows<1>& c;
+    A8Pages& pages;
+    int pos, kb;                 // kb: of the tile that is asked for
+    float k_scale;
+    int v_exp;
+    u32x4 kr[4][DP / 64], vr[DP / 16];
+    __device__ __forceinline__ u32x4 k(int i, int j) const { return kr[i][j]; }
+    __device__ __forceinline__ u32x4 v(int dt) const { return vr[dt]; }
+    __device__ __forceinline__ bool wanted() const { return kb <= pos && kb + A8_TILE > c.wave_lo; }
+    __device__ __forceinline__ void ask_k() {
+      if (!wanted()) return;
+      if (((kb + A8_TILE - 1) >> a.lp) - pages.base >= 64) pages.fill(a, c, kb >> a.lp, pos);
+      const int kkey = kb + 16 * (c.r >> 2), vkey = kb + 16 * c.g, kl = (kkey >> a.lp) - pages.base, vl = (vkey >> a.lp) - pages.base;
+      k_scale = __shfl(pages.k_scale, kl);
+      v_exp = __shfl(pages.v_exp, vl);
+      v_exp = vkey <= c.wave_pos && vkey + 15 >= c.wave_lo ? v_exp : -256;
+      const uint8_t* kp = a.kc + (((int64_t)__shfl(pages.page, kl) * a.nkv + c.kvh) * a.P + (kkey & (a.P - 1)) + (c.r & 3)) * a.d;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.f;
+      for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) acc[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  int unit = -256;
-  if (kb <= c.wave_pos && kb + A8_TILE > c.wave_lo) {
-    q_part q[DP / 64][NT][A8_QJ];
-    A8Tile<DP> t;
-    a8_load<DP, NT>(a, c, kb, t);
-    a8_load_q<DP, NT>(a, c, q);
-    a8_tile<DP, NT>(a, c, kb, t, q, m, l, acc, unit);
-  }
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-    if (c.g == 0) {
-      maxima[wave][16 * n + c.r] = m[n];
-      totals[wave][16 * n + c.r] = l[n];
+        for (int j = 0; j < DP / 64; ++j)
+          kr[s][j] = *reinterpret_cast<const u32x4*>(kp + 4 * s * a.d + min(64 * j + 16 * c.g, a.d - 16));     // beyond d: the last again, times q's zeros
     }
-  __syncthreads();
-  const int mine = DP / 64;                             // entries' tiles that a wave sums up: wave, wave + 4, ...
+    __device__ __forceinline__ void ask_v() {
+      if (!wanted()) return;
+      const int vkey = kb + 16 * c.g;
+      const uint8_t* vp = a.vc + (((int64_t)__shfl(pages.page, (vkey >> a.lp) - pages.base) * a.nkv + c.kvh) * a.d + c.r) * a.P + (vkey & (a.P - 1));
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int col = c.col0 + 16 * n + c.r;
-    float top = maxima[0][16 * n + c.r];
-#pragma unroll
-    for (int x = 1; x < 4; ++x) top = fmaxf(top, maxima[x][16 * n + c.r]);
-    const float ref = top > -INFINITY ? top : 0.f, by = exp2_fast(m[n] - ref) * unit_of(unit);
+      for (int dt = 0; dt < DP / 16; ++dt) vr[dt] = *reinterpret_cast<const u32x4*>(vp + min(16 * dt, a.d - 16) * a.P);     // and here for nothing
+    }
+    __device__ __forceinline__ void k_done() {
+      kb += A8_SEG / 2;
+      ask_k();
+    }
+    __device__ __forceinline__ void v_done() { ask_v(); }
+  } t{a, c, pages, pos, kb0, 1.f, -256};
+  t.ask_k();
+  t.ask_v();
+  q_part q[DP / 64][1][A8_QJ];
+  a8_load_q<DP, 1>(a, c, q);
+  A8Sums<DP, 1> o;
+  o.clear();
+  for (int kb = kb0; (kb & ~(A8_SEG - 1)) <= seg1 * A8_SEG; kb += A8_SEG / 2) {
+    if (t.wanted()) {
+      a8_tile<DP, 1>(a, c, kb, t, t.k_scale, t.v_exp, q, o);
+    } else {
+      t.k_done();
+      t.v_done();
+    }
+    if ((kb & (A8_SEG / 2)) == 0) continue;
+    // Both tiles of the segment.
+    const int seg = kb / A8_SEG;
+    const float l = over_groups_sum(o.l[0]);
+    if (c.g == 0) {
+      maxima[wave][c.r] = o.m[0];
+      totals[wave][c.r] = l;
+    }
+    __syncthreads();
+    const float top = fmaxf(fmaxf(maxima[0][c.r], maxima[1][c.r]), fmaxf(maxima[2][c.r], maxima[3][c.r])), ref = top > -INFINITY ? top : 0.f;
+    const float by = exp2_fast(o.m[0] - ref) * o.scale();
     float total = 0.f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) total = __builtin_fmaf(totals[x][16 * n + c.r], exp2_fast(maxima[x][16 * n + c.r] - ref), total);
-    if (n > 0) __syncthreads();
+    for (int x = 0; x < 4; ++x) total = __builtin_fmaf(totals[x][c.r], exp2_fast(maxima[x][c.r] - ref), total);
 #pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) *reinterpret_cast<f32x4*>(sums + ((wave * (DP / 16) + dt) * 64 + lane) * 4) = acc[n][dt] * by;
+    for (int dt = 0; dt < DP / 16; ++dt) *reinterpret_cast<f32x4*>(sums[wave][dt][lane]) = o.acc[0][dt] * by;
+    o.clear();
     __syncthreads();
-    if (col >= c.cols) continue;
-    const int row = col / a.group;
-    const int64_t part = (((int64_t)blockIdx.x * a.nkv + kvh) * a.nseg + seg) * a.cols_max + col;
+    const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg) * a.cols_max + c.r;
+    if (c.r < c.cols) {
 #pragma unroll
-    for (int x = 0; x < mine; ++x) {
-      const int dt = 4 * x + wave;
-      if (16 * dt >= a.d) continue;
-      f32x4 o = *reinterpret_cast<const f32x4*>(sums + (dt * 64 + lane) * 4);
+      for (int x = 0; x < DP / 64; ++x) {
+        const int dt = 4 * x + wave;
+        if (16 * dt >= a.d) continue;
+        f32x4 v = *reinterpret_cast<const f32x4*>(sums[0][dt][lane]);
 #pragma unroll
-      for (int y = 1; y < 4; ++y) o = o + *reinterpret_cast<const f32x4*>(sums + ((y * (DP / 16) + dt) * 64 + lane) * 4);
-      if (seg_first == seg_last) {
-        store_elems4(a.out + ((int64_t)(c.tok0 + row) * a.nq + kvh * a.group + col - row * a.group) * a.d + 16 * dt + 4 * c.g,
-                     total == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * (1.f / total));
-      } else {
-        *reinterpret_cast<f32x4*>(a.part_acc + part * a.d + 16 * dt + 4 * c.g) = o;
+        for (int y = 1; y < 4; ++y) v = v + *reinterpret_cast<const f32x4*>(sums[y][dt][lane]);
+        if (seg_first == seg_last) store_elems4(a8_out<1>(a, c, c.r) + 16 * dt, total == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v * (1.f / total));
+        else *reinterpret_cast<f32x4*>(a.part_acc + part * a.d + 16 * dt + 4 * c.g) = v;
       }
+      if (seg_first != seg_last && wave == 0 && c.g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * part) = f32x2{top, total};
     }
-    if (seg_first != seg_last && wave == 0 && c.g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * part) = f32x2{top, total};
+    // The next segment's sums are written behind its first barrier, which no wave passes before all have read these.
   }
 }
 
-// A wave a column: its segments' sums, in ascending order.
-template <int NT>
-__global__ __launch_bounds__(256) void a8_join_kernel(A8Args a) {
+// ---- more columns (prompts, several drafted tokens): tiles pass through LDS once for all waves, each of which has 16 NT columns.  SPLIT: a workgroup takes one segment.
+//
+// A tile in LDS: K's row 16 i + r (the key that lane row r reads for tile i) in DP bytes, V's entry in 64; the 16-byte piece p of K's row r lies at p ^ turn(r), of V's entry
+// e at p ^ (e / 4 % 4), so that the 16 lanes that read a piece of 16 rows read 16 different quads of banks.  Pieces come by loads that go to LDS without passing registers: a load
+// brings a kilobyte, lane l's 16 bytes to place l, and the order is made by what each lane asks for.
+template <int DP, int WAVES>
+struct A8Stage {
+  static constexpr int BYTES = 2 * A8_TILE * DP, LOADS = DP / 16 / WAVES;      // of a tile; of K, and of V, that a wave asks for
+  static_assert(DP / 16 % WAVES == 0, "every wave asks for the same number of loads");
+  static constexpr int PIECES = DP / 16;                                       // of a row of K
+  __device__ static __forceinline__ int turn(int r) { return DP == 128 ? r >> 1 & 7 : DP == 256 ? r : r >> 2 & 3; }
+};
+
+__device__ __forceinline__ void a8_load_to_lds(const uint8_t* p, unsigned lds_addr) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds_addr) : "memory");
+}
+
+template <int DP, int WAVES, int NT>
+__device__ __forceinline__ void a8_ask(const A8Args& a, const A8Rows<NT>& c, const A8Pages& pg, int kb, unsigned lds) {
+  typedef A8Stage<DP, WAVES> ST;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, last_k = a.d / 16 - 1;
+#pragma unroll
+  for (int i = 0; i < ST::LOADS; ++i) {
+    const int at = (i * WAVES + wave) * 64 + lane;             // piece of K's tile
+    const int row = at / ST::PIECES, r = row & 15, piece = min((at % ST::PIECES) ^ ST::turn(r), last_k);
+    const int key = kb + 16 * (r >> 2) + 4 * (row >> 4) + (r & 3);
+    const int page = __shfl(pg.page, (key >> a.lp) - pg.base);
+    a8_load_to_lds(a.kc + (((int64_t)page * a.nkv + c.kvh) * a.P + (key & (a.P - 1))) * a.d + 16 * piece, __builtin_amdgcn_readfirstlane(lds + (i * WAVES + wave) * 1024));
+  }
+#pragma unroll
+  for (int i = 0; i < ST::LOADS; ++i) {
+    const int at = (i * WAVES + wave) * 64 + lane, row = min(at >> 2, a.d - 1), piece = (at & 3) ^ (at >> 4 & 3);
+    const int key = kb + 16 * piece;
+    const int page = __shfl(pg.page, (key >> a.lp) - pg.base);
+    a8_load_to_lds(a.vc + (((int64_t)page * a.nkv + c.kvh) * a.d + row) * a.P + (key & (a.P - 1)),
+                   __builtin_amdgcn_readfirstlane(lds + A8_TILE * DP + (i * WAVES + wave) * 1024));
+  }
+}
+
+template <int DP, int WAVES>
+struct A8Shared {
+  const uint8_t* tile;
+  int r, g;
+  __device__ __forceinline__ u32x4 k(int i, int j) const {
+    return *reinterpret_cast<const u32x4*>(tile + (16 * i + r) * DP + (((4 * j + g) ^ A8Stage<DP, WAVES>::turn(r)) << 4));
+  }
+  __device__ __forceinline__ void k_done() {}
+  __device__ __forceinline__ void v_done() {}
+  __device__ __forceinline__ u32x4 v(int dt) const { return *reinterpret_cast<const u32x4*>(tile + A8_TILE * DP + (16 * dt + r) * 64 + ((g ^ (r >> 2)) << 4)); }
+};
+
+template <int DP, int NT, int WAVES, bool SPLIT>
+__global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kernel(A8Args a, int blocks) {
+  typedef A8Stage<DP, WAVES> ST;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t stages[];      // A8_STAGES tiles
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // The kv head first: the workgroups of one, which read the same pages, then fall to as few of the eight caches as there are.
+  int unit = blockIdx.x;
+  const int kvh = unit % a.nkv;
+  unit /= a.nkv;
+  const int seg = SPLIT ? unit % a.nseg : 0;
+  if (SPLIT) unit /= a.nseg;
+  const int block = unit % blocks, item = SPLIT ? unit / blocks : a.n_items - 1 - unit / blocks;     // a prompt's last rows, which see most keys, first
   A8Rows<NT> c;
-  const int kvh = blockIdx.y, lane = threadIdx.x & 63, col = blockIdx.z * 4 + (threadIdx.x >> 6);
-  if (!a8_rows<NT>(a, blockIdx.x, kvh, col / (16 * NT) * (16 * NT), c) || col >= c.cols) return;
+  A8Rows<NT * WAVES> all;                                                 // the workgroup's columns
+  if (!a8_rows<NT * WAVES>(a, item, kvh, block * 16 * NT * WAVES, all)) return;
+  const bool mine = a8_rows<NT>(a, item, kvh, (block * WAVES + wave) * 16 * NT, c);
+  int lo = all.wave_lo, pos = all.wave_pos, seg_first = 0, seg_last = 0;
+  if (SPLIT) {
+    a8_segments(lo, pos, seg_first, seg_last);
+    if (seg < seg_first || seg > seg_last) return;
+    lo = max(lo, seg * A8_SEG);
+    pos = min(pos, seg * A8_SEG + A8_SEG - 1);
+  }
+  if (!mine) {
+    c.seq = all.seq;
+    c.kvh = kvh;
+  }
+  q_part q[DP / 64][NT][A8_QJ];
+  if (mine) a8_load_q<DP, NT>(a, c, q);
+  A8Sums<DP, NT> o;
+  o.clear();
+  lo &= ~(A8_TILE - 1);
+  const int tiles = pos < lo ? 0 : ((pos - lo) >> 6) + 1;
+  const unsigned lds = (unsigned)(unsigned long)((__attribute__((address_space(3))) const void*)stages);
+  A8Pages ahead, now;                                                     // of the tiles that are asked for, of those that are computed
+  if (tiles > 0) ahead.fill(a, c, lo >> a.lp, pos);
+  now = ahead;
+  auto ask = [&](int i) {
+    const int kb = lo + i * A8_TILE;
+    if ((kb >> a.lp) - ahead.base >= 64) ahead.fill(a, c, kb >> a.lp, pos);
+    a8_ask<DP, WAVES, NT>(a, c, ahead, kb, lds + (unsigned)(i % A8_STAGES) * ST::BYTES);
+  };
+  if (tiles > 0) ask(0);
+  if (tiles > 1) ask(1);
+  for (int i = 0; i < tiles; ++i) {
+    const int kb = lo + i * A8_TILE;
+    // Tile i has arrived (at most the next one's loads are under way), this wave has what it read of tile i - 1; behind the barrier that holds for all.
+    asm volatile("" ::: "memory");
+    if (i + 1 < tiles) __builtin_amdgcn_s_waitcnt(0x0070 | (2 * ST::LOADS & 0xF) | ((2 * ST::LOADS >> 4) << 14));
+    else __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (i + 2 < tiles) ask(i + 2);
+    if ((kb >> a.lp) - now.base >= 64) now.fill(a, c, kb >> a.lp, pos);
+    if (mine && kb <= c.wave_pos && kb + A8_TILE > c.wave_lo) {
+      const int kp = ((kb + 16 * (c.r >> 2)) >> a.lp) - now.base, vp = ((kb + 16 * c.g) >> a.lp) - now.base;
+      const float k_scale = __shfl(now.k_scale, kp);
+      const int v_exp = __shfl(now.v_exp, vp), key = kb + 16 * c.g;
+      a8_tile<DP, NT>(a, c, kb, A8Shared<DP, WAVES>{stages + (i % A8_STAGES) * ST::BYTES, c.r, c.g}, k_scale,
+                      key <= c.wave_pos && key + 15 >= c.wave_lo ? v_exp : -256, q, o);
+    }
+  }
+  if (!mine) return;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = c.col0 + 16 * n + c.r;
+    const float l = over_groups_sum(o.l[n]);
+    if (col >= c.cols) continue;
+    if (SPLIT && seg_first != seg_last) {
+      const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg) * a.cols_max + col;
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt)
+        if (16 * dt < a.d) *reinterpret_cast<f32x4*>(a.part_acc + part * a.d + 16 * dt + 4 * c.g) = o.acc[n][dt] * o.scale();
+      if (c.g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * part) = f32x2{o.m[n], l};
+    } else {
+      elem_t* to = a8_out<NT>(a, c, col);
+      const float by = l == 0.f ? 0.f : o.scale() / l;
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt)
+        if (16 * dt < a.d) store_elems4(to + 16 * dt, l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o.acc[n][dt] * by);
+    }
+  }
+}
+
+// ---- the segments of a column, by a wave: weights relative to their largest maximum, sums in ascending order.  cols: of a block in the kernel that wrote them.
+__global__ __launch_bounds__(256) void a8_join_kernel(A8Args a, int cols) {
+  A8Rows<1> c;
+  const int kvh = blockIdx.x % a.nkv, item = blockIdx.x / a.nkv, lane = threadIdx.x & 63, col = blockIdx.y * 4 + (threadIdx.x >> 6);
+  if (!a8_rows<1>(a, item, kvh, col, c)) return;
+  const int block0 = col / cols * cols, row_first = block0 / a.group, row_last = (min(c.cols, block0 + cols) - 1) / a.group;
   int seg_first, seg_last;
-  a8_segments(c.wave_lo, c.wave_pos, seg_first, seg_last);
+  a8_segments(a.window > 0 ? max(0, c.pos0 + row_first - a.window + 1) : 0, c.pos0 + row_last, seg_first, seg_last);
   if (seg_first == seg_last) return;                    // the other kernel wrote the result
-  const int64_t part0 = ((int64_t)blockIdx.x * a.nkv + kvh) * a.nseg * a.cols_max + col;
+  const int64_t part0 = ((int64_t)item * a.nkv + kvh) * a.nseg * a.cols_max + col;
   float top = -INFINITY;
   for (int s = seg_first + lane; s <= seg_last; s += 64) top = fmaxf(top, a.part_ml[2 * (part0 + (int64_t)s * a.cols_max)]);
   top = wave_max_xor(top);
   const float ref = top > -INFINITY ? top : 0.f;
-  float total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = seg_first; s <= seg_last; ++s) {
-    const int64_t part = part0 + (int64_t)s * a.cols_max;
-    const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * part);
-    const float by = exp2_fast(ml.x - ref);
-    total = __builtin_fmaf(ml.y, by, total);
+  float total = 0.f;
+  f32x2 o[2] = {{0.f, 0.f}, {0.f, 0.f}};
+  for (int s0 = seg_first; s0 <= seg_last; s0 += 64) {
+    float by = 0.f;
+    if (s0 + lane <= seg_last) {
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * (part0 + (int64_t)(s0 + lane) * a.cols_max));
+      by = exp2_fast(ml.x - ref);
+      total = __builtin_fmaf(ml.y, by, total);
+    }
+    const int n = min(64, seg_last - s0 + 1);
+    const float* p = a.part_acc + (part0 + (int64_t)s0 * a.cols_max) * a.d + 2 * lane;
+    for (int s = 0; s < n; s += 8) {
+      f32x2 v[8][2];
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (lane + 64 * x < a.d) o[x] = __builtin_fmaf(a.part_acc[part * a.d + lane + 64 * x], by, o[x]);
+      for (int x = 0; x < 8; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          v[x][h] = f32x2{0.f, 0.f};
+          if (s + x < n && 2 * lane + 128 * h < a.d) v[x][h] = *reinterpret_cast<const f32x2*>(p + (int64_t)(s + x) * a.cols_max * a.d + 128 * h);
+        }
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const float b = __shfl(by, min(s + x, 63));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          o[h].x = s + x < n ? __builtin_fmaf(v[x][h].x, b, o[h].x) : o[h].x;
+          o[h].y = s + x < n ? __builtin_fmaf(v[x][h].y, b, o[h].y) : o[h].y;
+        }
+      }
+    }
   }
+  total = wave_sum_xor(total);
   const int row = col / a.group;
-  elem_t* to = a.out + ((int64_t)(c.tok0 + row) * a.nq + kvh * a.group + col - row * a.group) * a.d;
+  elem_t* to = a.out + ((int64_t)(c.tok0 + row) * a.nq + kvh * a.group + col - row * a.group) * a.d + 2 * lane;
 #pragma unroll
-  for (int x = 0; x < 4; ++x)
-    if (lane + 64 * x < a.d) to[lane + 64 * x] = from_f32<elem_t>(total == 0.f ? 0.f : o[x] / total);
+  for (int h = 0; h < 2; ++h)
+    if (2 * lane + 128 * h < a.d) {
+      to[128 * h] = from_f32<elem_t>(total == 0.f ? 0.f : o[h].x / total);
+      to[128 * h + 1] = from_f32<elem_t>(total == 0.f ? 0.f : o[h].y / total);
+    }
 }
 
-// Column tiles a wave of the few rows' kernel takes at once: as many as there are columns, up to what its registers hold.
-static int few_tiles(int cols, int d) { return cols <= 16 || d > 128 ? 1 : cols <= 32 || sizeof(elem_t) == 4 ? 2 : 4; }
+template <int DP, int NT, int WAVES, bool SPLIT>
+static int a8_shared(const A8Args& a, hipStream_t st) {
+  const int blocks = (a.cols_max + 16 * NT * WAVES - 1) / (16 * NT * WAVES);
+  const int64_t units = (int64_t)a.n_items * a.nkv * blocks * (SPLIT ? a.nseg : 1);
+  VK_REQUIRE(units < (1ll << 31), "attention8: %d items of %d rows, %d heads: too many for one launch", a.n_items, a.item_rows, a.nq);
+  const int lds = A8_STAGES * A8Stage<DP, WAVES>::BYTES;
+  if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)a8_shared_kernel<DP, NT, WAVES, SPLIT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  a8_shared_kernel<DP, NT, WAVES, SPLIT><<<(unsigned)units, 64 * WAVES, lds, st>>>(a, blocks);
+  return vk_check_launch("attention8");
+}
 
 extern "C" {
 
@@ -501,48 +716,47 @@ int vk_paged_attention8(elem_t* out, const elem_t* q, const uint8_t* kc, const u
   VK_REQUIRE(item_rows >= 1 && item_rows <= A8_ITEM_ROWS, "attention8: items of %d rows; at most %d", item_rows, A8_ITEM_ROWS);
   VK_REQUIRE(pages > 0 && W > 0 && max_k_len >= 0 && (int64_t)W * P >= max_k_len && (int64_t)W * P < (1ll << 31), "attention8: a table of %d pages of %d does not cover %d keys", W, P, max_k_len);
   VK_REQUIRE(window >= 0, "attention8: window %d", window);
+  VK_REQUIRE(scale > 0.f && scale < INFINITY, "attention8: scale %g is no positive number", (double)scale);
   if (n_items == 0 || T == 0 || S == 0) return 0;
   VK_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)scratch) % 16 == 0, "attention8: rows, cache and scratch have to lie on 16 bytes");
   const int group = nq / nkv, nseg = max(1, (int)(((int64_t)max_k_len + A8_SEG - 1) / A8_SEG));
   A8Args a{q, out, kc, vc, scales, table, cu_q, k_len, items, nullptr, nullptr, W, T, S, nq, nkv, d, P, 0, pages, group, item_rows, item_rows * group, window, nseg,
-           scale * 1.4426950408889634f};
+           n_items, scale * 1.4426950408889634f};
   while (1 << a.lp < P) ++a.lp;
+  constexpr bool F32 = sizeof(elem_t) == 4;
   if (item_rows > 16) {
-    constexpr int NT = sizeof(elem_t) == 4 ? 1 : 2;
-    const int blocks = (a.cols_max + 64 * NT - 1) / (64 * NT);
-    VK_REQUIRE((int64_t)blocks * nkv <= 65535, "attention8: %d heads of %d rows are too many for one launch", nq, item_rows);
-#define PROMPT(D) a8_prompt_kernel<D, NT><<<dim3(n_items, nkv * blocks), 256, 0, st>>>(a, blocks)
-    if (d <= 64) PROMPT(64);
-    else if (d <= 128) PROMPT(128);
-    else if (d <= 192) PROMPT(192);
-    else PROMPT(256);
-#undef PROMPT
-    return vk_check_launch("attention8 (prompt)");
+    constexpr int NT = F32 ? 1 : 2;
+    return d <= 64 ? a8_shared<64, NT, 4, false>(a, st) : d <= 128 ? a8_shared<128, NT, 4, false>(a, st) : d <= 192 ? a8_shared<192, NT, 4, false>(a, st)
+                                                                                                                   : a8_shared<256, NT, 4, false>(a, st);
   }
   const int64_t need = vk_attn8_scratch_floats(n_items, item_rows, nq, d, max_k_len);
   VK_REQUIRE(need == 0 || (scratch != nullptr && scratch_floats >= need), "attention8: scratch of %lld floats needed", (long long)need);
   a.part_acc = scratch;
   a.part_ml = scratch + need / (d + 2) * d;
-  const int nt = few_tiles(a.cols_max, d), blocks = (a.cols_max + 16 * nt - 1) / (16 * nt);
-  VK_REQUIRE((int64_t)blocks * nkv <= 65535 && nseg <= 65535 && (a.cols_max + 3) / 4 <= 65535, "attention8: %d heads, %d keys: too many for one launch", nq, max_k_len);
-  const dim3 grid(n_items, nkv * blocks, nseg), join(n_items, nkv, (a.cols_max + 3) / 4);
-#define FEW(D, N) (a8_few_kernel<D, N><<<grid, 256, D * 256, st>>>(a))
-#ifdef VK_BF16
-#define FEW_D(D) (nt == 1 ? FEW(D, 1) : nt == 2 ? FEW(D, 2) : FEW(D, 4))
-#else
-#define FEW_D(D) (nt == 1 ? FEW(D, 1) : FEW(D, 2))
-#endif
-  if (d <= 64) FEW_D(64);
-  else if (d <= 128) FEW_D(128);
-  else if (d <= 192) FEW(192, 1);
-  else FEW(256, 1);
-#undef FEW_D
-#undef FEW
-  if (vk_check_launch("attention8")) return 1;
+  const int64_t joins = (int64_t)n_items * nkv;
+  VK_REQUIRE(joins < (1ll << 31) && nseg <= 65535, "attention8: %d items, %d keys: too many for one launch", n_items, max_k_len);
+  int cols = 16;                                        // of a block
+  if (a.cols_max <= 16) {
+    // Workgroups of several segments where there are more than the card holds at once: what stands in front of a workgroup's first loads is then paid once.
+    const int64_t held = 2 * vk_device_cus();
+    const int each = (int)max((int64_t)1, min((int64_t)8, joins * nseg / (2 * held)));
+    const dim3 grid((unsigned)joins, (nseg + each - 1) / each);
+    if (d <= 64) a8_few_kernel<64><<<grid, 256, 0, st>>>(a, each);
+    else if (d <= 128) a8_few_kernel<128><<<grid, 256, 0, st>>>(a, each);
+    else if (d <= 192) a8_few_kernel<192><<<grid, 256, 0, st>>>(a, each);
+    else a8_few_kernel<256><<<grid, 256, 0, st>>>(a, each);
+    if (vk_check_launch("attention8")) return 1;
+  } else {
+    const bool two = a.cols_max <= 32;
+    cols = two ? 32 : 64;
+    const int bad = two ? (d <= 64 ? a8_shared<64, 1, 2, true>(a, st) : d <= 128 ? a8_shared<128, 1, 2, true>(a, st) : d <= 192 ? a8_shared<192, 1, 2, true>(a, st)
+                                                                                                                               : a8_shared<256, 1, 2, true>(a, st))
+                        : (d <= 64 ? a8_shared<64, 1, 4, true>(a, st) : d <= 128 ? a8_shared<128, 1, 4, true>(a, st) : d <= 192 ? a8_shared<192, 1, 4, true>(a, st)
+                                                                                                                               : a8_shared<256, 1, 4, true>(a, st));
+    if (bad) return 1;
+  }
   if (nseg == 1) return 0;
-  if (nt == 1) a8_join_kernel<1><<<join, 256, 0, st>>>(a);
-  else if (nt == 2) a8_join_kernel<2><<<join, 256, 0, st>>>(a);
-  else a8_join_kernel<4><<<join, 256, 0, st>>>(a);
+  a8_join_kernel<<<dim3((unsigned)joins, (a.cols_max + 3) / 4), 256, 0, st>>>(a, cols);
   return vk_check_launch("attention8 (join)");
 }
 
