@@ -19,7 +19,6 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
 __device__ __forceinline__ float pow2f(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }            // -126 .. 127
-__device__ __forceinline__ double pow2d(int e) { return __builtin_bit_cast(double, (uint64_t)(e + 1023) << 52); }         // -1022 .. 1023
 __device__ __forceinline__ int exponent_of(float scale) { return (int)(__builtin_bit_cast(uint32_t, scale) >> 23 & 255) - 127; }
 
 // The least e with |x| <= 448 * 2^e = 1.75 * 2^(e + 8); CACHE8_LOWEST at least, and for what is not finite.
@@ -28,23 +27,19 @@ __device__ __forceinline__ int least_exponent(float x) {
   const int e = (int)(u >> 23) - 127;
   return e > 127 ? CACHE8_LOWEST : max(CACHE8_LOWEST, e - 8 + ((u & 0x7fffffu) > 0x600000u));
 }
-__device__ __forceinline__ int least_exponent(double x) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, x) & 0x7fffffffffffffffull;
-  const int e = (int)(u >> 52) - 1023;
-  return e > 127 ? CACHE8_LOWEST : max(CACHE8_LOWEST, e - 8 + ((u & 0xfffffffffffffull) > 0xc000000000000ull));
+// A 64-bit number in 32 bits, the last of them set where bits were lost: whatever is rounded to fewer digits from there (four) is rounded as from all 53, for a number that is no tie, or
+// that is above a limit of few digits, remains so.
+__device__ __forceinline__ float round_to_odd(double x) {
+  const float f = (float)x;
+  const double back = (double)f;
+  uint32_t u = __builtin_bit_cast(uint32_t, f);
+  if (back != x && (u >> 23 & 255) != 255) u = (u - (fabs(back) > fabs(x) ? 1u : 0u)) | 1u;
+  return __builtin_bit_cast(float, u);
 }
-
 // What a conversion to e4m3 is given for the entry x of a page with the scale 2^e: x / 2^e, and NaN for what is not finite (e4m3 has no infinity, and a
-// clipped one would go unnoticed).  A 64-bit x is rounded to four digits here, half to even: rounded to 32 bits first it could end on a tie that it is not.
+// clipped one would go unnoticed).
 __device__ __forceinline__ float entry_of(float x, int e) {
   return (__builtin_bit_cast(uint32_t, x) >> 23 & 255) == 255 ? NAN : x * pow2f(-e);
-}
-__device__ __forceinline__ float entry_of(double x, int e) {
-  if ((int)(__builtin_bit_cast(uint64_t, x) >> 52 & 0x7ff) - 1023 > 127) return NAN;
-  const double y = x * pow2d(-e);
-  const int top = max(-6, (int)(__builtin_bit_cast(uint64_t, y) >> 52 & 0x7ff) - 1023);
-  const double step = __builtin_bit_cast(double, (uint64_t)(top - 3 + 52 + 1023) << 52 | 1ull << 51);      // 1.5 * 2^52 of the last digit
-  return (float)((y + step) - step);
 }
 
 // Four e4m3 values of four numbers, the first in the lowest byte.

@@ -29,47 +29,98 @@ struct Store8Args {
   int w_is_f32;
   const elem_t *cos_t, *sin_t;   // [at least max_k_len, rot_half] or null
   int rot_half;
+  int whole;                // weights and tables lie on 16 bytes, and rot_half is a whole number of vectors: a lane's entries of them are read at once
   const int32_t *table, *cu_q, *k_len;
-  int W, T, S, nq, nkv, d, P, lp, pages, kv_jobs, max_k_len;
-  double eps;
+  int W, T, S, nq, nkv, d, P, lp, pages, kv_blocks, held, max_k_len;
+  double eps, per_d;        // per_d: 1 / d
 };
 
 // Sum over the LPH neighbouring lanes of a head; the order is fixed by LPH.
 template <int LPH>
 __device__ __forceinline__ float head_sum(float v) { return group_sum<LPH>(v); }
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, true), hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 template <int LPH>
 __device__ __forceinline__ double head_sum(double v) {
-#pragma unroll
-  for (int off = 1; off < LPH; off <<= 1) v = v + __shfl_xor(v, off);
+  if (LPH >= 2) v = v + dpp_d<0xB1>(v);               // quad_perm [1, 0, 3, 2]
+  if (LPH >= 4) v = v + dpp_d<0x4E>(v);               // quad_perm [2, 3, 0, 1]
+  if (LPH >= 8) v = v + dpp_d<0x141>(v);              // row_half_mirror
+  if (LPH >= 16) v = v + dpp_d<0x140>(v);             // row_mirror
+  if (LPH >= 32) v = v + __shfl_xor(v, 16);
+  if (LPH >= 64) v = v + __shfl_xor(v, 32);
   return v;
 }
-__device__ __forceinline__ float root_of(float v) { return sqrtf(v); }
-__device__ __forceinline__ double root_of(double v) { return sqrt(v); }
+__device__ __forceinline__ float one_over_root(float v) { return rsqrtf(v); }
+__device__ __forceinline__ double one_over_root(double v) { return rsqrt(v); }
 
-// A lane's VK_VEC entries of a head, from entry c0 on: norm and turn.  y: the head's own LPH * VK_VEC numbers of LDS.
+// What a lane reads for its VK_VEC entries of a head from entry c0 on, whatever the head: the norm's weights and the angles' cosines and sines.  Entry c turns with
+// entry c + h, c < h, and c - h, c < 2 h; others stand, with cosine 1 and sine 0.
+struct Turn {
+  float w[VK_VEC], cs[VK_VEC], sn[VK_VEC];
+};
+__device__ __forceinline__ void read_weights(const Store8Args& a, const void* w, int c0, Turn& t) {
+  const int at = min(c0, a.d - VK_VEC);                 // lanes behind the head have nothing to multiply
+  if (a.whole && !a.w_is_f32) {
+    load_elems(static_cast<const elem_t*>(w) + at, t.w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VK_VEC; ++e) t.w[e] = load_weight(w, a.w_is_f32, at + e);
+  }
+}
+__device__ __forceinline__ void read_angles(const Store8Args& a, int c0, int place, Turn& t) {
+  const int h = a.rot_half;
+  const elem_t *cs = a.cos_t + (int64_t)place * h, *sn = a.sin_t + (int64_t)place * h;
+  if (a.whole) {
+    const int at = c0 < h ? c0 : c0 < 2 * h ? c0 - h : 0;
+    load_elems(cs + at, t.cs);
+    load_elems(sn + at, t.sn);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VK_VEC; ++e) {
+      const int c = c0 + e, at = c < h ? c : c < 2 * h ? c - h : 0;
+      t.cs[e] = to_f32(cs[at]);
+      t.sn[e] = to_f32(sn[at]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VK_VEC; ++e) {
+    t.cs[e] = c0 + e < 2 * h ? t.cs[e] : 1.f;
+    t.sn[e] = c0 + e < h ? -t.sn[e] : c0 + e < 2 * h ? t.sn[e] : 0.f;
+  }
+}
+
+// Norm and turn of a lane's entries.  y: the head's own LPH * VK_VEC numbers of LDS.
 template <int LPH, typename F>
-__device__ __forceinline__ void norm_and_turn(F (&v)[VK_VEC], const Store8Args& a, const void* w, int c0, int place, F* y) {
-  if (w != nullptr) {
+__device__ __forceinline__ void norm_and_turn(F (&v)[VK_VEC], const Store8Args& a, bool norm, const Turn& t, int c0, F* y) {
+  if (norm) {
     F part = 0;
 #pragma unroll
     for (int e = 0; e < VK_VEC; ++e) part = part + v[e] * v[e];
-    const F r = (F)1 / root_of(head_sum<LPH>(part) / (F)a.d + (F)a.eps);
+    const F r = one_over_root(head_sum<LPH>(part) * (F)a.per_d + (F)a.eps);
 #pragma unroll
-    for (int e = 0; e < VK_VEC; ++e) v[e] = c0 + e < a.d ? v[e] * r * (F)load_weight(w, a.w_is_f32, c0 + e) : (F)0;
+    for (int e = 0; e < VK_VEC; ++e) v[e] = v[e] * r * (F)t.w[e];
   }
   if (a.cos_t != nullptr) {
     const int h = a.rot_half;
-    const elem_t *cs = a.cos_t + (int64_t)place * h, *sn = a.sin_t + (int64_t)place * h;
 #pragma unroll
     for (int e = 0; e < VK_VEC; ++e) y[c0 + e] = v[e];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    F other[VK_VEC];
+    if (a.whole) {
+      const int at = c0 < h ? c0 + h : c0 < 2 * h ? c0 - h : c0;
 #pragma unroll
-    for (int e = 0; e < VK_VEC; ++e) {
-      const int c = c0 + e;
-      if (c < h) v[e] = v[e] * (F)to_f32(cs[c]) - y[c + h] * (F)to_f32(sn[c]);
-      else if (c < 2 * h) v[e] = v[e] * (F)to_f32(cs[c - h]) + y[c - h] * (F)to_f32(sn[c - h]);
+      for (int e = 0; e < VK_VEC; ++e) other[e] = y[at + e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < VK_VEC; ++e) other[e] = y[c0 + e < h ? c0 + e + h : c0 + e < 2 * h ? c0 + e - h : c0 + e];
     }
+#pragma unroll
+    for (int e = 0; e < VK_VEC; ++e) v[e] = v[e] * (F)t.cs[e] + other[e] * (F)t.sn[e];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
@@ -85,138 +136,176 @@ __device__ __forceinline__ int rows_of(const Store8Args& a, int i, int& first, i
   return first >= 0 && end <= a.T && n > 0 && n <= keys && keys <= a.max_k_len ? n : 0;
 }
 
+// LDS of a workgroup: each wave's heads while they turn, and the new entries of a page, `held` rows of d numbers, between their maximum and their rounding.
+constexpr int STORE8_TURN = 4 * 64 * VK_VEC;
+
 template <int LPH>
-__global__ __launch_bounds__(STORE8_THREADS) void store8_kernel(Store8Args a) {
-  constexpr int HPW = 64 / LPH;
-  __shared__ double turn_rows[4][64 * VK_VEC];
+__global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a, int first_block) {
+  constexpr int HPW = 64 / LPH, ROWS = 4 * HPW;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ int wave_need[4];
-  extern __shared__ uint8_t turned[];                // v's new entries, [d][P + 4]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane % LPH, sub = lane / LPH, c0 = j * VK_VEC, d = a.d, P = a.P;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPH, c0 = lane % LPH * VK_VEC, d = a.d, P = a.P, block = first_block + blockIdx.x;
   const bool inside = c0 < d;
 
-  if ((int)blockIdx.x >= a.kv_jobs * a.nkv * 2) {
+  if (block >= a.kv_blocks) {
     // ---- a token's q heads
-    const int tok = blockIdx.x - a.kv_jobs * a.nkv * 2;
+    const int tok = block - a.kv_blocks;
+    const elem_t* row = a.qkv + (int64_t)tok * a.row_stride + c0;
+    float* y = reinterpret_cast<float*>(lds) + (wave * HPW + sub) * LPH * VK_VEC;
+    float next[VK_VEC];
+    auto ask = [&](int h) {
+#pragma unroll
+      for (int e = 0; e < VK_VEC; ++e) next[e] = 0.f;
+      if (h + sub < a.nq && inside) load_elems(row + (h + sub) * d, next);
+    };
+    ask(wave * HPW);
+    Turn t;
+    if (a.q_w != nullptr) read_weights(a, a.q_w, c0, t);
     int place = -1;
     for (int base = 0; base < a.S && place < 0; base += 64) {
       int first, keys;
       const int n = rows_of(a, base + lane, first, keys);
       const uint64_t mine = __ballot(tok >= first && tok < first + n);
-      if (mine != 0) place = __shfl(keys - n + tok - first, __builtin_ctzll(mine));
+      if (mine != 0) place = __builtin_amdgcn_readlane(keys - n + tok - first, __builtin_ctzll(mine));
     }
     if (place < 0) return;                            // behind the last sequence's rows
-    float* y = reinterpret_cast<float*>(turn_rows[wave]) + sub * LPH * VK_VEC;
-    for (int h = wave * HPW; h < a.nq; h += 4 * HPW) {
-      const bool live = h + sub < a.nq && inside;
+    if (a.cos_t != nullptr) read_angles(a, c0, place, t);
+    for (int h = wave * HPW; h < a.nq; h += ROWS) {
       float v[VK_VEC];
 #pragma unroll
-      for (int e = 0; e < VK_VEC; ++e) v[e] = 0.f;
-      if (live) load_elems(a.qkv + (int64_t)tok * a.row_stride + (h + sub) * d + c0, v);
-      norm_and_turn<LPH>(v, a, a.q_w, c0, place, y);
-      if (live) store_elems(a.q_out + ((int64_t)tok * a.nq + h + sub) * d + c0, v);
+      for (int e = 0; e < VK_VEC; ++e) v[e] = next[e];
+      ask(h + ROWS);
+      norm_and_turn<LPH>(v, a, a.q_w != nullptr, t, c0, y);
+      if (h + sub < a.nq && inside) store_elems(a.q_out + ((int64_t)tok * a.nq + h + sub) * d + c0, v);
     }
     return;
   }
 
   // ---- a page's new keys or values of one head
-  const int job = blockIdx.x / (a.nkv * 2), head = (blockIdx.x >> 1) % a.nkv;
-  const bool is_v = blockIdx.x & 1;
+  const int job = block / (a.nkv * 2), head = (block >> 1) % a.nkv;
+  const bool is_v = block & 1;
+  Turn t;
+  if (!is_v && a.k_w != nullptr) read_weights(a, a.k_w, c0, t);
   int seq = -1, tok0 = 0, off0 = 0, m = 0, pidx = 0;
   for (int base = 0, run = 0; base < a.S; base += 64) {
     int first, keys;
     const int n = rows_of(a, base + lane, first, keys), from = keys - n;
     const int mine = n > 0 ? ((keys - 1) >> a.lp) - (from >> a.lp) + 1 : 0;
     int upto = mine;                                  // pages of the sequences up to this lane's
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int t = __shfl_up(upto, off);
-      if (lane >= off) upto += t;
-    }
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xF, 0xF, true);      // row_shr 1, 2, 4, 8: within 16 lanes
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xF, 0xF, true);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xF, 0xF, true);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xF, 0xF, true);
+    const int r0 = __builtin_amdgcn_readlane(upto, 15), r1 = r0 + __builtin_amdgcn_readlane(upto, 31), r2 = r1 + __builtin_amdgcn_readlane(upto, 47);
+    upto += lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r1 : r2;
     const uint64_t hit = __ballot(job < run + upto);
     if (hit != 0) {
       const int l = __builtin_ctzll(hit);
-      const int before = run + __shfl(upto - mine, l), k = __shfl(keys, l), f = __shfl(from, l), t = __shfl(first, l);
+      const int before = run + __builtin_amdgcn_readlane(upto - mine, l), k = __builtin_amdgcn_readlane(keys, l), f = __builtin_amdgcn_readlane(from, l);
       seq = base + l;
       pidx = (f >> a.lp) + job - before;
       const int lo = max(pidx << a.lp, f), hi = min((pidx + 1) << a.lp, k);
       off0 = lo - (pidx << a.lp);
       m = hi - lo;
-      tok0 = t + lo - f;
+      tok0 = __builtin_amdgcn_readlane(first, l) + lo - f;
       break;
     }
-    run += __shfl(upto, 63);
+    run += __builtin_amdgcn_readlane(upto, 63);
   }
   if (seq < 0 || pidx >= a.W) return;
+  const elem_t* rows = a.qkv + (int64_t)tok0 * a.row_stride + (a.nq + head + (is_v ? a.nkv : 0)) * d + c0;
+  float next[VK_VEC];
+  auto ask = [&](int i) {
+#pragma unroll
+    for (int e = 0; e < VK_VEC; ++e) next[e] = 0.f;
+    if (i < m && inside) load_elems(rows + (int64_t)i * a.row_stride, next);
+  };
+  ask(wave * HPW + sub);
+  const int place0 = (pidx << a.lp) + off0;
+  if (!is_v && a.cos_t != nullptr) read_angles(a, c0, place0 + min(wave * HPW + sub, m - 1), t);
   const int page = a.table[(int64_t)seq * a.W + pidx];
   if ((unsigned)page >= (unsigned)a.pages) return;    // a sequence whose rows are not to be kept
-  const int64_t block = (int64_t)page * a.nkv + head;
-  const int place0 = (pidx << a.lp) + off0;
-
-  double* y = turn_rows[wave] + sub * LPH * VK_VEC;
-  const elem_t* rows = a.qkv + (int64_t)tok0 * a.row_stride + (a.nq + head + (is_v ? a.nkv : 0)) * d + c0;
-  double k[VK_VEC];
-  float v[VK_VEC];
-  auto entries = [&](int i) {                         // this lane's entries of new row i
-#pragma unroll
-    for (int e = 0; e < VK_VEC; ++e) v[e] = 0.f;
-    if (i < m && inside) load_elems(rows + (int64_t)i * a.row_stride, v);
-    if (is_v) return;
-#pragma unroll
-    for (int e = 0; e < VK_VEC; ++e) k[e] = (double)v[e];
-    norm_and_turn<LPH>(k, a, a.k_w, c0, place0 + min(i, m - 1), y);
-  };
-  int need = CACHE8_LOWEST;
-  for (int i0 = 0; i0 < m; i0 += 4 * HPW) {
-    entries(i0 + wave * HPW + sub);
-    if (i0 + wave * HPW + sub < m) {
-#pragma unroll
-      for (int e = 0; e < VK_VEC; ++e) need = max(need, is_v ? least_exponent(v[e]) : least_exponent(k[e]));
-    }
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) need = max(need, __shfl_xor(need, off));
-  if (lane == 0) wave_need[wave] = need;
-  float* scale = a.scales + block * 2 + (is_v ? 1 : 0);
+  const int64_t head_page = (int64_t)page * a.nkv + head;
+  float* scale = a.scales + head_page * 2 + (is_v ? 1 : 0);
   const int stood = exponent_of(*scale), old = off0 > 0 ? stood : CACHE8_LOWEST;
+
+  double* y = reinterpret_cast<double*>(lds) + (wave * HPW + sub) * LPH * VK_VEC;
+  float* held = reinterpret_cast<float*>(lds + STORE8_TURN * sizeof(double));
+  // Rows i0 .. i0 + a.held - 1 into LDS: values as they are, keys normed and turned.  Returns the exponent that this lane's need.
+  auto entries = [&](int i0, bool angles) {
+    int need = CACHE8_LOWEST;
+    const int end = min(m, i0 + a.held);
+    for (int r0 = i0; r0 < end; r0 += ROWS) {
+      const int i = r0 + wave * HPW + sub;
+      float v[VK_VEC];
+#pragma unroll
+      for (int e = 0; e < VK_VEC; ++e) v[e] = next[e];
+      ask(i + ROWS);
+      if (!is_v) {
+        double k[VK_VEC];
+#pragma unroll
+        for (int e = 0; e < VK_VEC; ++e) k[e] = (double)v[e];
+        if (a.cos_t != nullptr && (angles || r0 > i0)) read_angles(a, c0, place0 + min(i, m - 1), t);
+        norm_and_turn<LPH>(k, a, a.k_w != nullptr, t, c0, y);
+#pragma unroll
+        for (int e = 0; e < VK_VEC; ++e) v[e] = round_to_odd(k[e]);
+      }
+      if (i < end && inside) {
+#pragma unroll
+        for (int e = 0; e < VK_VEC; ++e) {
+          need = max(need, least_exponent(v[e]));
+          held[(i - i0) * d + c0 + e] = v[e];
+        }
+      }
+    }
+    return need;
+  };
+  int need = entries(0, false);
+  for (int i0 = a.held; i0 < m; i0 += a.held) {       // more rows than LDS holds: their maximum first, and once more for their entries
+    __syncthreads();
+    ask(i0 + wave * HPW + sub);
+    need = max(need, entries(i0, true));
+  }
+  need = (int)wave_max_xor((float)need);
+  if (lane == 0) wave_need[wave] = need;
   __syncthreads();
   const int now = max(max(old, max(wave_need[0], wave_need[1])), max(wave_need[2], wave_need[3]));
 
-  uint8_t* kp = a.kc + block * P * d;
-  uint8_t* vp = a.vc + block * P * d;
-  const int ts = P + 4;
-  for (int i0 = 0; i0 < m; i0 += 4 * HPW) {
-    const int i = i0 + wave * HPW + sub;
-    if (m > 4 * HPW) entries(i);                      // else they are still there
-    if (i >= m || !inside) continue;
-    uint32_t b[VK_VEC / 4];
-#pragma unroll
-    for (int e = 0; e < VK_VEC; e += 4)
-      b[e / 4] = is_v ? to_fp8x4(entry_of(v[e], now), entry_of(v[e + 1], now), entry_of(v[e + 2], now), entry_of(v[e + 3], now))
-                      : to_fp8x4(entry_of(k[e], now), entry_of(k[e + 1], now), entry_of(k[e + 2], now), entry_of(k[e + 3], now));
-    if (!is_v) {
-      uint32_t* to = reinterpret_cast<uint32_t*>(kp + (off0 + i) * d + c0);
-#pragma unroll
-      for (int e = 0; e < VK_VEC / 4; ++e) to[e] = b[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < VK_VEC; ++e) {
-        const uint8_t one = b[e / 4] >> (8 * (e & 3));
-        if (m == 1) vp[(c0 + e) * P + off0] = one;
-        else turned[(c0 + e) * ts + off0 + i] = one;
-      }
+  uint8_t* kp = a.kc + head_page * P * d;
+  uint8_t* vp = a.vc + head_page * P * d;
+  for (int i0 = 0; i0 < m; i0 += a.held) {
+    const int n = min(a.held, m - i0), at = off0 + i0;           // rows in LDS, and the place in the page of the first
+    if (m > a.held) {
+      __syncthreads();
+      ask(i0 + wave * HPW + sub);
+      (void)entries(i0, true);
+      __syncthreads();
     }
-  }
-  if (is_v && m > 1) {
-    __syncthreads();
-    for (int x = threadIdx.x; x < d * (P >> 4); x += STORE8_THREADS) {
-      const int c = x / (P >> 4), o = (x % (P >> 4)) << 4;
-      if (o + 16 <= off0 || o >= off0 + m) continue;
-      const uint8_t* from = turned + c * ts + o;
-      if (o >= off0 && o + 16 <= off0 + m) {
-        const uint32_t* f = reinterpret_cast<const uint32_t*>(from);
-        *reinterpret_cast<u32x4*>(vp + c * P + o) = u32x4{f[0], f[1], f[2], f[3]};
-      } else {
-        for (int b = max(0, off0 - o); b < min(16, off0 + m - o); ++b) vp[c * P + o + b] = from[b];
+    if (!is_v) {
+      for (int x = threadIdx.x; x < n * d / 16; x += STORE8_THREADS) {
+        const float* from = held + x * 16;
+        u32x4 b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = to_fp8x4(entry_of(from[4 * e], now), entry_of(from[4 * e + 1], now), entry_of(from[4 * e + 2], now), entry_of(from[4 * e + 3], now));
+        *reinterpret_cast<u32x4*>(kp + at * d + x * 16) = b;
+      }
+    } else {
+      // Sixteen places of an entry: neighbouring threads take neighbouring entries, which lie side by side in LDS.
+      const int o0 = at & ~15, chunks = (at + n - o0 + 15) >> 4;
+      constexpr int WIDE = LPH * VK_VEC;              // d, filled up to a power of two
+      const int c = threadIdx.x % WIDE;
+      for (int x = threadIdx.x / WIDE; x < (c < d ? chunks : 0); x += STORE8_THREADS / WIDE) {
+        const int o = o0 + (x << 4);
+        if (o >= at && o + 16 <= at + n) {
+          const float* from = held + (o - at) * d + c;
+          u32x4 b;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            b[e] = to_fp8x4(entry_of(from[4 * e * d], now), entry_of(from[(4 * e + 1) * d], now), entry_of(from[(4 * e + 2) * d], now), entry_of(from[(4 * e + 3) * d], now));
+          *reinterpret_cast<u32x4*>(vp + c * P + o) = b;
+        } else {
+          for (int b = max(at, o); b < min(at + n, o + 16); ++b) vp[c * P + b] = (uint8_t)to_fp8x4(entry_of(held[(b - at) * d + c], now), 0.f, 0.f, 0.f);
+        }
       }
     }
   }
@@ -273,19 +362,28 @@ int vk_qkv_post8(const elem_t* qkv, int64_t row_stride, elem_t* q_out, uint8_t* 
   VK_REQUIRE(max_k_len >= 0 && (nkv == 0 || (int64_t)W * P >= max_k_len), "qkv_post8: a table of %d pages of %d does not cover %d keys", W, P, max_k_len);
   if (T == 0 || S == 0) return 0;
   VK_REQUIRE(((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)kc | (uintptr_t)vc) % 16 == 0, "qkv_post8: rows and cache have to lie on 16 bytes");
-  Store8Args a{qkv, row_stride, q_out, kc, vc, scales, q_w, k_w, w_is_f32, cos_t, sin_t, rot_half, table, cu_q, k_len, W, T, S, nq, nkv, d, P, 0, pages, 0,
-               max_k_len, eps};
+  Store8Args a{qkv, row_stride, q_out, kc, vc, scales, q_w, k_w, w_is_f32, cos_t, sin_t, rot_half, 0, table, cu_q, k_len, W, T, S, nq, nkv, d, P, 0, pages, 0, 0,
+               max_k_len, eps, 1.0 / d};
   while (1 << a.lp < P) ++a.lp;
+  a.whole = rot_half % VK_VEC == 0 && ((uintptr_t)q_w | (uintptr_t)k_w | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16 == 0;
   // Pages that n rows of a sequence touch: n at most, and (n - 1) / P + 2.
-  a.kv_jobs = nkv > 0 ? (int)min((int64_t)T, (int64_t)T / P + 2 * (int64_t)S) : 0;
-  const int64_t blocks = (int64_t)a.kv_jobs * nkv * 2 + (nq > 0 ? T : 0);
-  VK_REQUIRE(blocks < (1ll << 31), "qkv_post8: %d rows of %d heads are too many for one launch", T, nq + 2 * nkv);
-  const size_t lds = nkv > 0 ? (size_t)d * (P + 4) : 0;
+  const int64_t jobs = nkv > 0 ? min((int64_t)T, (int64_t)T / P + 2 * (int64_t)S) : 0, kv_blocks = jobs * nkv * 2, q_blocks = nq > 0 ? T : 0;
+  VK_REQUIRE(kv_blocks + q_blocks < (1ll << 31), "qkv_post8: %d rows of %d heads are too many for one launch", T, nq + 2 * nkv);
+  a.kv_blocks = (int)kv_blocks;
+  // Rows that a workgroup holds in LDS: a page's, up to 32 KB, and one where every sequence has one.
+  a.held = T <= S ? 1 : min(P, 32 * 1024 / 4 / d);
+  const int lds_q = STORE8_TURN * (int)sizeof(float), lds_kv = STORE8_TURN * (int)sizeof(double) + a.held * d * 4;
   const int vecs = d / VK_VEC;
-#define STORE8(L)                                                                                                                         \
-  {                                                                                                                                       \
-    if (lds > 48 * 1024) (void)hipFuncSetAttribute((const void*)store8_kernel<L>, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024); \
-    store8_kernel<L><<<(unsigned)blocks, STORE8_THREADS, lds, st>>>(a);                                                                   \
+  // Many rows: the q heads' workgroups apart, so that they do not take the LDS that the others need.
+  const bool apart = kv_blocks > 0 && q_blocks >= 2048;
+#define STORE8(L)                                                                                                                          \
+  {                                                                                                                                        \
+    if (apart) {                                                                                                                           \
+      store8_kernel<L><<<(unsigned)kv_blocks, STORE8_THREADS, lds_kv, st>>>(a, 0);                                                         \
+      store8_kernel<L><<<(unsigned)q_blocks, STORE8_THREADS, lds_q, st>>>(a, (int)kv_blocks);                                              \
+    } else {                                                                                                                               \
+      store8_kernel<L><<<(unsigned)(kv_blocks + q_blocks), STORE8_THREADS, kv_blocks > 0 ? lds_kv : lds_q, st>>>(a, 0);                    \
+    }                                                                                                                                      \
   }
 #ifdef VK_BF16
   if (vecs <= 2) STORE8(2)
