@@ -23,7 +23,7 @@ def floats(values):
 
 
 def check(name, logits, ids, cu, draft_logits=None, temps=None, accept_u=None, draw_u=None):
-    """Tokens and counts are the definition's; the chances are off by their rounding to 32 bits and by the exponentials' 3e-13."""
+    """Tokens and counts are the definition's; the chances are off by their rounding to 32 bits and by the exponentials' 1.1e-12."""
     k = kernels_for(name)
     dev = lambda x: None if x is None else floats(x)   # noqa: E731
     got = k.verify(logits, ints(ids), ints(cu), draft_logits=draft_logits, temps=dev(temps), accept_uniforms=dev(accept_u), draw_uniforms=dev(draw_u))

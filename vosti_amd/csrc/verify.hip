@@ -9,7 +9,7 @@
 //   running sum over 0..j exceeds (the sequence's random number) * (the sum over all).
 //
 // Everything behind the logits is 64-bit.  The drawn token is the one in whose share of the line the number lies, and 150,000 shares stand
-// in the line: sums of 32-bit terms would move its borders by some 1e-9 of it each, and one token in some thousand draws would be another one.  The vector unit's
+// in the line: sums of 32-bit terms would move its borders by some 1e-9 of it each, and one token in some thousand draws would be another one; the exponentials' 1e-12 moves one in ten million.  The vector unit's
 // 64-bit fused multiply-adds are as fast as its 32-bit ones.
 //
 // Three launches: maximum and sum of pieces of every row; which tokens stand, and what each piece of the row behind them weighs; the piece and the token in it.  Pieces
@@ -18,13 +18,13 @@
 #include "sampling.h"
 
 #define VERIFY_THREADS 256
-#define VERIFY_PIECE 8192                    // logits a workgroup takes of a row
+#define VERIFY_PIECE 4096                    // logits a workgroup takes of a row
 #define VERIFY_VEC (16 / (int)sizeof(elem_t))
 #define VERIFY_ITER (VERIFY_PIECE / VERIFY_VEC / VERIFY_THREADS)
 
 typedef u32x4 __attribute__((aligned(sizeof(elem_t)))) u32x4_any;      // rows of odd length begin anywhere
 
-struct VerifyPart {                          // of a piece of a row: its maximum, where that is first, the sum of exp((x - maximum) / T)
+struct VerifyPart {                          // of a piece of a row: its maximum, the sum of exp((x - maximum) / T), or else where the maximum is first
   float top;
   int at;
   double sum;
@@ -53,40 +53,64 @@ struct VerifyArgs {
   int R, D, S, V, pieces;
 };
 
-// e^x for x <= 0, 0 below -700 and for NaN: 2^k times the Taylor polynomial of degree 10 on |r| <= ln 2 / 2, which is off by 3e-13 of it.
-__device__ __forceinline__ double exp_down(double x) {
-  const double k = __builtin_rint(x * 1.4426950408889634);
-  const double r = __builtin_fma(-k, 0.6931471805599453, x);
-  double p = 1.0 / 3628800;
-  p = __builtin_fma(p, r, 1.0 / 362880);
-  p = __builtin_fma(p, r, 1.0 / 40320);
-  p = __builtin_fma(p, r, 1.0 / 5040);
-  p = __builtin_fma(p, r, 1.0 / 720);
-  p = __builtin_fma(p, r, 1.0 / 120);
-  p = __builtin_fma(p, r, 1.0 / 24);
-  p = __builtin_fma(p, r, 1.0 / 6);
-  p = __builtin_fma(p, r, 0.5);
-  p = __builtin_fma(p, r, 1.0);
-  p = __builtin_fma(p, r, 1.0);
-  const uint64_t two = (uint64_t)((int)k + 1023) << 52;
-  return x > -700.0 ? p * __builtin_bit_cast(double, two) : 0.0;
+// 2^t for t <= 0, and 0 for NaN: 2^k, k the nearest whole number, times the polynomial of degree 8 that meets 2^f at the nine Chebyshev points of |f| <= 1/2; it is off by
+// 1.1e-12 of it.  k is what the addition of 1.5 * 2^52 leaves in the last bits.
+#define VERIFY_LOG2E 1.4426950408889634
+// a * b + c with c in scalar registers.  The compiler's own form adds onto a copy of c that it makes for every addition, two moves of it (103 -> 82 us where 576 rows of 151,936
+// logits are summed).
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
+}
+__device__ __forceinline__ double exp2_down(double t) {
+  const double big = 6755399441055744.0, low = fmax(t, -2000.0), sum = low + big, f = low - (sum - big);
+  double p = fma_const(f, 1.3255224887698904e-06, 1.5310079402479794e-05);
+  p = fma_const(p, f, 0.00015403455852411408);
+  p = fma_const(p, f, 0.0013333450567999659);
+  p = fma_const(p, f, 0.00961812915940262);
+  p = fma_const(p, f, 0.05550410941205934);
+  p = fma_const(p, f, 0.2402265069581299);
+  p = fma_const(p, f, 0.6931471805459335);
+  p = fma_const(p, f, 1.0);
+  return __builtin_ldexp(p, (int)(uint32_t)__builtin_bit_cast(uint64_t, sum));
 }
 
-// VERIFY_VEC logits from x[i] on as numbers; those that the row does not have are -infinity.
-__device__ __forceinline__ void load_logits(const elem_t* x, int i, int V, float (&out)[VERIFY_VEC]) {
-  if (i + VERIFY_VEC <= V) {
-    const u32x4 raw = *reinterpret_cast<const u32x4_any*>(x + i);
+// The vector of logits from x[j] on; where the row ends inside it, its last whole vector (from `at` on, below j), so that a vector is one load anywhere.  Rows shorter than a vector are read one
+// by one.
+struct VerifyVec {
+  u32x4 raw;
+  int at;
+};
+__device__ __forceinline__ VerifyVec load_vec(const elem_t* x, int j, int V) {
+  VerifyVec v;
+  if (V >= VERIFY_VEC) {
+    v.at = min(j, V - VERIFY_VEC);
+    v.raw = *reinterpret_cast<const u32x4_any*>(x + v.at);
+  } else {
+    v.at = j;
 #pragma unroll
-    for (int e = 0; e < VERIFY_VEC; ++e) {
+    for (int e = 0; e < 4; ++e) {
 #ifdef VK_BF16
-      out[e] = __builtin_bit_cast(float, (e & 1) ? raw[e / 2] & 0xffff0000u : raw[e / 2] << 16);
+      const uint32_t lo = j + 2 * e < V ? __builtin_bit_cast(uint16_t, x[j + 2 * e]) : 0xff80u, hi = j + 2 * e + 1 < V ? __builtin_bit_cast(uint16_t, x[j + 2 * e + 1]) : 0xff80u;
+      v.raw[e] = lo | hi << 16;
 #else
-      out[e] = __builtin_bit_cast(float, (uint32_t)raw[e]);
+      v.raw[e] = j + e < V ? __builtin_bit_cast(uint32_t, x[j + e]) : 0xff800000u;
 #endif
     }
-  } else {
+  }
+  return v;
+}
+// Its numbers: element e is the logit v.at + e, or -infinity where that lies before j, in another vector.
+__device__ __forceinline__ void numbers_of(const VerifyVec& v, int j, float (&out)[VERIFY_VEC]) {
 #pragma unroll
-    for (int e = 0; e < VERIFY_VEC; ++e) out[e] = i + e < V ? to_f32(x[i + e]) : -INFINITY;
+  for (int e = 0; e < VERIFY_VEC; ++e) {
+#ifdef VK_BF16
+    const float x = __builtin_bit_cast(float, (e & 1) ? v.raw[e / 2] & 0xffff0000u : v.raw[e / 2] << 16);
+#else
+    const float x = __builtin_bit_cast(float, (uint32_t)v.raw[e]);
+#endif
+    out[e] = v.at + e >= j ? x : -INFINITY;
   }
 }
 
@@ -112,9 +136,9 @@ __device__ __forceinline__ int drafts_of(const VerifyArgs& a, int base, int& fir
   seen += __builtin_popcountll(some);
   return rows > 0 && first >= 0 && first + rows <= a.R && draft >= 0 && draft + rows - 1 <= a.D ? rows - 1 : -1;
 }
-__device__ __forceinline__ double per_temperature(const VerifyArgs& a, int seq) {        // 0: the maximum alone
+__device__ __forceinline__ double per_temperature(const VerifyArgs& a, int seq) {        // log2(e) / T; 0: the maximum alone
   const float t = a.temps != nullptr ? a.temps[seq] : 0.f;
-  return t > 0.f ? fmax(1.0 / (double)t, 1e-300) : 0.0;                                // an infinite one: every finite logit weighs the same
+  return t > 0.f ? fmax(VERIFY_LOG2E / (double)t, 1e-300) : 0.0;                       // an infinite one: every finite logit weighs the same
 }
 __device__ __forceinline__ bool is_finite(float x) { return (__builtin_bit_cast(uint32_t, x) >> 23 & 255) != 255; }
 
@@ -134,11 +158,15 @@ __global__ __launch_bounds__(VERIFY_THREADS) void verify_parts_kernel(VerifyArgs
   if (seq < 0) return;
   const double per_t = per_temperature(a, seq);
   const elem_t* x = drafted ? a.drafts + (int64_t)(row - a.R) * a.V : a.logits + (int64_t)row * a.V;
+  VerifyVec raw[VERIFY_ITER];
   float v[VERIFY_ITER][VERIFY_VEC];
   float top = -INFINITY;
   bool nan = false;
+  const int j0 = piece * VERIFY_PIECE + tid * VERIFY_VEC;
 #pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i) load_logits(x, piece * VERIFY_PIECE + (i * VERIFY_THREADS + tid) * VERIFY_VEC, a.V, v[i]);
+  for (int i = 0; i < VERIFY_ITER; ++i) raw[i] = load_vec(x, j0 + i * VERIFY_THREADS * VERIFY_VEC, a.V);
+#pragma unroll
+  for (int i = 0; i < VERIFY_ITER; ++i) numbers_of(raw[i], j0 + i * VERIFY_THREADS * VERIFY_VEC, v[i]);
 #pragma unroll
   for (int i = 0; i < VERIFY_ITER; ++i)
 #pragma unroll
@@ -155,15 +183,21 @@ __global__ __launch_bounds__(VERIFY_THREADS) void verify_parts_kernel(VerifyArgs
   nan = (s_nan[0] | s_nan[1] | s_nan[2] | s_nan[3]) != 0;
   int at = 0x7fffffff;
   double sum = 0.0;
-  const bool sums = per_t > 0.0 && !nan && is_finite(top);
+  // Where a piece's maximum is not finite the row's is not, or comes from another piece.
+  if (per_t > 0.0 && !nan && is_finite(top)) {
 #pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i)
+    for (int i = 0; i < VERIFY_ITER; ++i)
 #pragma unroll
-    for (int e = 0; e < VERIFY_VEC; ++e) {
-      const int j = piece * VERIFY_PIECE + (i * VERIFY_THREADS + tid) * VERIFY_VEC + e;
-      if (j < a.V && (nan ? v[i][e] != v[i][e] : v[i][e] == top)) at = min(at, j);
-      if (sums) sum = sum + exp_down(((double)v[i][e] - (double)top) * per_t);
-    }
+      for (int e = 0; e < VERIFY_VEC; ++e) sum = sum + exp2_down(((double)v[i][e] - (double)top) * per_t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VERIFY_ITER; ++i)
+#pragma unroll
+      for (int e = 0; e < VERIFY_VEC; ++e) {
+        const int from = j0 + i * VERIFY_THREADS * VERIFY_VEC, j = raw[i].at + e;
+        if (j >= from && j < a.V && (nan ? v[i][e] != v[i][e] : v[i][e] == top)) at = min(at, j);
+      }
+  }
   at = wave_min_i(at);
   sum = wave_sum_d(sum);
   if (lane == 0) {
@@ -190,7 +224,7 @@ __device__ __forceinline__ VerifyRow join_row(const VerifyArgs& a, int row, doub
   nan = __any(nan);
   if (per_t > 0.0 && !nan && is_finite(top)) {
     double sum = 0.0;
-    for (int c = lane; c < a.pieces; c += 64) sum = sum + parts[c].sum * exp_down(((double)parts[c].top - (double)top) * per_t);
+    for (int c = lane; c < a.pieces; c += 64) sum = sum + parts[c].sum * exp2_down(((double)parts[c].top - (double)top) * per_t);
     return VerifyRow{1.0 / wave_sum_d(sum), top, -1};
   }
   int at = 0x7fffffff;
@@ -199,20 +233,43 @@ __device__ __forceinline__ VerifyRow join_row(const VerifyArgs& a, int row, doub
   return VerifyRow{0.0, top, wave_min_i(at)};
 }
 __device__ __forceinline__ double chance(const VerifyRow& r, int j, float x, double per_t) {
-  return r.at >= 0 ? (j == r.at ? 1.0 : 0.0) : exp_down(((double)x - (double)r.top) * per_t) * r.scale;
+  return r.at >= 0 ? (j == r.at ? 1.0 : 0.0) : exp2_down(((double)x - (double)r.top) * per_t) * r.scale;
 }
 
-// p and max(p - q, 0) of the logits from j on.
-__device__ __forceinline__ void weights_of(const VerifyArgs& a, const VerifySeq& s, int j, double (&whole)[VERIFY_VEC], double (&left)[VERIFY_VEC]) {
-  float x[VERIFY_VEC], y[VERIFY_VEC];
-  load_logits(a.logits + (int64_t)s.row * a.V, j, a.V, x);
-  if (s.draft >= 0 && s.q.at < 0) load_logits(a.drafts + (int64_t)s.draft * a.V, j, a.V, y);
+// p and max(p - q, 0) of N vectors of logits, the i-th from j[i] on; at[i]: the logit that its first element is (those before j[i] weigh nothing).
+template <int N>
+__device__ __forceinline__ void weights_of(const VerifyArgs& a, const VerifySeq& s, const int (&j)[N], int (&at)[N], double (&whole)[N][VERIFY_VEC], double (&left)[N][VERIFY_VEC]) {
+  const bool drawn = s.draft >= 0 && s.q.at < 0;
+  VerifyVec vx[N], vy[N];
 #pragma unroll
-  for (int e = 0; e < VERIFY_VEC; ++e) {
-    const double p = exp_down(((double)x[e] - (double)s.p.top) * s.per_t) * s.p.scale;
-    const double q = s.draft < 0 ? 0.0 : s.q.at >= 0 ? (j + e == s.q.at ? 1.0 : 0.0) : exp_down(((double)y[e] - (double)s.q.top) * s.per_t) * s.q.scale;
-    whole[e] = p;
-    left[e] = fmax(p - q, 0.0);
+  for (int i = 0; i < N; ++i) {
+    vx[i] = load_vec(a.logits + (int64_t)s.row * a.V, j[i], a.V);
+    at[i] = vx[i].at;
+  }
+  if (drawn) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) vy[i] = load_vec(a.drafts + (int64_t)s.draft * a.V, j[i], a.V);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float x[VERIFY_VEC];
+    numbers_of(vx[i], j[i], x);
+#pragma unroll
+    for (int e = 0; e < VERIFY_VEC; ++e) whole[i][e] = exp2_down(((double)x[e] - (double)s.p.top) * s.per_t) * s.p.scale;
+  }
+  if (drawn) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float y[VERIFY_VEC];
+      numbers_of(vy[i], j[i], y);
+#pragma unroll
+      for (int e = 0; e < VERIFY_VEC; ++e) left[i][e] = fmax(whole[i][e] - exp2_down(((double)y[e] - (double)s.q.top) * s.per_t) * s.q.scale, 0.0);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < VERIFY_VEC; ++e) left[i][e] = s.draft >= 0 && at[i] + e == s.q.at ? 0.0 : whole[i][e];        // q is 1 there, and p at most
   }
 }
 
@@ -279,19 +336,18 @@ __global__ __launch_bounds__(VERIFY_THREADS) void verify_weigh_kernel(VerifyArgs
     }
   }
   if (s.p.at >= 0) return;
-  double left = 0.0, whole = 0.0;
+  double left = 0.0, whole = 0.0, w[VERIFY_ITER][VERIFY_VEC], l[VERIFY_ITER][VERIFY_VEC];
+  int j[VERIFY_ITER], at[VERIFY_ITER];
 #pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i) {
-    const int j = piece * VERIFY_PIECE + (i * VERIFY_THREADS + tid) * VERIFY_VEC;
-    if (j >= a.V) break;
-    double w[VERIFY_VEC], l[VERIFY_VEC];
-    weights_of(a, s, j, w, l);
+  for (int i = 0; i < VERIFY_ITER; ++i) j[i] = piece * VERIFY_PIECE + (i * VERIFY_THREADS + tid) * VERIFY_VEC;
+  weights_of<VERIFY_ITER>(a, s, j, at, w, l);
+#pragma unroll
+  for (int i = 0; i < VERIFY_ITER; ++i)
 #pragma unroll
     for (int e = 0; e < VERIFY_VEC; ++e) {
-      whole = whole + w[e];
-      left = left + l[e];
+      whole = whole + w[i][e];
+      left = left + l[i][e];
     }
-  }
   left = wave_sum_d(left);
   whole = wave_sum_d(whole);
   if (lane == 0) {
@@ -308,49 +364,60 @@ __global__ __launch_bounds__(VERIFY_THREADS) void verify_draw_kernel(VerifyArgs 
   const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const VerifySeq s = a.seqs[seq];
   if (s.row < 0 || s.p.at >= 0) return;
+  // A lane a piece, 64 at a time: running sums over them, the first that ends beyond the target, else (the target is the end, by rounding) the last that weighs
+  // anything.  Every wave for itself.
   const VerifySums* sums = a.sums + (int64_t)seq * a.pieces;
   double all = 0.0, all_whole = 0.0;
-  for (int c = 0; c < a.pieces; ++c) {
-    all = all + sums[c].left;
-    all_whole = all_whole + sums[c].whole;
+  for (int c0 = 0; c0 < a.pieces; c0 += 64) {
+    const VerifySums mine = c0 + lane < a.pieces ? sums[c0 + lane] : VerifySums{0.0, 0.0};
+    all = all + wave_sum_d(mine.left);
+    all_whole = all_whole + wave_sum_d(mine.whole);
   }
   const bool use_left = all > 0.0;
   const double target = (double)a.draw_u[seq] * (use_left ? all : all_whole);
-  // The piece: the first whose end lies beyond the target, else (the target is the end, by rounding) the last that weighs anything.
   int piece = -1, last = 0;
   double before = 0.0, run = 0.0, last_before = 0.0;
-  for (int c = 0; c < a.pieces; ++c) {
-    const double w = use_left ? sums[c].left : sums[c].whole;
-    if (w > 0.0) {
-      last = c;
-      last_before = run;
+  for (int c0 = 0; c0 < a.pieces && piece < 0; c0 += 64) {
+    const VerifySums mine = c0 + lane < a.pieces ? sums[c0 + lane] : VerifySums{0.0, 0.0};
+    const double w = use_left ? mine.left : mine.whole;
+    double upto = w;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const double t = __shfl_up(upto, off);
+      if (lane >= off) upto = upto + t;
     }
-    if (piece < 0 && target < run + w) {
-      piece = c;
-      before = run;
+    const double begin = run + (upto - w);
+    const uint64_t beyond = __ballot(w > 0.0 && target < run + upto), some = __ballot(w > 0.0);
+    if (beyond != 0) {
+      const int l = __builtin_ctzll(beyond);
+      piece = c0 + l;
+      before = __shfl(begin, l);
     }
-    run = run + w;
+    if (some != 0) {
+      const int l = 63 - __builtin_clzll(some);
+      last = c0 + l;
+      last_before = __shfl(begin, l);
+    }
+    run = run + __shfl(upto, 63);
   }
   if (piece < 0) {
     piece = last;
     before = last_before;
   }
   // The token in it: a thread has as many neighbouring logits as it has vectors of them.
-  double w[VERIFY_ITER][VERIFY_VEC];
-  double sum = 0.0;
-  const int j0 = piece * VERIFY_PIECE + tid * VERIFY_ITER * VERIFY_VEC;
-  int my_last = -1;
+  double w[VERIFY_ITER][VERIFY_VEC], l[VERIFY_ITER][VERIFY_VEC], sum = 0.0;
+  int j[VERIFY_ITER], at[VERIFY_ITER], my_last = -1;
 #pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i) {
-    double whole[VERIFY_VEC], left[VERIFY_VEC];
-    weights_of(a, s, j0 + i * VERIFY_VEC, whole, left);
+  for (int i = 0; i < VERIFY_ITER; ++i) j[i] = piece * VERIFY_PIECE + (tid * VERIFY_ITER + i) * VERIFY_VEC;
+  weights_of<VERIFY_ITER>(a, s, j, at, w, l);
+#pragma unroll
+  for (int i = 0; i < VERIFY_ITER; ++i)
 #pragma unroll
     for (int e = 0; e < VERIFY_VEC; ++e) {
-      w[i][e] = use_left ? left[e] : whole[e];
+      w[i][e] = use_left ? l[i][e] : w[i][e];
       sum = sum + w[i][e];
-      if (w[i][e] > 0.0) my_last = j0 + i * VERIFY_VEC + e;
+      if (w[i][e] > 0.0) my_last = at[i] + e;
     }
-  }
   double upto = sum;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -371,7 +438,7 @@ __global__ __launch_bounds__(VERIFY_THREADS) void verify_draw_kernel(VerifyArgs 
 #pragma unroll
     for (int e = 0; e < VERIFY_VEC; ++e) {
       start = start + w[i][e];
-      if (w[i][e] > 0.0 && target < start) pick = min(pick, j0 + i * VERIFY_VEC + e);
+      if (w[i][e] > 0.0 && target < start) pick = min(pick, at[i] + e);
     }
   if (pick != 0x7fffffff) atomicMin(&s_pick, pick);
   __syncthreads();
