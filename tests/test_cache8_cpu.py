@@ -58,7 +58,7 @@ def ver(kernels, tokens=GOOD, logits=GOOD, ids=GOOD, temps=None, au=None, du=Non
 
 
 @pytest.mark.parametrize("bad", [dict(R=-1), dict(D=-1), dict(S=-1), dict(V=0), dict(V=1 << 30), dict(temps=GOOD), dict(temps=GOOD, du=GOOD), dict(temps=GOOD, au=GOOD), dict(tokens=None),
-                                 dict(logits=None), dict(ids=None), dict(scratch=None), dict(scratch=GOOD + 8), dict(size=100), dict(V=600_000_000, size=1 << 60)])
+                                 dict(logits=None), dict(ids=None), dict(scratch=None), dict(scratch=GOOD + 8), dict(size=100), dict(V=(1 << 30) - 1, size=1 << 60)])
 def test_verification_refuses(kernels, bad):
     assert "verify" in refused(kernels, *ver(kernels, **bad))
 

@@ -156,6 +156,34 @@ __device__ __forceinline__ float wave_sum_xor(float v) {
   v = v + wave_partner<2>(v);
   return v + wave_partner<1>(v);
 }
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, true), hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// The value of lane l ^ 32 (l ^ 16) plus one's own.
+__device__ __forceinline__ double add_xor32(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t a = (uint32_t)u, b = (uint32_t)(u >> 32);
+  const auto lo = __builtin_amdgcn_permlane32_swap(a, a, false, false), hi = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  const uint32_t l0 = lo[0], l1 = lo[1], h0 = hi[0], h1 = hi[1];
+  return __builtin_bit_cast(double, (uint64_t)h0 << 32 | l0) + __builtin_bit_cast(double, (uint64_t)h1 << 32 | l1);
+}
+__device__ __forceinline__ double add_xor16(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t a = (uint32_t)u, b = (uint32_t)(u >> 32);
+  const auto lo = __builtin_amdgcn_permlane16_swap(a, a, false, false), hi = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  const uint32_t l0 = lo[0], l1 = lo[1], h0 = hi[0], h1 = hi[1];
+  return __builtin_bit_cast(double, (uint64_t)h0 << 32 | l0) + __builtin_bit_cast(double, (uint64_t)h1 << 32 | l1);
+}
+__device__ __forceinline__ double wave_sum_xor(double v) {
+  v = add_xor16(add_xor32(v));
+  v = v + dpp_d<0x128>(v);        // row_ror:8, row_ror:4 and the quads, as above
+  v = v + dpp_d<0x124>(v);
+  v = v + dpp_d<0x4E>(v);
+  return v + dpp_d<0xB1>(v);
+}
 __device__ __forceinline__ float wave_max_xor(float v) {
   v = fmaxf(v, wave_partner<32>(v));
   v = fmaxf(v, wave_partner<16>(v));

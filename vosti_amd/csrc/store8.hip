@@ -38,20 +38,14 @@ struct Store8Args {
 // Sum over the LPH neighbouring lanes of a head; the order is fixed by LPH.
 template <int LPH>
 __device__ __forceinline__ float head_sum(float v) { return group_sum<LPH>(v); }
-template <int CTRL>
-__device__ __forceinline__ double dpp_d(double v) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, true), hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
 template <int LPH>
 __device__ __forceinline__ double head_sum(double v) {
   if (LPH >= 2) v = v + dpp_d<0xB1>(v);               // quad_perm [1, 0, 3, 2]
   if (LPH >= 4) v = v + dpp_d<0x4E>(v);               // quad_perm [2, 3, 0, 1]
   if (LPH >= 8) v = v + dpp_d<0x141>(v);              // row_half_mirror
   if (LPH >= 16) v = v + dpp_d<0x140>(v);             // row_mirror
-  if (LPH >= 32) v = v + __shfl_xor(v, 16);
-  if (LPH >= 64) v = v + __shfl_xor(v, 32);
+  if (LPH >= 32) v = add_xor16(v);
+  if (LPH >= 64) v = add_xor32(v);
   return v;
 }
 __device__ __forceinline__ float one_over_root(float v) { return rsqrtf(v); }

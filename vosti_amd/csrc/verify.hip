@@ -12,15 +12,15 @@
 // in the line: sums of 32-bit terms would move its borders by some 1e-9 of it each, and one token in some thousand draws would be another one; the exponentials' 1e-12 moves one in ten million.  The vector unit's
 // 64-bit fused multiply-adds are as fast as its 32-bit ones.
 //
-// Three launches: maximum and sum of pieces of every row; which tokens stand, and what each piece of the row behind them weighs; the piece and the token in it.  Pieces
-// have the same borders and their sums the same order whatever else is in the call.
+// Four launches: maximum and sum of pieces of every row, a wave each; which tokens stand, and the distributions behind them; what the pieces of those weigh; the piece and
+// the token in it.  Pieces have the same borders and their sums the same order whatever else is in the call.
 #include "common.h"
 #include "sampling.h"
 
 #define VERIFY_THREADS 256
-#define VERIFY_PIECE 4096                    // logits a workgroup takes of a row
+#define VERIFY_PIECE 2048                    // logits a wave takes of a row
 #define VERIFY_VEC (16 / (int)sizeof(elem_t))
-#define VERIFY_ITER (VERIFY_PIECE / VERIFY_VEC / VERIFY_THREADS)
+#define VERIFY_ITER (VERIFY_PIECE / VERIFY_VEC / 64)
 
 typedef u32x4 __attribute__((aligned(sizeof(elem_t)))) u32x4_any;      // rows of odd length begin anywhere
 
@@ -101,24 +101,27 @@ __device__ __forceinline__ VerifyVec load_vec(const elem_t* x, int j, int V) {
   }
   return v;
 }
-// Its numbers: element e is the logit v.at + e, or -infinity where that lies before j, in another vector.
-__device__ __forceinline__ void numbers_of(const VerifyVec& v, int j, float (&out)[VERIFY_VEC]) {
+// A row's last piece: elements of v that lie before j, in another vector, become -infinity.
+__device__ __forceinline__ void only_own(VerifyVec& v, int j) {
 #pragma unroll
-  for (int e = 0; e < VERIFY_VEC; ++e) {
+  for (int e = 0; e < 4; ++e) {
 #ifdef VK_BF16
-    const float x = __builtin_bit_cast(float, (e & 1) ? v.raw[e / 2] & 0xffff0000u : v.raw[e / 2] << 16);
+    const uint32_t lo = v.at + 2 * e >= j ? v.raw[e] & 0xffffu : 0xff80u, hi = v.at + 2 * e + 1 >= j ? v.raw[e] & 0xffff0000u : 0xff800000u;
+    v.raw[e] = lo | hi;
 #else
-    const float x = __builtin_bit_cast(float, (uint32_t)v.raw[e]);
+    v.raw[e] = v.at + e >= j ? v.raw[e] : 0xff800000u;
 #endif
-    out[e] = v.at + e >= j ? x : -INFINITY;
   }
 }
-
-__device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = v + __shfl_xor(v, off);
-  return v;
+// Its numbers: element e is the logit v.at + e.
+__device__ __forceinline__ float number_of(const VerifyVec& v, int e) {
+#ifdef VK_BF16
+  return __builtin_bit_cast(float, (e & 1) ? v.raw[e / 2] & 0xffff0000u : v.raw[e / 2] << 16);
+#else
+  return __builtin_bit_cast(float, (uint32_t)v.raw[e]);
+#endif
 }
+
 __device__ __forceinline__ int wave_min_i(int v) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) v = min(v, __shfl_xor(v, off));
@@ -143,11 +146,14 @@ __device__ __forceinline__ double per_temperature(const VerifyArgs& a, int seq) 
 __device__ __forceinline__ bool is_finite(float x) { return (__builtin_bit_cast(uint32_t, x) >> 23 & 255) != 255; }
 
 __global__ __launch_bounds__(VERIFY_THREADS) void verify_parts_kernel(VerifyArgs a) {
-  __shared__ float s_top[4];
-  __shared__ int s_at[4], s_nan[4];
-  __shared__ double s_sum[4];
-  const int row = blockIdx.x, piece = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = blockIdx.x, lane = threadIdx.x & 63, piece = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (piece >= a.pieces) return;
   const bool drafted = row >= a.R;
+  const elem_t* x = drafted ? a.drafts + (int64_t)(row - a.R) * a.V : a.logits + (int64_t)row * a.V;
+  const int j0 = piece * VERIFY_PIECE + lane * VERIFY_VEC;
+  VerifyVec raw[VERIFY_ITER];
+#pragma unroll
+  for (int i = 0; i < VERIFY_ITER; ++i) raw[i] = load_vec(x, j0 + i * 64 * VERIFY_VEC, a.V);
   int seq = -1;
   for (int base = 0, seen = 0; base < a.S && seq < 0; base += 64) {
     int first, draft;
@@ -157,30 +163,17 @@ __global__ __launch_bounds__(VERIFY_THREADS) void verify_parts_kernel(VerifyArgs
   }
   if (seq < 0) return;
   const double per_t = per_temperature(a, seq);
-  const elem_t* x = drafted ? a.drafts + (int64_t)(row - a.R) * a.V : a.logits + (int64_t)row * a.V;
-  VerifyVec raw[VERIFY_ITER];
-  float v[VERIFY_ITER][VERIFY_VEC];
+  if ((piece + 1) * VERIFY_PIECE > a.V) {
+#pragma unroll
+    for (int i = 0; i < VERIFY_ITER; ++i) only_own(raw[i], j0 + i * 64 * VERIFY_VEC);
+  }
   float top = -INFINITY;
-  bool nan = false;
-  const int j0 = piece * VERIFY_PIECE + tid * VERIFY_VEC;
-#pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i) raw[i] = load_vec(x, j0 + i * VERIFY_THREADS * VERIFY_VEC, a.V);
-#pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i) numbers_of(raw[i], j0 + i * VERIFY_THREADS * VERIFY_VEC, v[i]);
 #pragma unroll
   for (int i = 0; i < VERIFY_ITER; ++i)
 #pragma unroll
-    for (int e = 0; e < VERIFY_VEC; ++e) {
-      top = fmaxf(top, v[i][e]);
-      nan = nan || v[i][e] != v[i][e];
-    }
+    for (int e = 0; e < VERIFY_VEC; ++e) top = __builtin_elementwise_maximum(top, number_of(raw[i], e));       // NaN where there is one
+  const bool nan = __any(top != top);
   top = wave_max_xor(top);
-  if (lane == 0) s_top[wave] = top;
-  if (lane == 0) s_nan[wave] = 0;
-  if (__any(nan) && lane == 0) s_nan[wave] = 1;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  nan = (s_nan[0] | s_nan[1] | s_nan[2] | s_nan[3]) != 0;
   int at = 0x7fffffff;
   double sum = 0.0;
   // Where a piece's maximum is not finite the row's is not, or comes from another piece.
@@ -188,26 +181,20 @@ __global__ __launch_bounds__(VERIFY_THREADS) void verify_parts_kernel(VerifyArgs
 #pragma unroll
     for (int i = 0; i < VERIFY_ITER; ++i)
 #pragma unroll
-      for (int e = 0; e < VERIFY_VEC; ++e) sum = sum + exp2_down(((double)v[i][e] - (double)top) * per_t);
+      for (int e = 0; e < VERIFY_VEC; ++e) sum = sum + exp2_down(((double)number_of(raw[i], e) - (double)top) * per_t);
+    sum = wave_sum_xor(sum);
   } else {
 #pragma unroll
     for (int i = 0; i < VERIFY_ITER; ++i)
 #pragma unroll
       for (int e = 0; e < VERIFY_VEC; ++e) {
-        const int from = j0 + i * VERIFY_THREADS * VERIFY_VEC, j = raw[i].at + e;
-        if (j >= from && j < a.V && (nan ? v[i][e] != v[i][e] : v[i][e] == top)) at = min(at, j);
+        const float v = number_of(raw[i], e);
+        const int from = j0 + i * 64 * VERIFY_VEC, j = raw[i].at + e;
+        if (j >= from && j < a.V && (nan ? v != v : v == top)) at = min(at, j);
       }
+    at = wave_min_i(at);
   }
-  at = wave_min_i(at);
-  sum = wave_sum_d(sum);
-  if (lane == 0) {
-    s_at[wave] = at;
-    s_sum[wave] = sum;
-  }
-  __syncthreads();
-  if (tid == 0)
-    a.parts[(int64_t)row * a.pieces + piece] =
-        VerifyPart{nan ? NAN : top, min(min(s_at[0], s_at[1]), min(s_at[2], s_at[3])), (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3])};
+  if (lane == 0) a.parts[(int64_t)row * a.pieces + piece] = VerifyPart{nan ? NAN : top, at, sum};
 }
 
 // A row's distribution from its pieces, by a whole wave.
@@ -225,7 +212,7 @@ __device__ __forceinline__ VerifyRow join_row(const VerifyArgs& a, int row, doub
   if (per_t > 0.0 && !nan && is_finite(top)) {
     double sum = 0.0;
     for (int c = lane; c < a.pieces; c += 64) sum = sum + parts[c].sum * exp2_down(((double)parts[c].top - (double)top) * per_t);
-    return VerifyRow{1.0 / wave_sum_d(sum), top, -1};
+    return VerifyRow{1.0 / wave_sum_xor(sum), top, -1};
   }
   int at = 0x7fffffff;
   for (int c = lane; c < a.pieces; c += 64)
@@ -236,9 +223,9 @@ __device__ __forceinline__ double chance(const VerifyRow& r, int j, float x, dou
   return r.at >= 0 ? (j == r.at ? 1.0 : 0.0) : exp2_down(((double)x - (double)r.top) * per_t) * r.scale;
 }
 
-// p and max(p - q, 0) of N vectors of logits, the i-th from j[i] on; at[i]: the logit that its first element is (those before j[i] weigh nothing).
+// p and max(p - q, 0) of N vectors of logits, the i-th from j[i] on; at[i]: the logit that its first element is (those before j[i] weigh nothing).  edge: the row's last piece.
 template <int N>
-__device__ __forceinline__ void weights_of(const VerifyArgs& a, const VerifySeq& s, const int (&j)[N], int (&at)[N], double (&whole)[N][VERIFY_VEC], double (&left)[N][VERIFY_VEC]) {
+__device__ __forceinline__ void weights_of(const VerifyArgs& a, const VerifySeq& s, bool edge, const int (&j)[N], int (&at)[N], double (&whole)[N][VERIFY_VEC], double (&left)[N][VERIFY_VEC]) {
   const bool drawn = s.draft >= 0 && s.q.at < 0;
   VerifyVec vx[N], vy[N];
 #pragma unroll
@@ -250,21 +237,22 @@ __device__ __forceinline__ void weights_of(const VerifyArgs& a, const VerifySeq&
 #pragma unroll
     for (int i = 0; i < N; ++i) vy[i] = load_vec(a.drafts + (int64_t)s.draft * a.V, j[i], a.V);
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float x[VERIFY_VEC];
-    numbers_of(vx[i], j[i], x);
-#pragma unroll
-    for (int e = 0; e < VERIFY_VEC; ++e) whole[i][e] = exp2_down(((double)x[e] - (double)s.p.top) * s.per_t) * s.p.scale;
-  }
-  if (drawn) {
+  if (edge) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      float y[VERIFY_VEC];
-      numbers_of(vy[i], j[i], y);
-#pragma unroll
-      for (int e = 0; e < VERIFY_VEC; ++e) left[i][e] = fmax(whole[i][e] - exp2_down(((double)y[e] - (double)s.q.top) * s.per_t) * s.q.scale, 0.0);
+      only_own(vx[i], j[i]);
+      if (drawn) only_own(vy[i], j[i]);
     }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < VERIFY_VEC; ++e) whole[i][e] = exp2_down(((double)number_of(vx[i], e) - (double)s.p.top) * s.per_t) * s.p.scale;
+  if (drawn) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < VERIFY_VEC; ++e) left[i][e] = fmax(whole[i][e] - exp2_down(((double)number_of(vy[i], e) - (double)s.q.top) * s.per_t) * s.q.scale, 0.0);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -273,92 +261,124 @@ __device__ __forceinline__ void weights_of(const VerifyArgs& a, const VerifySeq&
   }
 }
 
-__global__ __launch_bounds__(VERIFY_THREADS) void verify_weigh_kernel(VerifyArgs a) {
+// Which of a sequence's tokens stand, and what stands behind them: by a workgroup, a wave every fourth row.  write: tokens, counts and chances too.
+#define VERIFY_KEPT 16                       // rows whose distributions stay in LDS until it is known which one is needed
+__device__ __forceinline__ VerifySeq decide(const VerifyArgs& a, int seq, bool write) {
   __shared__ int s_first;
-  __shared__ double s_left[4], s_whole[4];
-  const int seq = blockIdx.x, piece = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ VerifyRow s_p[VERIFY_KEPT], s_q[VERIFY_KEPT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  VerifySeq s;
+  s.row = -1;
+  s.draft = -1;
+  s.per_t = per_temperature(a, seq);
+  s.p = s.q = VerifyRow{0.0, 0.f, -1};
   int n = -1, row0 = 0, draft0 = 0;
   for (int base = 0, seen = 0; base <= seq; base += 64) {
     const int mine = drafts_of(a, base, row0, draft0, seen);
     if (seq < base + 64) {
-      n = __shfl(mine, seq - base);
-      row0 = __shfl(row0, seq - base);
-      draft0 = __shfl(draft0, seq - base);
+      n = __builtin_amdgcn_readlane(mine, seq - base);
+      row0 = __builtin_amdgcn_readlane(row0, seq - base);
+      draft0 = __builtin_amdgcn_readlane(draft0, seq - base);
     }
   }
-  if (n < 0) {
-    if (piece == 0 && tid == 0) {
-      a.counts[seq] = 0;
-      a.seqs[seq].row = -1;
-    }
-    return;
-  }
-  const double per_t = per_temperature(a, seq);
   if (tid == 0) s_first = n;
+  if (n < 0) {
+    if (write && tid == 0) a.counts[seq] = 0;
+    return s;
+  }
   __syncthreads();
-  for (int i = wave; i < n; i += 4) {
-    const int id = a.ids[draft0 + i];
+  for (int i = wave; i <= n; i += 4) {
+    int id = -1;
+    float x = 0.f, y = 0.f, u = 0.f;
+    if (i < n) {
+      id = a.ids[draft0 + i];
+      if (a.accept_u != nullptr) u = a.accept_u[draft0 + i];
+    }
     const bool known = (unsigned)id < (unsigned)a.V;
-    const VerifyRow p = join_row(a, row0 + i, per_t);
-    double pd = 0.0, qd = 0.0;
-    if (known) pd = chance(p, id, to_f32(a.logits[(int64_t)(row0 + i) * a.V + id]), per_t);
-    if (a.drafts != nullptr) {
-      const VerifyRow q = join_row(a, a.R + draft0 + i, per_t);
-      if (known) qd = chance(q, id, to_f32(a.drafts[(int64_t)(draft0 + i) * a.V + id]), per_t);
-    } else if (known) {
-      qd = 1.0;
+    if (known) {
+      x = to_f32(a.logits[(int64_t)(row0 + i) * a.V + id]);
+      if (a.drafts != nullptr) y = to_f32(a.drafts[(int64_t)(draft0 + i) * a.V + id]);
     }
-    const double u = a.accept_u != nullptr ? (double)a.accept_u[draft0 + i] : 0.0;
-    if (lane == 0) {
-      if (!(u * qd < pd)) atomicMin(&s_first, i);
-      if (piece == 0) a.accept[draft0 + i] = (float)(qd > 0.0 ? fmin(1.0, pd / qd) : pd > 0.0 ? 1.0 : 0.0);
+    const VerifyRow p = join_row(a, row0 + i, s.per_t);
+    VerifyRow q{0.0, 0.f, known ? id : 0x7fffffff};
+    if (a.drafts != nullptr && i < n) q = join_row(a, a.R + draft0 + i, s.per_t);
+    if (lane != 0) continue;
+    if (i < VERIFY_KEPT) {
+      s_p[i] = p;
+      s_q[i] = q;
     }
+    if (i == n) continue;
+    const double pd = known ? chance(p, id, x, s.per_t) : 0.0, qd = known ? chance(q, id, y, s.per_t) : 0.0;
+    if (!((double)u * qd < pd)) atomicMin(&s_first, i);
+    if (write) a.accept[draft0 + i] = (float)(qd > 0.0 ? fmin(1.0, pd / qd) : pd > 0.0 ? 1.0 : 0.0);
   }
   __syncthreads();
   const int stand = s_first;
-  VerifySeq s;
   s.row = row0 + stand;
   s.draft = stand < n ? draft0 + stand : -1;
-  s.per_t = per_t;
-  s.p = join_row(a, s.row, per_t);
-  s.q = VerifyRow{0.0, 0.f, -1};
-  if (stand < n) {
-    if (a.drafts != nullptr) s.q = join_row(a, a.R + s.draft, per_t);
-    else s.q.at = (unsigned)a.ids[s.draft] < (unsigned)a.V ? a.ids[s.draft] : 0x7fffffff;
+  if (stand < VERIFY_KEPT) {
+    s.p = s_p[stand];
+    s.q = s_q[stand];
+  } else {
+    s.p = join_row(a, s.row, s.per_t);
+    if (stand < n) {
+      if (a.drafts != nullptr) s.q = join_row(a, a.R + s.draft, s.per_t);
+      else s.q.at = (unsigned)a.ids[s.draft] < (unsigned)a.V ? a.ids[s.draft] : 0x7fffffff;
+    }
   }
-  if (piece == 0) {
+  if (write) {
     for (int i = tid; i <= n; i += VERIFY_THREADS)
       if (i != stand) a.tokens[row0 + i] = i < stand ? a.ids[draft0 + i] : -1;
     if (tid == 0) {
       a.counts[seq] = stand + 1;
-      a.seqs[seq] = s;
       if (s.p.at >= 0) a.tokens[s.row] = s.p.at;         // 1 there: whatever is taken away, it is what is left, or nothing is
     }
   }
-  if (s.p.at >= 0) return;
-  double left = 0.0, whole = 0.0, w[VERIFY_ITER][VERIFY_VEC], l[VERIFY_ITER][VERIFY_VEC];
-  int j[VERIFY_ITER], at[VERIFY_ITER];
-#pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i) j[i] = piece * VERIFY_PIECE + (i * VERIFY_THREADS + tid) * VERIFY_VEC;
-  weights_of<VERIFY_ITER>(a, s, j, at, w, l);
-#pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i)
-#pragma unroll
-    for (int e = 0; e < VERIFY_VEC; ++e) {
-      whole = whole + w[i][e];
-      left = left + l[i][e];
-    }
-  left = wave_sum_d(left);
-  whole = wave_sum_d(whole);
-  if (lane == 0) {
-    s_left[wave] = left;
-    s_whole[wave] = whole;
+  return s;
+}
+
+__global__ __launch_bounds__(VERIFY_THREADS) void verify_decide_kernel(VerifyArgs a) {
+  const VerifySeq s = decide(a, blockIdx.x, true);
+  if (threadIdx.x == 0) a.seqs[blockIdx.x] = s;
+}
+
+// DECIDE: every workgroup decides for itself, in place of a launch of its own.
+template <bool DECIDE>
+__global__ __launch_bounds__(VERIFY_THREADS) void verify_weigh_kernel(VerifyArgs a) {
+  const int seq = blockIdx.x, lane = threadIdx.x & 63, piece = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  VerifySeq s;
+  if (DECIDE) {
+    s = decide(a, seq, blockIdx.y == 0);
+    if (blockIdx.y == 0 && threadIdx.x == 0) a.seqs[seq] = s;
+  } else {
+    s = a.seqs[seq];
   }
-  __syncthreads();
-  if (tid == 0) a.sums[(int64_t)seq * a.pieces + piece] = VerifySums{(s_left[0] + s_left[1]) + (s_left[2] + s_left[3]), (s_whole[0] + s_whole[1]) + (s_whole[2] + s_whole[3])};
+  if (piece >= a.pieces || s.row < 0 || s.p.at >= 0) return;
+  // A quarter of a piece at a time: the 64-bit numbers of more would leave room for fewer waves.
+  constexpr int PART = VERIFY_ITER / 4;
+  double left = 0.0, whole = 0.0;
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    double w[PART][VERIFY_VEC], l[PART][VERIFY_VEC];
+    int j[PART], at[PART];
+#pragma unroll
+    for (int i = 0; i < PART; ++i) j[i] = piece * VERIFY_PIECE + ((h * PART + i) * 64 + lane) * VERIFY_VEC;
+    weights_of<PART>(a, s, (piece + 1) * VERIFY_PIECE > a.V, j, at, w, l);
+#pragma unroll
+    for (int i = 0; i < PART; ++i)
+#pragma unroll
+      for (int e = 0; e < VERIFY_VEC; ++e) {
+        whole = whole + w[i][e];
+        left = left + l[i][e];
+      }
+  }
+  left = wave_sum_xor(left);
+  whole = wave_sum_xor(whole);
+  if (lane == 0) a.sums[(int64_t)seq * a.pieces + piece] = VerifySums{left, whole};
 }
 
 __global__ __launch_bounds__(VERIFY_THREADS) void verify_draw_kernel(VerifyArgs a) {
+  constexpr int PER = VERIFY_PIECE / VERIFY_VEC / VERIFY_THREADS;      // vectors a thread
   __shared__ double s_wave[4];
   __shared__ int s_last[4], s_pick;
   const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -370,8 +390,8 @@ __global__ __launch_bounds__(VERIFY_THREADS) void verify_draw_kernel(VerifyArgs 
   double all = 0.0, all_whole = 0.0;
   for (int c0 = 0; c0 < a.pieces; c0 += 64) {
     const VerifySums mine = c0 + lane < a.pieces ? sums[c0 + lane] : VerifySums{0.0, 0.0};
-    all = all + wave_sum_d(mine.left);
-    all_whole = all_whole + wave_sum_d(mine.whole);
+    all = all + wave_sum_xor(mine.left);
+    all_whole = all_whole + wave_sum_xor(mine.whole);
   }
   const bool use_left = all > 0.0;
   const double target = (double)a.draw_u[seq] * (use_left ? all : all_whole);
@@ -405,13 +425,13 @@ __global__ __launch_bounds__(VERIFY_THREADS) void verify_draw_kernel(VerifyArgs 
     before = last_before;
   }
   // The token in it: a thread has as many neighbouring logits as it has vectors of them.
-  double w[VERIFY_ITER][VERIFY_VEC], l[VERIFY_ITER][VERIFY_VEC], sum = 0.0;
-  int j[VERIFY_ITER], at[VERIFY_ITER], my_last = -1;
+  double w[PER][VERIFY_VEC], l[PER][VERIFY_VEC], sum = 0.0;
+  int j[PER], at[PER], my_last = -1;
 #pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i) j[i] = piece * VERIFY_PIECE + (tid * VERIFY_ITER + i) * VERIFY_VEC;
-  weights_of<VERIFY_ITER>(a, s, j, at, w, l);
+  for (int i = 0; i < PER; ++i) j[i] = piece * VERIFY_PIECE + (tid * PER + i) * VERIFY_VEC;
+  weights_of<PER>(a, s, (piece + 1) * VERIFY_PIECE > a.V, j, at, w, l);
 #pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i)
+  for (int i = 0; i < PER; ++i)
 #pragma unroll
     for (int e = 0; e < VERIFY_VEC; ++e) {
       w[i][e] = use_left ? l[i][e] : w[i][e];
@@ -434,7 +454,7 @@ __global__ __launch_bounds__(VERIFY_THREADS) void verify_draw_kernel(VerifyArgs 
   start = start + (upto - sum);
   int pick = 0x7fffffff;
 #pragma unroll
-  for (int i = 0; i < VERIFY_ITER; ++i)
+  for (int i = 0; i < PER; ++i)
 #pragma unroll
     for (int e = 0; e < VERIFY_VEC; ++e) {
       start = start + w[i][e];
@@ -462,17 +482,25 @@ int vk_verify(int32_t* tokens, int32_t* counts, float* accept, const elem_t* log
   VK_REQUIRE(scratch != nullptr && (uintptr_t)scratch % 16 == 0 && scratch_bytes >= vk_verify_scratch_bytes(R, D, S, V), "verify: %lld bytes of scratch needed, on 16 bytes",
              (long long)vk_verify_scratch_bytes(R, D, S, V));
   const int pieces = (int)verify_pieces(V);
-  VK_REQUIRE(pieces <= 65535, "verify: a vocabulary of %d is too large", V);
+  VK_REQUIRE(pieces <= 4 * 65535, "verify: a vocabulary of %d is too large", V);
   VerifyArgs a{tokens, counts, accept, logits, draft_logits, ids, cu, temps, accept_u, draw_u, static_cast<VerifyPart*>(scratch), nullptr, nullptr, R, D, S, V, pieces};
   a.sums = reinterpret_cast<VerifySums*>(a.parts + ((int64_t)R + D) * pieces);
   a.seqs = reinterpret_cast<VerifySeq*>(a.sums + (int64_t)S * pieces);
   const int64_t rows = (int64_t)R + (draft_logits != nullptr ? D : 0);
   VK_REQUIRE(rows < (1ll << 31), "verify: %lld rows are too many", (long long)rows);
   if (rows > 0) {
-    verify_parts_kernel<<<dim3((unsigned)rows, pieces), VERIFY_THREADS, 0, st>>>(a);
+    verify_parts_kernel<<<dim3((unsigned)rows, (pieces + 3) / 4), VERIFY_THREADS, 0, st>>>(a);
     if (vk_check_launch("verify (parts)")) return 1;
   }
-  verify_weigh_kernel<<<dim3(S, pieces), VERIFY_THREADS, 0, st>>>(a);
+  // Where the next launch's workgroups fit the card at once they decide for themselves.
+  const dim3 weigh(S, (pieces + 3) / 4);
+  if ((int64_t)weigh.x * weigh.y <= vk_device_cus()) {
+    verify_weigh_kernel<true><<<weigh, VERIFY_THREADS, 0, st>>>(a);
+  } else {
+    verify_decide_kernel<<<S, VERIFY_THREADS, 0, st>>>(a);
+    if (vk_check_launch("verify (decide)")) return 1;
+    verify_weigh_kernel<false><<<weigh, VERIFY_THREADS, 0, st>>>(a);
+  }
   if (vk_check_launch("verify (weigh)")) return 1;
   verify_draw_kernel<<<S, VERIFY_THREADS, 0, st>>>(a);
   return vk_check_launch("verify (draw)");
