@@ -80,7 +80,7 @@ def store(qkv, nq, nkv, d, k, v, scales, q_w, k_w, eps, cos, sin, table, cu, k_l
 
 
 def attention(q, k, v, scales, table, cu, k_len, scale, window=0):
-    """(out, weighted |v|, largest sum of |q k| scale, sum of |v| seen) of every row [T, nq, d] ([T, nq, 1] the third): rows of no sequence are NaN."""
+    """(out, weighted |v|, largest sum of |q k| scale, sum of |v - out| over the keys seen) of every row [T, nq, d] ([T, nq, 1] the third): rows of no sequence are NaN."""
     T, nq, d = q.shape
     nkv, P = k.shape[1], k.shape[2]
     group = nq // nkv
@@ -110,7 +110,7 @@ def attention(q, k, v, scales, table, cu, k_len, scale, window=0):
                     out[a + r, m] = w @ vv[see]
                     weighted[a + r, m] = w @ np.abs(vv[see])
                     most[a + r, m] = (np.abs(kk[see]) @ np.abs(q[a + r, m])).max() * scale
-                    flushed[a + r, m] = np.abs(vv[see]).sum(0)
+                    flushed[a + r, m] = np.abs(vv[see] - out[a + r, m]).sum(0)
     return out, weighted, most, flushed
 
 

@@ -160,14 +160,15 @@ def test_rows_of_a_wider_tensor_and_either_half_alone():
 
 # ------------------------------------------------------------------------------------------------------ attention
 def close(got, plain, name, d):
-    """A result is off by half a step of its type; by the weights' rounding (half a step of sixteen-bit floating point, 2^-11, of the sum of weights times |v|; weights
-    below 2^-24 of the largest by 2^-25 of it); and by the scores', sums of d products in 32 bits: (d + 16) 2^-24 of the largest sum of |q k|, twice (numerator
-    and denominator), and 2^-20 for the exponentials."""
+    """A result is off by half a step of its type; by the weights' rounding, in the sum of weights times values and in that of weights alike: weights w (1 + e) with |e| at most half a
+    step of sixteen-bit floating point, 2^-11, move it by at most 2^-11 of the mean of |v - out|, at most that of |v| and |out|; those below 2^-24 of the largest are off by up
+    to 2^-25 of it, which moves it by 2^-25 of the sum of |v - out|; and by the scores', sums of d products in 32 bits: (d + 16) 2^-24 of the largest sum of |q k|, twice
+    (numerator and denominator), and 2^-20 for the exponentials."""
     out, weighted, most, flushed = plain
     dtype = TYPES[name]
     score = 2 * (d + 16) * 2.0 ** -24 * most + 2.0 ** -20
     weights = 2.0 ** -11 if name == "bf16" else 2.0 ** -20
-    bound = torch.finfo(dtype).eps / 2 * np.abs(out) * 1.01 + weighted * (weights + score) + (2.0 ** -25 if name == "bf16" else 0.0) * flushed + 1e-30
+    bound = torch.finfo(dtype).eps / 2 * np.abs(out) * 1.01 + (weighted + np.abs(out)) * weights + weighted * score + (2.0 ** -25 if name == "bf16" else 0.0) * flushed + 1e-30
     got = host(got)
     assert np.array_equal(np.isnan(got), np.isnan(out)), np.argwhere(np.isnan(got) != np.isnan(out))[:5]
     fine = ~np.isnan(out)

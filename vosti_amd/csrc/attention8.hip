@@ -10,18 +10,23 @@
 //
 // Arithmetic.  A key's entry times its scale is exact in the element type, so the first product takes q as it is and 32-bit sums.  Weights are at most 1 (2^8
 // where a reference maximum is kept) and go into the second product in 16-bit floating point with eleven digits, against values without their scale, which
-// they hold to the bit: bfloat16 weights, with eight, doubled the squared error of the result.  Values' scales that differ within a product stand in its
-// entries relative to the largest of them.  The 32-bit build takes everything in 32 bits.  Sums of weights are of the unrounded ones.
+// they hold to the bit: bfloat16 weights, with eight, would double the squared error of the result.  Values' scales that differ within a product stand in its
+// entries relative to the largest of them.  The 32-bit build takes everything in 32 bits.  The sum of the weights comes from the matrix
+// unit too, a product with ones: it is that of the very weights that the values are multiplied by, and the vector unit has enough to do.
 //
 // Keys that a row does not see weigh 0, whatever is stored: their scores are never used, and values outside what the wave's rows see, or NaN, are
 // taken out of the second product of a tile that not all rows see whole; a row that does see a NaN gets it back through a product of its own.
+#include <type_traits>
+
 #include "cache8.h"
+#include "lines.h"
 #include "mma.h"
 #include "vec.h"
 
 #define A8_TILE 64
 #define A8_SEG 512               // keys that are summed up apart where a row's keys are split over workgroups
 #define A8_STEP 8.0f             // a column's reference maximum moves where the tile's exceeds it by more (log2)
+#define A8_NONE -3.0e38f          // the reference maximum of a column that has seen no key: finite, so that differences with it are numbers
 #define A8_STAGES 3              // tiles in LDS: one is computed, the next has arrived or is arriving, one is being asked for
 #define A8_ITEM_ROWS 128         // rows of an item, at most
 
@@ -37,13 +42,14 @@ struct A8Args {
 };
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// Over the lanes l, l ^ 16, l ^ 32, l ^ 48, in every one of them.
 __device__ __forceinline__ float over_groups_max(float v) {
-  v = fmaxf(v, lane_xor16(v));
-  return fmaxf(v, lane_xor32(v));
-}
-__device__ __forceinline__ float over_groups_sum(float v) {
-  v = v + lane_xor16(v);
-  return v + lane_xor32(v);
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const unsigned a = r[0], b = r[1], w = __builtin_bit_cast(unsigned, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+  const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  const unsigned c = q[0], e = q[1];
+  return fmaxf(__builtin_bit_cast(float, c), __builtin_bit_cast(float, e));
 }
 
 // ---- operands of the two products
@@ -80,6 +86,16 @@ __device__ __forceinline__ void values_times(u32x4 raw, float scale, const w_par
     for (int n = 0; n < NT; ++n) o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[n][h], o[n], 0, 0, 0);
   }
 }
+// The sum of the weights of a column, in every row of the result.
+template <int NT>
+__device__ __forceinline__ void ones_times(const w_part (&w)[NT][A8_WP], f32x4 (&o)[NT]) {
+  const _Float16 one = (_Float16)1.f;
+  const f16x8 ones = {one, one, one, one, one, one, one, one};
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, w[n][h], o[n], 0, 0, 0);
+}
 __device__ __forceinline__ void set_weights(const float (&p)[16], w_part (&w)[A8_WP]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h)
@@ -107,6 +123,13 @@ template <int NT>
 __device__ __forceinline__ void keys_times(u32x4 raw, float scale, const q_part (&q)[NT][A8_QJ], f32x4 (&s)[NT]) { bytes_times<NT>(raw, scale, q, s); }
 template <int NT>
 __device__ __forceinline__ void values_times(u32x4 raw, float scale, const w_part (&w)[NT][A8_WP], f32x4 (&o)[NT]) { bytes_times<NT>(raw, scale, w, o); }
+template <int NT>
+__device__ __forceinline__ void ones_times(const w_part (&w)[NT][A8_WP], f32x4 (&o)[NT]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.f, w[n][e], o[n], 0, 0, 0);
+}
 __device__ __forceinline__ void set_weights(const float (&p)[16], w_part (&w)[A8_WP]) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) w[e] = p[e];
@@ -128,17 +151,18 @@ __device__ __forceinline__ bool a8_rows(const A8Args& a, int item, int kvh, int 
   c.r = lane & 15;
   c.g = lane >> 4;
   c.kvh = kvh;
-  c.seq = a.items[2 * item];
-  const int first = a.items[2 * item + 1];
+  // (Read first lane: the same for the wave, which the compiler cannot know of what is loaded.)
+  c.seq = __builtin_amdgcn_readfirstlane(a.items[2 * item]);
+  const int first = __builtin_amdgcn_readfirstlane(a.items[2 * item + 1]);
   if ((unsigned)c.seq >= (unsigned)a.S || first < 0) return false;
-  const int t0 = a.cu_q[c.seq], t1 = a.cu_q[c.seq + 1];
+  const int t0 = __builtin_amdgcn_readfirstlane(a.cu_q[c.seq]), t1 = __builtin_amdgcn_readfirstlane(a.cu_q[c.seq + 1]);
   if (t0 < 0 || t1 > a.T) return false;
   c.rows = min(a.item_rows, t1 - t0 - first);
   c.cols = c.rows * a.group;
   c.col0 = col0;
   if (c.rows <= 0 || col0 >= c.cols) return false;
   c.tok0 = t0 + first;
-  c.pos0 = a.k_len[c.seq] - (t1 - t0) + first;
+  c.pos0 = __builtin_amdgcn_readfirstlane(a.k_len[c.seq]) - (t1 - t0) + first;
   const int row_first = col0 / a.group, row_last = (min(c.cols, col0 + 16 * NT) - 1) / a.group;
   c.all_pos = c.pos0 + row_first;
   c.wave_pos = c.pos0 + row_last;
@@ -178,21 +202,33 @@ __device__ __forceinline__ void a8_load_q(const A8Args& a, const A8Rows<NT>& c, 
   }
 }
 
+// q has arrived: waited for in front of a loop, so that no wait for it stands inside, where it would be one for all loads under way.
+template <int DP, int NT>
+__device__ __forceinline__ void a8_wait_q(q_part (&q)[DP / 64][NT][A8_QJ]) {
+#pragma unroll
+  for (int j = 0; j < DP / 64; ++j)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < A8_QJ; ++e) asm volatile("" : "+v"(q[j][n][e]));
+}
+
 // Bytes of four that hold a NaN, as 0x01 each.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u; }
 
 // A column's sums: m its reference maximum, l the sum of its weights, acc those of weights times values in units of 2^unit (the same for the wave).
 template <int DP, int NT>
 struct A8Sums {
-  float m[NT], l[NT];
+  float m[NT];
+  f32x4 l[NT];                 // the same number in all four
   f32x4 acc[NT][DP / 16];
   int unit;
   __device__ __forceinline__ void clear() {
     unit = -256;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      m[n] = -INFINITY;
-      l[n] = 0.f;
+      m[n] = A8_NONE;
+      l[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt) acc[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -207,16 +243,18 @@ struct A8Sums {
 };
 
 // One tile onto the wave's sums.  src.k(i, j) and src.v(dt): the lane's 16 bytes of K's tile i and of V's entries 16 dt + r; src.k_done() and src.v_done(): they are not asked
-// for again.  k_scale: of the keys whose K the lane reads; v_exp: of the 16 keys whose V it reads, -256: none of them is there.
+// for again.  k_scale: of the keys whose K the lane reads; v_exp: of the 16 keys whose V it reads, -256: none of them is there; top_exp: the wave's
+// largest.
 //
 // A column's reference maximum follows its maximum only where that is more than 2^8 above: weights are 2^8 at most then (their sums are 32-bit, and 2^8 is nothing to
 // sixteen bits), and the sums are scaled in few tiles.  Which columns move is each column's own business; whether any does is the wave's.
-template <int DP, int NT, typename SRC>
-__device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, int kb, SRC&& src, float k_scale, int v_exp, const q_part (&q)[DP / 64][NT][A8_QJ],
+// WHOLE: 1: every column that stands for a row sees every key; 0: not so; 2: that is found out here.  (Both in one loop, on scores and sums that come together again, cost a copy of
+// the scores a tile; a loop each costs none: 225 -> 196 us for a prompt of 4,096 rows of 32 heads of 128.)
+template <int WHOLE, int DP, int NT, typename SRC>
+__device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, int kb, SRC&& src, float k_scale, int v_exp, int top_exp, const q_part (&q)[DP / 64][NT][A8_QJ],
                                         A8Sums<DP, NT>& o) {
   const bool there = v_exp > -256;
-  // full: every column that stands for a row sees every key.
-  const bool full = kb >= c.all_lo && kb + A8_TILE - 1 <= c.all_pos && __all(there);
+  const bool full = WHOLE == 1 || (WHOLE == 2 && kb >= c.all_lo && kb + A8_TILE - 1 <= c.all_pos && __all(there));
   // What a product reads is asked for one product ahead, and not further: the scheduler would take all of a tile first, and spill.
   f32x4 s[4][NT];
   u32x4 next[DP / 64];
@@ -242,13 +280,14 @@ __device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, in
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     float top = -INFINITY;
+    const int lo = c.lo[n] - first, pos = there ? c.pos[n] - first : -1;
     if (full) {
 #pragma unroll
       for (int x = 0; x < 16; ++x) top = fmaxf(top, s[x / 4][n][x % 4]);
     } else {
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
-        const float v = there && first + x >= c.lo[n] && first + x <= c.pos[n] ? s[x / 4][n][x % 4] : -INFINITY;
+        const float v = x >= lo && x <= pos ? s[x / 4][n][x % 4] : -INFINITY;
         s[x / 4][n][x % 4] = v;
         top = fmaxf(top, v);
       }
@@ -259,15 +298,15 @@ __device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, in
   float by[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const bool move = m_tile[n] > o.m[n] + A8_STEP || (o.m[n] == -INFINITY && m_tile[n] > -INFINITY);
+    const bool move = m_tile[n] > o.m[n] + A8_STEP;
     const float to = move ? m_tile[n] : o.m[n];
-    by[n] = move ? exp2_fast(o.m[n] - to) : 1.f;
+    by[n] = exp2_fast(o.m[n] - to);
     o.m[n] = to;
     moves = moves || move;
   }
 #ifdef VK_BF16
   // The unit never falls, so that sums are scaled down only: what a smaller page adds is then in units of a larger one's.
-  const int unit = max(o.unit, __builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp)));
+  const int unit = max(o.unit, top_exp);
   const float to_unit = o.unit - unit < -126 ? 0.f : pow2f(o.unit - unit), v_scale = pow2f(max(-126, v_exp - unit));
   moves = moves || unit != o.unit;
   o.unit = unit;
@@ -285,16 +324,12 @@ __device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, in
   w_part w[NT][A8_WP];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float ref = o.m[n] > -INFINITY ? o.m[n] : 0.f;      // a column that has seen no key: its scores are -infinity, its weights 0
-    float p[16], sum = 0.f;
+    float p[16];
 #pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      p[x] = exp2_fast(__builtin_fmaf(s[x / 4][n][x % 4], a.scale_log2, -ref));
-      sum = sum + p[x];
-    }
-    o.l[n] = o.l[n] + sum;                                     // this lane's keys alone: joined where the sums are used
+    for (int x = 0; x < 16; ++x) p[x] = exp2_fast(__builtin_fmaf(s[x / 4][n][x % 4], a.scale_log2, -o.m[n]));
     set_weights(p, w[n]);
   }
+  ones_times<NT>(w, o.l);
   // Values that no column sees are taken out; so are NaN, which some may not see: those that do get it back through a product of ones.
   uint32_t keep[4] = {0, 0, 0, 0}, nans = 0;
   if (!full) {
@@ -370,6 +405,7 @@ struct A8Pages {
   int base, page;
   float k_scale;
   int v_exp;
+  uint64_t good;             // which of them there are
   template <int NT>
   __device__ __forceinline__ void fill(const A8Args& a, const A8Rows<NT>& c, int at, int pos) {
     base = at;
@@ -381,6 +417,8 @@ struct A8Pages {
     k_scale = there ? ks : 1.f;
     v_exp = there ? exponent_of(vs) : -256;
     page = there ? page : 0;
+    good = __ballot(there);
+    asm volatile("" : "+v"(page), "+v"(k_scale), "+v"(v_exp));     // waited for here: a wait where they are used would be one for every load that is under way there
   }
 };
 
@@ -449,7 +487,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void a8_few_kernel(A8Args a
   o.clear();
   for (int kb = kb0; (kb & ~(A8_SEG - 1)) <= seg1 * A8_SEG; kb += A8_SEG / 2) {
     if (t.wanted()) {
-      a8_tile<DP, 1>(a, c, kb, t, t.k_scale, t.v_exp, q, o);
+      a8_tile<2, DP, 1>(a, c, kb, t, t.k_scale, t.v_exp, __builtin_amdgcn_readfirstlane((int)over_groups_max((float)t.v_exp)), q, o);
     } else {
       t.k_done();
       t.v_done();
@@ -457,17 +495,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void a8_few_kernel(A8Args a
     if ((kb & (A8_SEG / 2)) == 0) continue;
     // Both tiles of the segment.
     const int seg = kb / A8_SEG;
-    const float l = over_groups_sum(o.l[0]);
+    const float l = o.l[0][0];
     if (c.g == 0) {
       maxima[wave][c.r] = o.m[0];
       totals[wave][c.r] = l;
     }
     __syncthreads();
-    const float top = fmaxf(fmaxf(maxima[0][c.r], maxima[1][c.r]), fmaxf(maxima[2][c.r], maxima[3][c.r])), ref = top > -INFINITY ? top : 0.f;
-    const float by = exp2_fast(o.m[0] - ref) * o.scale();
+    const float top = fmaxf(fmaxf(maxima[0][c.r], maxima[1][c.r]), fmaxf(maxima[2][c.r], maxima[3][c.r])), by = exp2_fast(o.m[0] - top) * o.scale();
     float total = 0.f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) total = __builtin_fmaf(totals[x][c.r], exp2_fast(maxima[x][c.r] - ref), total);
+    for (int x = 0; x < 4; ++x) total = __builtin_fmaf(totals[x][c.r], exp2_fast(maxima[x][c.r] - top), total);
 #pragma unroll
     for (int dt = 0; dt < DP / 16; ++dt) *reinterpret_cast<f32x4*>(sums[wave][dt][lane]) = o.acc[0][dt] * by;
     o.clear();
@@ -503,29 +540,59 @@ struct A8Stage {
   __device__ static __forceinline__ int turn(int r) { return DP == 128 ? r >> 1 & 7 : DP == 256 ? r : r >> 2 & 3; }
 };
 
+// What stands in scalar registers for an instruction written out, said to the compiler next to it: it may have moved the arithmetic to vector registers.
+__device__ __forceinline__ const uint8_t* a8_scalar(const uint8_t* p) {
+  const uint64_t u = (uint64_t)p;
+  return (const uint8_t*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)u));
+}
 __device__ __forceinline__ void a8_load_to_lds(const uint8_t* p, unsigned lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds_addr) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(__builtin_amdgcn_readfirstlane(lds_addr)) : "memory");
 }
 
-template <int DP, int WAVES, int NT>
-__device__ __forceinline__ void a8_ask(const A8Args& a, const A8Rows<NT>& c, const A8Pages& pg, int kb, unsigned lds) {
+// Pages of a tile and more: what a lane asks for lies at the same distance from the tile's first key in every tile, and that is scalar arithmetic.
+template <int DP, int WAVES>
+struct A8Offsets {
+  unsigned k[A8Stage<DP, WAVES>::LOADS], v[A8Stage<DP, WAVES>::LOADS];
+  __device__ __forceinline__ void set(const A8Args& a, int wave, int lane) {
+    typedef A8Stage<DP, WAVES> ST;
+#pragma unroll
+    for (int i = 0; i < ST::LOADS; ++i) {
+      const int at = (i * WAVES + wave) * 64 + lane;           // piece of K's tile
+      const int row = at / ST::PIECES, r = row & 15, piece = min((at % ST::PIECES) ^ ST::turn(r), a.d / 16 - 1);
+      k[i] = (16 * (r >> 2) + 4 * (row >> 4) + (r & 3)) * a.d + 16 * piece;
+      v[i] = min(at >> 2, a.d - 1) * a.P + 16 * ((at & 3) ^ (at >> 4 & 3));
+    }
+  }
+};
+
+template <int DP, int WAVES>
+__device__ __forceinline__ void a8_ask(const A8Args& a, int kvh, const A8Pages& pg, const A8Offsets<DP, WAVES>& off, int wave, int kb, unsigned lds) {
   typedef A8Stage<DP, WAVES> ST;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, last_k = a.d / 16 - 1;
+  if (a.P >= A8_TILE) {
+    const int64_t block = (int64_t)__builtin_amdgcn_readlane(pg.page, (kb >> a.lp) - pg.base) * a.nkv + kvh;
+    const uint8_t *kp = a8_scalar(a.kc + (block * a.P + (kb & (a.P - 1))) * a.d), *vp = a8_scalar(a.vc + block * a.P * a.d + (kb & (a.P - 1)));
+    const unsigned to = __builtin_amdgcn_readfirstlane(lds + wave * 1024);
+#pragma unroll
+    for (int i = 0; i < ST::LOADS; ++i) pipe_load_to_lds16_sv(kp, off.k[i], to + i * WAVES * 1024);
+#pragma unroll
+    for (int i = 0; i < ST::LOADS; ++i) pipe_load_to_lds16_sv(vp, off.v[i], to + A8_TILE * DP + i * WAVES * 1024);
+    return;
+  }
+  // Several pages a tile: a lane's is that of its 16 keys.
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int i = 0; i < ST::LOADS; ++i) {
-    const int at = (i * WAVES + wave) * 64 + lane;             // piece of K's tile
-    const int row = at / ST::PIECES, r = row & 15, piece = min((at % ST::PIECES) ^ ST::turn(r), last_k);
-    const int key = kb + 16 * (r >> 2) + 4 * (row >> 4) + (r & 3);
-    const int page = __shfl(pg.page, (key >> a.lp) - pg.base);
-    a8_load_to_lds(a.kc + (((int64_t)page * a.nkv + c.kvh) * a.P + (key & (a.P - 1))) * a.d + 16 * piece, __builtin_amdgcn_readfirstlane(lds + (i * WAVES + wave) * 1024));
+    const int at = (i * WAVES + wave) * 64 + lane, row = at / ST::PIECES, chunk = 16 * ((row & 15) >> 2);
+    const int64_t block = (int64_t)__shfl(pg.page, ((kb + chunk) >> a.lp) - pg.base) * a.nkv + kvh;
+    const uint8_t* kp = a.kc + (block * a.P + ((kb + chunk) & (a.P - 1))) * a.d;
+    a8_load_to_lds(kp + off.k[i] - chunk * a.d, lds + (i * WAVES + wave) * 1024);
   }
 #pragma unroll
   for (int i = 0; i < ST::LOADS; ++i) {
-    const int at = (i * WAVES + wave) * 64 + lane, row = min(at >> 2, a.d - 1), piece = (at & 3) ^ (at >> 4 & 3);
-    const int key = kb + 16 * piece;
-    const int page = __shfl(pg.page, (key >> a.lp) - pg.base);
-    a8_load_to_lds(a.vc + (((int64_t)page * a.nkv + c.kvh) * a.d + row) * a.P + (key & (a.P - 1)),
-                   __builtin_amdgcn_readfirstlane(lds + A8_TILE * DP + (i * WAVES + wave) * 1024));
+    const int at = (i * WAVES + wave) * 64 + lane, chunk = 16 * ((at & 3) ^ (at >> 4 & 3));
+    const int64_t block = (int64_t)__shfl(pg.page, ((kb + chunk) >> a.lp) - pg.base) * a.nkv + kvh;
+    const uint8_t* vp = a.vc + block * a.P * a.d + ((kb + chunk) & (a.P - 1));
+    a8_load_to_lds(vp + off.v[i] - chunk, lds + A8_TILE * DP + (i * WAVES + wave) * 1024);
   }
 }
 
@@ -572,21 +639,32 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
   if (mine) a8_load_q<DP, NT>(a, c, q);
   A8Sums<DP, NT> o;
   o.clear();
+  a8_wait_q<DP, NT>(q);
   lo &= ~(A8_TILE - 1);
   const int tiles = pos < lo ? 0 : ((pos - lo) >> 6) + 1;
   const unsigned lds = (unsigned)(unsigned long)((__attribute__((address_space(3))) const void*)stages);
   A8Pages ahead, now;                                                     // of the tiles that are asked for, of those that are computed
+  A8Offsets<DP, WAVES> off;
+  off.set(a, wave, threadIdx.x & 63);
   if (tiles > 0) ahead.fill(a, c, lo >> a.lp, pos);
   now = ahead;
-  auto ask = [&](int i) {
-    const int kb = lo + i * A8_TILE;
+  auto ask = [&](int tile) {
+    const int i = __builtin_amdgcn_readfirstlane(tile), kb = lo + i * A8_TILE;
     if ((kb >> a.lp) - ahead.base >= 64) ahead.fill(a, c, kb >> a.lp, pos);
-    a8_ask<DP, WAVES, NT>(a, c, ahead, kb, lds + (unsigned)(i % A8_STAGES) * ST::BYTES);
+    a8_ask<DP, WAVES>(a, kvh, ahead, off, wave, kb, lds + (unsigned)(i % A8_STAGES) * ST::BYTES);
   };
   if (tiles > 0) ask(0);
   if (tiles > 1) ask(1);
-  for (int i = 0; i < tiles; ++i) {
-    const int kb = lo + i * A8_TILE;
+  // Whether all of the wave's rows see all of tile i.
+  auto whole = [&](int tile) {
+    const int kb = lo + __builtin_amdgcn_readfirstlane(tile) * A8_TILE;
+    if (!mine || kb < c.all_lo || kb + A8_TILE - 1 > c.all_pos) return false;
+    if ((kb >> a.lp) - now.base >= 64) now.fill(a, c, kb >> a.lp, pos);
+    const uint64_t pages = a.P >= A8_TILE ? 1 : (1ull << (A8_TILE >> a.lp)) - 1;
+    return __builtin_amdgcn_readfirstlane((int)((now.good >> ((kb >> a.lp) - now.base) & pages) == pages)) != 0;
+  };
+  auto step = [&](int tile, auto all_see) {
+    const int i = __builtin_amdgcn_readfirstlane(tile), kb = lo + i * A8_TILE;
     // Tile i has arrived (at most the next one's loads are under way), this wave has what it read of tile i - 1; behind the barrier that holds for all.
     asm volatile("" ::: "memory");
     if (i + 1 < tiles) __builtin_amdgcn_s_waitcnt(0x0070 | (2 * ST::LOADS & 0xF) | ((2 * ST::LOADS >> 4) << 14));
@@ -594,20 +672,33 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (i + 2 < tiles) ask(i + 2);
+    if (!all_see.value && (!mine || kb > c.wave_pos || kb + A8_TILE <= c.wave_lo)) return;
     if ((kb >> a.lp) - now.base >= 64) now.fill(a, c, kb >> a.lp, pos);
-    if (mine && kb <= c.wave_pos && kb + A8_TILE > c.wave_lo) {
-      const int kp = ((kb + 16 * (c.r >> 2)) >> a.lp) - now.base, vp = ((kb + 16 * c.g) >> a.lp) - now.base;
-      const float k_scale = __shfl(now.k_scale, kp);
-      const int v_exp = __shfl(now.v_exp, vp), key = kb + 16 * c.g;
-      a8_tile<DP, NT>(a, c, kb, A8Shared<DP, WAVES>{stages + (i % A8_STAGES) * ST::BYTES, c.r, c.g}, k_scale,
-                      key <= c.wave_pos && key + 15 >= c.wave_lo ? v_exp : -256, q, o);
+    const int key = kb + 16 * c.g;
+    float k_scale;
+    int v_exp, top_exp;
+    if (a.P >= A8_TILE) {
+      const int l = (kb >> a.lp) - now.base;
+      k_scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.k_scale), l));
+      v_exp = top_exp = __builtin_amdgcn_readlane(now.v_exp, l);
+    } else {
+      k_scale = __shfl(now.k_scale, ((kb + 16 * (c.r >> 2)) >> a.lp) - now.base);
+      v_exp = __shfl(now.v_exp, (key >> a.lp) - now.base);
+      if (!all_see.value) v_exp = key <= c.wave_pos && key + 15 >= c.wave_lo ? v_exp : -256;
+      top_exp = __builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp));
     }
+    if (!all_see.value) v_exp = key <= c.wave_pos && key + 15 >= c.wave_lo ? v_exp : -256;
+    a8_tile<all_see.value, DP, NT>(a, c, kb, A8Shared<DP, WAVES>{stages + (i % A8_STAGES) * ST::BYTES, c.r, c.g}, k_scale, v_exp, top_exp, q, o);
+  };
+  for (int i = 0; i < tiles;) {
+    for (; i < tiles && !whole(i); ++i) step(i, std::integral_constant<int, 0>());
+    for (; i < tiles && whole(i); ++i) step(i, std::integral_constant<int, 1>());
   }
   if (!mine) return;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int col = c.col0 + 16 * n + c.r;
-    const float l = over_groups_sum(o.l[n]);
+    const float l = o.l[n][0];
     if (col >= c.cols) continue;
     if (SPLIT && seg_first != seg_last) {
       const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg) * a.cols_max + col;
@@ -635,17 +726,16 @@ __global__ __launch_bounds__(256) void a8_join_kernel(A8Args a, int cols) {
   a8_segments(a.window > 0 ? max(0, c.pos0 + row_first - a.window + 1) : 0, c.pos0 + row_last, seg_first, seg_last);
   if (seg_first == seg_last) return;                    // the other kernel wrote the result
   const int64_t part0 = ((int64_t)item * a.nkv + kvh) * a.nseg * a.cols_max + col;
-  float top = -INFINITY;
+  float top = A8_NONE;
   for (int s = seg_first + lane; s <= seg_last; s += 64) top = fmaxf(top, a.part_ml[2 * (part0 + (int64_t)s * a.cols_max)]);
   top = wave_max_xor(top);
-  const float ref = top > -INFINITY ? top : 0.f;
   float total = 0.f;
   f32x2 o[2] = {{0.f, 0.f}, {0.f, 0.f}};
   for (int s0 = seg_first; s0 <= seg_last; s0 += 64) {
     float by = 0.f;
     if (s0 + lane <= seg_last) {
       const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * (part0 + (int64_t)(s0 + lane) * a.cols_max));
-      by = exp2_fast(ml.x - ref);
+      by = exp2_fast(ml.x - top);
       total = __builtin_fmaf(ml.y, by, total);
     }
     const int n = min(64, seg_last - s0 + 1);
@@ -747,10 +837,9 @@ int vk_paged_attention8(elem_t* out, const elem_t* q, const uint8_t* kc, const u
     else a8_few_kernel<256><<<grid, 256, 0, st>>>(a, each);
     if (vk_check_launch("attention8")) return 1;
   } else {
-    const bool two = a.cols_max <= 32;
+    const bool two = a.cols_max <= 32 && d <= 192;      // two waves; of the largest heads' tiles a wave's share of the loads would not fit its registers
     cols = two ? 32 : 64;
-    const int bad = two ? (d <= 64 ? a8_shared<64, 1, 2, true>(a, st) : d <= 128 ? a8_shared<128, 1, 2, true>(a, st) : d <= 192 ? a8_shared<192, 1, 2, true>(a, st)
-                                                                                                                               : a8_shared<256, 1, 2, true>(a, st))
+    const int bad = two ? (d <= 64 ? a8_shared<64, 1, 2, true>(a, st) : d <= 128 ? a8_shared<128, 1, 2, true>(a, st) : a8_shared<192, 1, 2, true>(a, st))
                         : (d <= 64 ? a8_shared<64, 1, 4, true>(a, st) : d <= 128 ? a8_shared<128, 1, 4, true>(a, st) : d <= 192 ? a8_shared<192, 1, 4, true>(a, st)
                                                                                                                                : a8_shared<256, 1, 4, true>(a, st));
     if (bad) return 1;

@@ -102,7 +102,8 @@ class Kernels:
 
     @staticmethod
     def _stream() -> int:
-        return torch.cuda.current_stream().cuda_stream
+        # torch.cuda.current_stream().cuda_stream without the object around it (0.3 instead of 2.7 us of every call)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
     def _elem(self, t: torch.Tensor, what: str, *shape) -> int:
         self._check(t, what, self.dtype, shape)
@@ -118,7 +119,7 @@ class Kernels:
             raise KernelError(f"{what} has type {t.dtype}, expected {dtype}")
         if not t.is_contiguous():
             raise KernelError(f"{what} is not contiguous")
-        if shape and tuple(t.shape) != tuple(shape):
+        if shape and t.shape != tuple(shape):
             raise KernelError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
     def _i32(self, t: torch.Tensor, what: str, *shape) -> int:
@@ -394,7 +395,7 @@ class Kernels:
         """The launch goes to the current device: what lies on another one is refused."""
         here = torch.cuda.current_device()
         for t in tensors:
-            if t is not None and t.device.index != here:
+            if t is not None and t.get_device() != here:
                 raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{here}")
 
     def empty_cache8(self, pages: int, nkv: int, page_size: int, d: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -489,7 +490,7 @@ class Kernels:
         ip = self._i32(items, "items", n_items, 2)
         out = torch.empty_like(q) if out is None else out
         self._elem(out, "out", T, nq, d)
-        need = self.attn8_scratch_floats(n_items, item_rows, nq, d, max_k_len)
+        need = self.attn8_scratch_floats(n_items, item_rows, nq, d, max_k_len) if item_rows <= 16 else 0
         if need and scratch is None:
             scratch = torch.empty(need, dtype=torch.float32, device=q.device)
         self._here(q, k_cache, v_cache, scales, block_table, cu_q, k_len, items, scratch, out)
