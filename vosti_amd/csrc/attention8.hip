@@ -256,6 +256,7 @@ __device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, in
   const bool there = v_exp > -256;
   const bool full = WHOLE == 1 || (WHOLE == 2 && kb >= c.all_lo && kb + A8_TILE - 1 <= c.all_pos && __all(there));
   // What a product reads is asked for one product ahead, and not further: the scheduler would take all of a tile first, and spill.
+  __builtin_amdgcn_s_setprio(1);
   f32x4 s[4][NT];
   u32x4 next[DP / 64];
 #pragma unroll
@@ -274,6 +275,7 @@ __device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, in
     for (int j = 0; j < DP / 64; ++j) keys_times<NT>(k[j], k_scale, q[j], s[i]);
     asm volatile("" ::: "memory");
   }
+  __builtin_amdgcn_s_setprio(0);
   src.k_done();
   const int first = kb + 16 * c.g;
   float m_tile[NT];
@@ -329,6 +331,7 @@ __device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, in
     for (int x = 0; x < 16; ++x) p[x] = exp2_fast(__builtin_fmaf(s[x / 4][n][x % 4], a.scale_log2, -o.m[n]));
     set_weights(p, w[n]);
   }
+  __builtin_amdgcn_s_setprio(1);
   ones_times<NT>(w, o.l);
   // Values that no column sees are taken out; so are NaN, which some may not see: those that do get it back through a product of ones.
   uint32_t keep[4] = {0, 0, 0, 0}, nans = 0;
@@ -358,6 +361,7 @@ __device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, in
     for (int n = 0; n < NT; ++n) o.acc[n][dt] = x[n];
     asm volatile("" ::: "memory");
   }
+  __builtin_amdgcn_s_setprio(0);
   if (__any(nans != 0)) {
     w_part seen[NT][A8_WP];
 #pragma unroll
@@ -402,24 +406,31 @@ __device__ __forceinline__ void a8_segments(int lo, int pos, int& first, int& la
 
 // The pages that a workgroup walks, 64 at a time: lane l has number `base + l` of the sequence's.
 struct A8Pages {
-  int base, page;
+  int base;
+  uint64_t at;               // where its block of the kv head begins, in keys and in values alike (the first page's, for a page that is none)
   float k_scale;
   int v_exp;
   uint64_t good;             // which of them there are
   template <int NT>
-  __device__ __forceinline__ void fill(const A8Args& a, const A8Rows<NT>& c, int at, int pos) {
-    base = at;
-    const int i = at + (threadIdx.x & 63);
-    page = i < a.W && i <= pos >> a.lp ? a.table[(int64_t)c.seq * a.W + i] : -1;
+  __device__ __forceinline__ void fill(const A8Args& a, const A8Rows<NT>& c, int first, int pos) {
+    base = first;
+    const int i = first + (threadIdx.x & 63);
+    const int page = i < a.W && i <= pos >> a.lp ? a.table[(int64_t)c.seq * a.W + i] : -1;
     const bool there = (unsigned)page < (unsigned)a.pages;
-    const float* s = a.scales + ((int64_t)(there ? page : 0) * a.nkv + c.kvh) * 2;
-    const float ks = s[0], vs = s[1];
+    const int64_t block = (int64_t)(there ? page : 0) * a.nkv + c.kvh;
+    const float ks = a.scales[2 * block], vs = a.scales[2 * block + 1];
+    unsigned lo = (unsigned)(block * a.P * a.d), hi = (unsigned)((uint64_t)(block * a.P * a.d) >> 32);
     k_scale = there ? ks : 1.f;
     v_exp = there ? exponent_of(vs) : -256;
-    page = there ? page : 0;
     good = __ballot(there);
-    asm volatile("" : "+v"(page), "+v"(k_scale), "+v"(v_exp));     // waited for here: a wait where they are used would be one for every load that is under way there
+    // Waited for here: a wait where they are used would be one for every load that is under way there.
+    asm volatile("" : "+v"(lo), "+v"(hi), "+v"(k_scale), "+v"(v_exp));
+    at = (uint64_t)hi << 32 | lo;
   }
+  __device__ __forceinline__ uint64_t of_lane(int lane) const {                  // the same lane for the wave
+    return (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(at >> 32), lane) << 32 | (unsigned)__builtin_amdgcn_readlane((int)at, lane);
+  }
+  __device__ __forceinline__ uint64_t of_any(int lane) const { return (uint64_t)(unsigned)__shfl((int)(at >> 32), lane) << 32 | (unsigned)__shfl((int)at, lane); }
 };
 
 // ---- up to 16 columns (decoded tokens): a workgroup takes segments of 512 keys one after the other, a wave two of a segment's tiles, every fourth.  They come straight into
@@ -459,7 +470,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void a8_few_kernel(A8Args a
       k_scale = __shfl(pages.k_scale, kl);
       v_exp = __shfl(pages.v_exp, vl);
       v_exp = vkey <= c.wave_pos && vkey + 15 >= c.wave_lo ? v_exp : -256;
-      const uint8_t* kp = a.kc + (((int64_t)__shfl(pages.page, kl) * a.nkv + c.kvh) * a.P + (kkey & (a.P - 1)) + (c.r & 3)) * a.d;
+      const uint8_t* kp = a.kc + pages.of_any(kl) + ((kkey & (a.P - 1)) + (c.r & 3)) * a.d;
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -469,7 +480,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void a8_few_kernel(A8Args a
     __device__ __forceinline__ void ask_v() {
       if (!wanted()) return;
       const int vkey = kb + 16 * c.g;
-      const uint8_t* vp = a.vc + (((int64_t)__shfl(pages.page, (vkey >> a.lp) - pages.base) * a.nkv + c.kvh) * a.d + c.r) * a.P + (vkey & (a.P - 1));
+      const uint8_t* vp = a.vc + pages.of_any((vkey >> a.lp) - pages.base) + c.r * a.P + (vkey & (a.P - 1));
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt) vr[dt] = *reinterpret_cast<const u32x4*>(vp + min(16 * dt, a.d - 16) * a.P);     // and here for nothing
     }
@@ -549,50 +560,45 @@ __device__ __forceinline__ void a8_load_to_lds(const uint8_t* p, unsigned lds_ad
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(__builtin_amdgcn_readfirstlane(lds_addr)) : "memory");
 }
 
-// Pages of a tile and more: what a lane asks for lies at the same distance from the tile's first key in every tile, and that is scalar arithmetic.
+// What a lane asks for lies at the same distance from the start of the page (of pages smaller than a tile: of the one of its 16 keys) in every tile, but for the tile's own place in a
+// larger page.
 template <int DP, int WAVES>
 struct A8Offsets {
   unsigned k[A8Stage<DP, WAVES>::LOADS], v[A8Stage<DP, WAVES>::LOADS];
+  int k_page[A8Stage<DP, WAVES>::LOADS], v_page[A8Stage<DP, WAVES>::LOADS];      // which of the tile's pages
   __device__ __forceinline__ void set(const A8Args& a, int wave, int lane) {
     typedef A8Stage<DP, WAVES> ST;
+    const int within = min(a.P, A8_TILE) - 1;
 #pragma unroll
     for (int i = 0; i < ST::LOADS; ++i) {
       const int at = (i * WAVES + wave) * 64 + lane;           // piece of K's tile
       const int row = at / ST::PIECES, r = row & 15, piece = min((at % ST::PIECES) ^ ST::turn(r), a.d / 16 - 1);
-      k[i] = (16 * (r >> 2) + 4 * (row >> 4) + (r & 3)) * a.d + 16 * piece;
-      v[i] = min(at >> 2, a.d - 1) * a.P + 16 * ((at & 3) ^ (at >> 4 & 3));
+      const int k_key = 16 * (r >> 2) + 4 * (row >> 4) + (r & 3), v_key = 16 * ((at & 3) ^ (at >> 4 & 3));
+      k[i] = (k_key & within) * a.d + 16 * piece;
+      v[i] = min(at >> 2, a.d - 1) * a.P + (v_key & within);
+      k_page[i] = k_key >> a.lp;
+      v_page[i] = v_key >> a.lp;
     }
   }
 };
 
 template <int DP, int WAVES>
-__device__ __forceinline__ void a8_ask(const A8Args& a, int kvh, const A8Pages& pg, const A8Offsets<DP, WAVES>& off, int wave, int kb, unsigned lds) {
+__device__ __forceinline__ void a8_ask(const A8Args& a, const A8Pages& pg, const A8Offsets<DP, WAVES>& off, int wave, int kb, unsigned lds) {
   typedef A8Stage<DP, WAVES> ST;
+  const int first = (kb >> a.lp) - pg.base;
+  const unsigned to = __builtin_amdgcn_readfirstlane(lds + wave * 1024);
   if (a.P >= A8_TILE) {
-    const int64_t block = (int64_t)__builtin_amdgcn_readlane(pg.page, (kb >> a.lp) - pg.base) * a.nkv + kvh;
-    const uint8_t *kp = a8_scalar(a.kc + (block * a.P + (kb & (a.P - 1))) * a.d), *vp = a8_scalar(a.vc + block * a.P * a.d + (kb & (a.P - 1)));
-    const unsigned to = __builtin_amdgcn_readfirstlane(lds + wave * 1024);
+    const uint64_t at = pg.of_lane(first);
+    const uint8_t *kp = a8_scalar(a.kc + at + (kb & (a.P - 1)) * a.d), *vp = a8_scalar(a.vc + at + (kb & (a.P - 1)));
 #pragma unroll
     for (int i = 0; i < ST::LOADS; ++i) pipe_load_to_lds16_sv(kp, off.k[i], to + i * WAVES * 1024);
 #pragma unroll
     for (int i = 0; i < ST::LOADS; ++i) pipe_load_to_lds16_sv(vp, off.v[i], to + A8_TILE * DP + i * WAVES * 1024);
-    return;
-  }
-  // Several pages a tile: a lane's is that of its 16 keys.
-  const int lane = threadIdx.x & 63;
+  } else {
 #pragma unroll
-  for (int i = 0; i < ST::LOADS; ++i) {
-    const int at = (i * WAVES + wave) * 64 + lane, row = at / ST::PIECES, chunk = 16 * ((row & 15) >> 2);
-    const int64_t block = (int64_t)__shfl(pg.page, ((kb + chunk) >> a.lp) - pg.base) * a.nkv + kvh;
-    const uint8_t* kp = a.kc + (block * a.P + ((kb + chunk) & (a.P - 1))) * a.d;
-    a8_load_to_lds(kp + off.k[i] - chunk * a.d, lds + (i * WAVES + wave) * 1024);
-  }
+    for (int i = 0; i < ST::LOADS; ++i) a8_load_to_lds(a.kc + pg.of_any(first + off.k_page[i]) + off.k[i], to + i * WAVES * 1024);
 #pragma unroll
-  for (int i = 0; i < ST::LOADS; ++i) {
-    const int at = (i * WAVES + wave) * 64 + lane, chunk = 16 * ((at & 3) ^ (at >> 4 & 3));
-    const int64_t block = (int64_t)__shfl(pg.page, ((kb + chunk) >> a.lp) - pg.base) * a.nkv + kvh;
-    const uint8_t* vp = a.vc + block * a.P * a.d + ((kb + chunk) & (a.P - 1));
-    a8_load_to_lds(vp + off.v[i] - chunk, lds + A8_TILE * DP + (i * WAVES + wave) * 1024);
+    for (int i = 0; i < ST::LOADS; ++i) a8_load_to_lds(a.vc + pg.of_any(first + off.v_page[i]) + off.v[i], to + A8_TILE * DP + i * WAVES * 1024);
   }
 }
 
@@ -651,7 +657,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
   auto ask = [&](int tile) {
     const int i = __builtin_amdgcn_readfirstlane(tile), kb = lo + i * A8_TILE;
     if ((kb >> a.lp) - ahead.base >= 64) ahead.fill(a, c, kb >> a.lp, pos);
-    a8_ask<DP, WAVES>(a, kvh, ahead, off, wave, kb, lds + (unsigned)(i % A8_STAGES) * ST::BYTES);
+    a8_ask<DP, WAVES>(a, ahead, off, wave, kb, lds + (unsigned)(i % A8_STAGES) * ST::BYTES);
   };
   if (tiles > 0) ask(0);
   if (tiles > 1) ask(1);
