@@ -242,22 +242,12 @@ struct A8Sums {
   }
 };
 
-// One tile onto the wave's sums.  src.k(i, j) and src.v(dt): the lane's 16 bytes of K's tile i and of V's entries 16 dt + r; src.k_done() and src.v_done(): they are not asked
-// for again.  k_scale: of the keys whose K the lane reads; v_exp: of the 16 keys whose V it reads, -256: none of them is there; top_exp: the wave's
-// largest.
-//
-// A column's reference maximum follows its maximum only where that is more than 2^8 above: weights are 2^8 at most then (their sums are 32-bit, and 2^8 is nothing to
-// sixteen bits), and the sums are scaled in few tiles.  Which columns move is each column's own business; whether any does is the wave's.
-// WHOLE: 1: every column that stands for a row sees every key; 0: not so; 2: that is found out here.  (Both in one loop, on scores and sums that come together again, cost a copy of
-// the scores a tile; a loop each costs none: 225 -> 196 us for a prompt of 4,096 rows of 32 heads of 128.)
-template <int WHOLE, int DP, int NT, typename SRC>
-__device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, int kb, SRC&& src, float k_scale, int v_exp, int top_exp, const q_part (&q)[DP / 64][NT][A8_QJ],
-                                        A8Sums<DP, NT>& o) {
-  const bool there = v_exp > -256;
-  const bool full = WHOLE == 1 || (WHOLE == 2 && kb >= c.all_lo && kb + A8_TILE - 1 <= c.all_pos && __all(there));
-  // What a product reads is asked for one product ahead, and not further: the scheduler would take all of a tile first, and spill.
+// The scores of a tile: S^T's, unscaled.  src.k(i, j): the lane's 16 bytes of K's tile i; k_scale: of the keys that they belong to.
+template <int DP, int NT, typename SRC>
+__device__ __forceinline__ void a8_scores(const SRC& src, float k_scale, const q_part (&q)[DP / 64][NT][A8_QJ], f32x4 (&s)[4][NT]) {
+  // Where two waves meet on a unit the one in front of its products goes first: they leave the other three of four cycles for its arithmetic (196 -> 186 us for a prompt of 4,096 rows).
   __builtin_amdgcn_s_setprio(1);
-  f32x4 s[4][NT];
+  // What a product reads is asked for one product ahead, and not further: the scheduler would take all of a tile first, and spill.
   u32x4 next[DP / 64];
 #pragma unroll
   for (int j = 0; j < DP / 64; ++j) next[j] = src.k(0, j);
@@ -276,7 +266,19 @@ __device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, in
     asm volatile("" ::: "memory");
   }
   __builtin_amdgcn_s_setprio(0);
-  src.k_done();
+}
+
+// A tile's scores and values onto the wave's sums.  src.v(dt): the lane's 16 bytes of V's entries 16 dt + r; v_exp: of the 16 keys that they belong to, -256: none of them is there;
+// top_exp: the wave's largest.
+//
+// A column's reference maximum follows its maximum only where that is more than 2^8 above: weights are 2^8 at most then (their sums are 32-bit, and 2^8 is nothing to
+// sixteen bits), and the sums are scaled in few tiles.  Which columns move is each column's own business; whether any does is the wave's.
+// WHOLE: 1: every column that stands for a row sees every key; 0: not so; 2: that is found out here.  (Both in one loop, on scores and sums that come together again, cost a copy of
+// the scores a tile; a loop each costs none: 225 -> 196 us for that prompt.)
+template <int WHOLE, int DP, int NT, typename SRC>
+__device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, int kb, const SRC& src, f32x4 (&s)[4][NT], int v_exp, int top_exp, A8Sums<DP, NT>& o) {
+  const bool there = v_exp > -256;
+  const bool full = WHOLE == 1 || (WHOLE == 2 && kb >= c.all_lo && kb + A8_TILE - 1 <= c.all_pos && __all(there));
   const int first = kb + 16 * c.g;
   float m_tile[NT];
 #pragma unroll
@@ -363,6 +365,9 @@ __device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, in
   }
   __builtin_amdgcn_s_setprio(0);
   if (__any(nans != 0)) {
+    // Made anew from here on, not kept for this: what follows happens next to never.
+#pragma unroll
+    for (int b = 0; b < 4; ++b) asm volatile("" : "+v"(keep[b]));
     w_part seen[NT][A8_WP];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -387,7 +392,6 @@ __device__ __forceinline__ void a8_tile(const A8Args& a, const A8Rows<NT>& c, in
       asm volatile("" ::: "memory");
     }
   }
-  src.v_done();
 }
 
 // Where a column's result goes, from its first entry 4 g on.
@@ -437,6 +441,27 @@ struct A8Pages {
 // registers: a tile's keys are asked for when the last tile's have been multiplied, its values when those have, so that there is something under way at any time and no
 // load waits for another (page numbers and scales are read 64 pages ahead; a page number read in turn would wait for all loads before it).  The waves' sums meet in LDS,
 // the segments' in a8_join_kernel.
+// A tile in registers.  Of heads of 128 a load takes eight rows of K in whole lines of the cache, 128 bytes, and not half of each of sixteen: the load of the other halves
+// would wait in the first cache for the lines that are under way, and what stands behind it too (200 -> 188 us for 64 rows of 8,192 keys).  So kr[i][0] has in lane rows 0..7 the first
+// half of rows 0..7, in lane rows 8..15 their second half, kr[i][1] the same of rows 8..15, and a lane's own row comes together when it is used.
+template <int DP>
+struct A8Held {
+  static constexpr bool LINES = DP % 128 == 0;
+  u32x4 kr[4][DP / 64], vr[DP / 16];
+  __device__ __forceinline__ u32x4 k(int i, int j) const {
+    if (!LINES) return kr[i][j];
+    u32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int a = (int)kr[i][j & ~1][e], b = (int)kr[i][j | 1][e];
+      // Lane rows 8 apart change places (row_ror:8), in those lanes that have another row's half.
+      x[e] = (j & 1) ? (uint32_t)__builtin_amdgcn_update_dpp(b, a, 0x128, 0xF, 0x3, false) : (uint32_t)__builtin_amdgcn_update_dpp(a, b, 0x128, 0xF, 0xC, false);
+    }
+    return x;
+  }
+  __device__ __forceinline__ u32x4 v(int dt) const { return vr[dt]; }
+};
+
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void a8_few_kernel(A8Args a, int segs_each) {
   __shared__ float sums[4][DP / 16][64][4];
@@ -449,60 +474,59 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void a8_few_kernel(A8Args a
   const int seg0 = max(seg_first, (int)blockIdx.y * segs_each), seg1 = min(seg_last, (int)blockIdx.y * segs_each + segs_each - 1);
   if (seg0 > seg1) return;
   const int kb0 = seg0 * A8_SEG + wave * A8_TILE, pos = min(c.wave_pos, seg1 * A8_SEG + A8_SEG - 1);
+  q_part q[DP / 64][1][A8_QJ];
+  a8_load_q<DP, 1>(a, c, q);
   A8Pages pages;
   pages.fill(a, c, seg0 * A8_SEG >> a.lp, pos);
 
-  struct Tile {
-    const A8Args& a;
-    const A8Rows<1>& c;
-    A8Pages& pages;
-    int pos, kb;                 // kb: of the tile that is asked for
-    float k_scale;
-    int v_exp;
-    u32x4 kr[4][DP / 64], vr[DP / 16];
-    __device__ __forceinline__ u32x4 k(int i, int j) const { return kr[i][j]; }
-    __device__ __forceinline__ u32x4 v(int dt) const { return vr[dt]; }
-    __device__ __forceinline__ bool wanted() const { return kb <= pos && kb + A8_TILE > c.wave_lo; }
-    __device__ __forceinline__ void ask_k() {
-      if (!wanted()) return;
-      if (((kb + A8_TILE - 1) >> a.lp) - pages.base >= 64) pages.fill(a, c, kb >> a.lp, pos);
-      const int kkey = kb + 16 * (c.r >> 2), vkey = kb + 16 * c.g, kl = (kkey >> a.lp) - pages.base, vl = (vkey >> a.lp) - pages.base;
-      k_scale = __shfl(pages.k_scale, kl);
-      v_exp = __shfl(pages.v_exp, vl);
-      v_exp = vkey <= c.wave_pos && vkey + 15 >= c.wave_lo ? v_exp : -256;
-      const uint8_t* kp = a.kc + pages.of_any(kl) + ((kkey & (a.P - 1)) + (c.r & 3)) * a.d;
+  A8Held<DP> t;
+  // Loads that stand under a condition are waited for where the ways meet again: every tile asks for the next one, the last for itself once more (from the cache).
+  const int tile_lo = max(c.wave_lo, seg0 * A8_SEG) & ~(A8_TILE - 1), tile_hi = max(pos, 0) & ~(A8_TILE - 1);
+  float k_scale;
+  int v_exp, v_key;
+  auto ask_k = [&](int kb) {
+    const int at = min(max(kb, tile_lo), tile_hi);
+    if (((at + A8_TILE - 1) >> a.lp) - pages.base >= 64) pages.fill(a, c, at >> a.lp, pos);
+    v_key = at + 16 * c.g;
+    k_scale = __shfl(pages.k_scale, ((at + 16 * (c.r >> 2)) >> a.lp) - pages.base);
+    v_exp = __shfl(pages.v_exp, (v_key >> a.lp) - pages.base);
+    v_exp = v_key <= c.wave_pos && v_key + 15 >= c.wave_lo ? v_exp : -256;
+    constexpr bool LINES = A8Held<DP>::LINES;
+    constexpr int HALVES = LINES ? 2 : 1;
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+      const int r = LINES ? (c.r & 7) + 8 * h : c.r, key = at + 16 * (r >> 2);
+      const uint8_t* kp = a.kc + pages.of_any((key >> a.lp) - pages.base) + ((key & (a.P - 1)) + (r & 3)) * a.d;
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int j = 0; j < DP / 64; ++j)
-          kr[s][j] = *reinterpret_cast<const u32x4*>(kp + 4 * s * a.d + min(64 * j + 16 * c.g, a.d - 16));     // beyond d: the last again, times q's zeros
+        for (int j = 0; j < DP / 64 / HALVES; ++j) {
+          const int piece = LINES ? 128 * j + 64 * (c.r >> 3) + 16 * c.g : 64 * j + 16 * c.g;
+          t.kr[s][HALVES * j + h] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + 4 * s * a.d + min(piece, a.d - 16)));     // beyond d: the last again, times q's zeros
+        }
     }
-    __device__ __forceinline__ void ask_v() {
-      if (!wanted()) return;
-      const int vkey = kb + 16 * c.g;
-      const uint8_t* vp = a.vc + pages.of_any((vkey >> a.lp) - pages.base) + c.r * a.P + (vkey & (a.P - 1));
+  };
+  auto ask_v = [&]() {
+    const uint8_t* vp = a.vc + pages.of_any((v_key >> a.lp) - pages.base) + c.r * a.P + (v_key & (a.P - 1));
 #pragma unroll
-      for (int dt = 0; dt < DP / 16; ++dt) vr[dt] = *reinterpret_cast<const u32x4*>(vp + min(16 * dt, a.d - 16) * a.P);     // and here for nothing
-    }
-    __device__ __forceinline__ void k_done() {
-      kb += A8_SEG / 2;
-      ask_k();
-    }
-    __device__ __forceinline__ void v_done() { ask_v(); }
-  } t{a, c, pages, pos, kb0, 1.f, -256};
-  t.ask_k();
-  t.ask_v();
-  q_part q[DP / 64][1][A8_QJ];
-  a8_load_q<DP, 1>(a, c, q);
+    for (int dt = 0; dt < DP / 16; ++dt) t.vr[dt] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vp + min(16 * dt, a.d - 16) * a.P));     // and here for nothing
+  };
+  ask_k(kb0);
+  ask_v();
+  a8_wait_q<DP, 1>(q);
   A8Sums<DP, 1> o;
   o.clear();
   for (int kb = kb0; (kb & ~(A8_SEG - 1)) <= seg1 * A8_SEG; kb += A8_SEG / 2) {
-    if (t.wanted()) {
-      a8_tile<2, DP, 1>(a, c, kb, t, t.k_scale, t.v_exp, __builtin_amdgcn_readfirstlane((int)over_groups_max((float)t.v_exp)), q, o);
-    } else {
-      t.k_done();
-      t.v_done();
+    const bool mine = kb <= pos && kb + A8_TILE > c.wave_lo;
+    const int exp_now = v_exp, top_now = __builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp));
+    f32x4 s[4][1];
+    if (mine) a8_scores<DP, 1>(t, k_scale, q, s);
+    ask_k(kb + A8_SEG / 2);
+    if (mine) {
+      if (kb >= c.all_lo && kb + A8_TILE - 1 <= c.all_pos && __all(exp_now > -256)) a8_weigh<1, DP, 1>(a, c, kb, t, s, exp_now, top_now, o);
+      else a8_weigh<0, DP, 1>(a, c, kb, t, s, exp_now, top_now, o);
     }
+    ask_v();
     if ((kb & (A8_SEG / 2)) == 0) continue;
     // Both tiles of the segment.
     const int seg = kb / A8_SEG;
@@ -609,8 +633,6 @@ struct A8Shared {
   __device__ __forceinline__ u32x4 k(int i, int j) const {
     return *reinterpret_cast<const u32x4*>(tile + (16 * i + r) * DP + (((4 * j + g) ^ A8Stage<DP, WAVES>::turn(r)) << 4));
   }
-  __device__ __forceinline__ void k_done() {}
-  __device__ __forceinline__ void v_done() {}
   __device__ __forceinline__ u32x4 v(int dt) const { return *reinterpret_cast<const u32x4*>(tile + A8_TILE * DP + (16 * dt + r) * 64 + ((g ^ (r >> 2)) << 4)); }
 };
 
@@ -694,7 +716,10 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
       top_exp = __builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp));
     }
     if (!all_see.value) v_exp = key <= c.wave_pos && key + 15 >= c.wave_lo ? v_exp : -256;
-    a8_tile<all_see.value, DP, NT>(a, c, kb, A8Shared<DP, WAVES>{stages + (i % A8_STAGES) * ST::BYTES, c.r, c.g}, k_scale, v_exp, top_exp, q, o);
+    const A8Shared<DP, WAVES> src{stages + (i % A8_STAGES) * ST::BYTES, c.r, c.g};
+    f32x4 s[4][NT];
+    a8_scores<DP, NT>(src, k_scale, q, s);
+    a8_weigh<all_see.value, DP, NT>(a, c, kb, src, s, v_exp, top_exp, o);
   };
   for (int i = 0; i < tiles;) {
     for (; i < tiles && !whole(i); ++i) step(i, std::integral_constant<int, 0>());
