@@ -222,16 +222,25 @@ struct A8Sums {
   float m[NT];
   f32x4 l[NT];                 // the same number in all four
   f32x4 acc[NT][DP / 16];
+  typename std::conditional<(DP > 128), uint64_t, uint32_t>::type bad[NT];     // bit 4 dt + i: acc[n][dt][i] is NaN, by a value that is (where tiles are in registers; else it is set so)
   int unit;
   __device__ __forceinline__ void clear() {
     unit = -256;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n] = A8_NONE;
+      bad[n] = 0;
       l[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt) acc[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+  }
+  // acc[n][dt] times a number.
+  __device__ __forceinline__ f32x4 times(int n, int dt, float by) const {
+    f32x4 x = acc[n][dt] * by;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (bad[n] >> (4 * dt + i) & 1) ? NAN : x[i];
+    return x;
   }
   __device__ __forceinline__ float scale() const {
 #ifdef VK_BF16
@@ -273,8 +282,8 @@ __device__ __forceinline__ void a8_scores(const SRC& src, float k_scale, const q
 //
 // A column's reference maximum follows its maximum only where that is more than 2^8 above: weights are 2^8 at most then (their sums are 32-bit, and 2^8 is nothing to
 // sixteen bits), and the sums are scaled in few tiles.  Which columns move is each column's own business; whether any does is the wave's.
-// WHOLE: 1: every column that stands for a row sees every key; 0: not so; 2: that is found out here.  (Both in one loop, on scores and sums that come together again, cost a copy of
-// the scores a tile; a loop each costs none: 225 -> 196 us for that prompt.)
+// WHOLE: 1: every column that stands for a row sees every key; 0: not so; 2: unknown, and found out for the values.  (What is only done under a condition must not touch scores and sums:
+// where the ways meet again they would be copied, and held twice.  A loop for each kind of tile in place of a condition: 225 -> 196 us for that prompt.)
 template <int WHOLE, int DP, int NT, typename SRC>
 __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, int kb, const SRC& src, f32x4 (&s)[4][NT], int v_exp, int top_exp, A8Sums<DP, NT>& o) {
   const bool there = v_exp > -256;
@@ -285,7 +294,7 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
   for (int n = 0; n < NT; ++n) {
     float top = -INFINITY;
     const int lo = c.lo[n] - first, pos = there ? c.pos[n] - first : -1;
-    if (full) {
+    if (WHOLE == 1) {
 #pragma unroll
       for (int x = 0; x < 16; ++x) top = fmaxf(top, s[x / 4][n][x % 4]);
     } else {
@@ -388,7 +397,10 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o.acc[n][dt][i] = o.acc[n][dt][i] + (count[n][i] > 0.f ? NAN : 0.f);
+        for (int i = 0; i < 4; ++i) {
+          if (SRC::HELD) o.bad[n] |= (decltype(o.bad[n] + 0))(count[n][i] > 0.f) << (4 * dt + i);
+          else o.acc[n][dt][i] = o.acc[n][dt][i] + (count[n][i] > 0.f ? NAN : 0.f);
+        }
       asm volatile("" ::: "memory");
     }
   }
@@ -437,16 +449,16 @@ struct A8Pages {
   __device__ __forceinline__ uint64_t of_any(int lane) const { return (uint64_t)(unsigned)__shfl((int)(at >> 32), lane) << 32 | (unsigned)__shfl((int)at, lane); }
 };
 
-// ---- up to 16 columns (decoded tokens): a workgroup takes segments of 512 keys one after the other, a wave two of a segment's tiles, every fourth.  They come straight into
-// registers: a tile's keys are asked for when the last tile's have been multiplied, its values when those have, so that there is something under way at any time and no
-// load waits for another (page numbers and scales are read 64 pages ahead; a page number read in turn would wait for all loads before it).  The waves' sums meet in LDS,
-// the segments' in a8_join_kernel.
+// ---- few columns (decoded and drafted tokens): a workgroup takes segments of 512 keys one after the other, a wave two of a segment's tiles, every fourth, for up to 16 NT columns.
+// Tiles come straight into registers: a tile's keys are asked for when the last tile's have been multiplied, its values when those have, so that there is something under way at any
+// time and no load waits for another (page numbers and scales are read 64 pages ahead; a page number read in turn would wait for all loads before it).  The waves' sums meet in LDS, the
+// segments' in a8_join_kernel.
 // A tile in registers.  Of heads of 128 a load takes eight rows of K in whole lines of the cache, 128 bytes, and not half of each of sixteen: the load of the other halves
 // would wait in the first cache for the lines that are under way, and what stands behind it too (200 -> 188 us for 64 rows of 8,192 keys).  So kr[i][0] has in lane rows 0..7 the first
 // half of rows 0..7, in lane rows 8..15 their second half, kr[i][1] the same of rows 8..15, and a lane's own row comes together when it is used.
 template <int DP>
 struct A8Held {
-  static constexpr bool LINES = DP % 128 == 0;
+  static constexpr bool HELD = true, LINES = DP % 128 == 0;
   u32x4 kr[4][DP / 64], vr[DP / 16];
   __device__ __forceinline__ u32x4 k(int i, int j) const {
     if (!LINES) return kr[i][j];
@@ -462,20 +474,20 @@ struct A8Held {
   __device__ __forceinline__ u32x4 v(int dt) const { return vr[dt]; }
 };
 
-template <int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void a8_few_kernel(A8Args a, int segs_each) {
+template <int DP, int NT>
+__global__ __launch_bounds__(256, DP <= 128 && NT == 1 ? 2 : 1) void a8_few_kernel(A8Args a, int segs_each, int blocks) {
   __shared__ float sums[4][DP / 16][64][4];
-  __shared__ float maxima[4][16], totals[4][16];
-  A8Rows<1> c;
-  const int kvh = blockIdx.x % a.nkv, item = blockIdx.x / a.nkv, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (!a8_rows<1>(a, item, kvh, 0, c)) return;
+  __shared__ float maxima[4][16 * NT], totals[4][16 * NT];
+  A8Rows<NT> c;
+  const int kvh = blockIdx.x % a.nkv, block = blockIdx.x / a.nkv % blocks, item = blockIdx.x / a.nkv / blocks, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (!a8_rows<NT>(a, item, kvh, block * 16 * NT, c)) return;
   int seg_first, seg_last;
   a8_segments(c.wave_lo, c.wave_pos, seg_first, seg_last);
   const int seg0 = max(seg_first, (int)blockIdx.y * segs_each), seg1 = min(seg_last, (int)blockIdx.y * segs_each + segs_each - 1);
   if (seg0 > seg1) return;
   const int kb0 = seg0 * A8_SEG + wave * A8_TILE, pos = min(c.wave_pos, seg1 * A8_SEG + A8_SEG - 1);
-  q_part q[DP / 64][1][A8_QJ];
-  a8_load_q<DP, 1>(a, c, q);
+  q_part q[DP / 64][NT][A8_QJ];
+  a8_load_q<DP, NT>(a, c, q);
   A8Pages pages;
   pages.fill(a, c, seg0 * A8_SEG >> a.lp, pos);
 
@@ -513,52 +525,54 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void a8_few_kernel(A8Args a
   };
   ask_k(kb0);
   ask_v();
-  a8_wait_q<DP, 1>(q);
-  A8Sums<DP, 1> o;
+  a8_wait_q<DP, NT>(q);
+  A8Sums<DP, NT> o;
   o.clear();
   for (int kb = kb0; (kb & ~(A8_SEG - 1)) <= seg1 * A8_SEG; kb += A8_SEG / 2) {
     const bool mine = kb <= pos && kb + A8_TILE > c.wave_lo;
     const int exp_now = v_exp, top_now = __builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp));
-    f32x4 s[4][1];
-    if (mine) a8_scores<DP, 1>(t, k_scale, q, s);
+    f32x4 s[4][NT];
+    if (mine) a8_scores<DP, NT>(t, k_scale, q, s);
     ask_k(kb + A8_SEG / 2);
-    if (mine) {
-      if (kb >= c.all_lo && kb + A8_TILE - 1 <= c.all_pos && __all(exp_now > -256)) a8_weigh<1, DP, 1>(a, c, kb, t, s, exp_now, top_now, o);
-      else a8_weigh<0, DP, 1>(a, c, kb, t, s, exp_now, top_now, o);
-    }
+    if (mine) a8_weigh<2, DP, NT>(a, c, kb, t, s, exp_now, top_now, o);
     ask_v();
     if ((kb & (A8_SEG / 2)) == 0) continue;
     // Both tiles of the segment.
     const int seg = kb / A8_SEG;
-    const float l = o.l[0][0];
-    if (c.g == 0) {
-      maxima[wave][c.r] = o.m[0];
-      totals[wave][c.r] = l;
-    }
-    __syncthreads();
-    const float top = fmaxf(fmaxf(maxima[0][c.r], maxima[1][c.r]), fmaxf(maxima[2][c.r], maxima[3][c.r])), by = exp2_fast(o.m[0] - top) * o.scale();
-    float total = 0.f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) total = __builtin_fmaf(totals[x][c.r], exp2_fast(maxima[x][c.r] - top), total);
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) *reinterpret_cast<f32x4*>(sums[wave][dt][lane]) = o.acc[0][dt] * by;
-    o.clear();
-    __syncthreads();
-    const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg) * a.cols_max + c.r;
-    if (c.r < c.cols) {
-#pragma unroll
-      for (int x = 0; x < DP / 64; ++x) {
-        const int dt = 4 * x + wave;
-        if (16 * dt >= a.d) continue;
-        f32x4 v = *reinterpret_cast<const f32x4*>(sums[0][dt][lane]);
-#pragma unroll
-        for (int y = 1; y < 4; ++y) v = v + *reinterpret_cast<const f32x4*>(sums[y][dt][lane]);
-        if (seg_first == seg_last) store_elems4(a8_out<1>(a, c, c.r) + 16 * dt, total == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v * (1.f / total));
-        else *reinterpret_cast<f32x4*>(a.part_acc + part * a.d + 16 * dt + 4 * c.g) = v;
+    for (int n = 0; n < NT; ++n)
+      if (c.g == 0) {
+        maxima[wave][16 * n + c.r] = o.m[n];
+        totals[wave][16 * n + c.r] = o.l[n][0];
       }
-      if (seg_first != seg_last && wave == 0 && c.g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * part) = f32x2{top, total};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      __syncthreads();                                  // the maxima are there; the sums of the columns before have been read
+      const int x0 = 16 * n + c.r, col = c.col0 + x0;
+      const float top = fmaxf(fmaxf(maxima[0][x0], maxima[1][x0]), fmaxf(maxima[2][x0], maxima[3][x0])), by = exp2_fast(o.m[n] - top) * o.scale();
+      float total = 0.f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) total = __builtin_fmaf(totals[x][x0], exp2_fast(maxima[x][x0] - top), total);
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt) *reinterpret_cast<f32x4*>(sums[wave][dt][lane]) = o.times(n, dt, by);
+      __syncthreads();
+      if (col < c.cols) {
+        const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg) * a.cols_max + col;
+#pragma unroll
+        for (int x = 0; x < DP / 64; ++x) {
+          const int dt = 4 * x + wave;
+          if (16 * dt >= a.d) continue;
+          f32x4 v = *reinterpret_cast<const f32x4*>(sums[0][dt][lane]);
+#pragma unroll
+          for (int y = 1; y < 4; ++y) v = v + *reinterpret_cast<const f32x4*>(sums[y][dt][lane]);
+          if (seg_first == seg_last) store_elems4(a8_out<NT>(a, c, col) + 16 * dt, total == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v * (1.f / total));
+          else *reinterpret_cast<f32x4*>(a.part_acc + part * a.d + 16 * dt + 4 * c.g) = v;
+        }
+        if (seg_first != seg_last && wave == 0 && c.g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * part) = f32x2{top, total};
+      }
     }
-    // The next segment's sums are written behind its first barrier, which no wave passes before all have read these.
+    o.clear();
+    __syncthreads();                                    // all have read the maxima: the next segment's may be written
   }
 }
 
@@ -628,6 +642,7 @@ __device__ __forceinline__ void a8_ask(const A8Args& a, const A8Pages& pg, const
 
 template <int DP, int WAVES>
 struct A8Shared {
+  static constexpr bool HELD = false;
   const uint8_t* tile;
   int r, g;
   __device__ __forceinline__ u32x4 k(int i, int j) const {
@@ -641,6 +656,8 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
   typedef A8Stage<DP, WAVES> ST;
   extern __shared__ __attribute__((aligned(1024))) uint8_t stages[];      // A8_STAGES tiles
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Which wave has which columns turns with the workgroup: where there are none for the last one it is not always the same unit of the CU that has nothing to do.
+  const unsigned turn = SPLIT ? blockIdx.x ^ blockIdx.x >> 3 ^ blockIdx.x >> 8 : 0;
   // The kv head first: the workgroups of one, which read the same pages, then fall to as few of the eight caches as there are.
   int unit = blockIdx.x;
   const int kvh = unit % a.nkv;
@@ -651,7 +668,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
   A8Rows<NT> c;
   A8Rows<NT * WAVES> all;                                                 // the workgroup's columns
   if (!a8_rows<NT * WAVES>(a, item, kvh, block * 16 * NT * WAVES, all)) return;
-  const bool mine = a8_rows<NT>(a, item, kvh, (block * WAVES + wave) * 16 * NT, c);
+  const bool mine = a8_rows<NT>(a, item, kvh, (block * WAVES + (wave + turn) % WAVES) * 16 * NT, c);
   int lo = all.wave_lo, pos = all.wave_pos, seg_first = 0, seg_last = 0;
   if (SPLIT) {
     a8_segments(lo, pos, seg_first, seg_last);
@@ -735,14 +752,14 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
       const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg) * a.cols_max + col;
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt)
-        if (16 * dt < a.d) *reinterpret_cast<f32x4*>(a.part_acc + part * a.d + 16 * dt + 4 * c.g) = o.acc[n][dt] * o.scale();
+        if (16 * dt < a.d) *reinterpret_cast<f32x4*>(a.part_acc + part * a.d + 16 * dt + 4 * c.g) = o.times(n, dt, o.scale());
       if (c.g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * part) = f32x2{o.m[n], l};
     } else {
       elem_t* to = a8_out<NT>(a, c, col);
       const float by = l == 0.f ? 0.f : o.scale() / l;
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt)
-        if (16 * dt < a.d) store_elems4(to + 16 * dt, l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o.acc[n][dt] * by);
+        if (16 * dt < a.d) store_elems4(to + 16 * dt, l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o.times(n, dt, by));
     }
   }
 }
@@ -856,16 +873,29 @@ int vk_paged_attention8(elem_t* out, const elem_t* q, const uint8_t* kc, const u
   a.part_ml = scratch + need / (d + 2) * d;
   const int64_t joins = (int64_t)n_items * nkv;
   VK_REQUIRE(joins < (1ll << 31) && nseg <= 65535, "attention8: %d items, %d keys: too many for one launch", n_items, max_k_len);
-  int cols = 16;                                        // of a block
-  if (a.cols_max <= 16) {
+  // Column tiles a wave: as many as there are columns, up to what a wave's registers hold beside a tile of the cache; more columns than that go through LDS.
+  const int most = F32 ? (d <= 64 ? 2 : 1) : d <= 64 ? 4 : d <= 128 ? 2 : 1, nt = (a.cols_max + 15) / 16;
+  int cols;                                             // of a block
+  if (nt <= most) {
+    cols = 16 * nt;
     // Workgroups of several segments where there are more than the card holds at once: what stands in front of a workgroup's first loads is then paid once.
-    const int64_t held = 2 * vk_device_cus();
+    const int64_t held = (nt == 1 ? 2 : 1) * vk_device_cus();
     const int each = (int)max((int64_t)1, min((int64_t)8, joins * nseg / (2 * held)));
     const dim3 grid((unsigned)joins, (nseg + each - 1) / each);
-    if (d <= 64) a8_few_kernel<64><<<grid, 256, 0, st>>>(a, each);
-    else if (d <= 128) a8_few_kernel<128><<<grid, 256, 0, st>>>(a, each);
-    else if (d <= 192) a8_few_kernel<192><<<grid, 256, 0, st>>>(a, each);
-    else a8_few_kernel<256><<<grid, 256, 0, st>>>(a, each);
+#define FEW(D, N) a8_few_kernel<D, N><<<grid, 256, 0, st>>>(a, each, 1)
+    if (d <= 64) {
+      if (nt == 1) FEW(64, 1);
+      else if (nt == 2) FEW(64, 2);
+#ifdef VK_BF16
+      else if (nt == 3) FEW(64, 3);
+      else FEW(64, 4);
+    } else if (d <= 128 && nt == 2) {
+      FEW(128, 2);
+#endif
+    } else if (d <= 128) FEW(128, 1);
+    else if (d <= 192) FEW(192, 1);
+    else FEW(256, 1);
+#undef FEW
     if (vk_check_launch("attention8")) return 1;
   } else {
     const bool two = a.cols_max <= 32 && d <= 192;      // two waves; of the largest heads' tiles a wave's share of the loads would not fit its registers
