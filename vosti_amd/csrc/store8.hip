@@ -87,7 +87,7 @@ __device__ __forceinline__ void read_angles(const Store8Args& a, int c0, int pla
   }
 }
 
-// Norm and turn of a lane's entries.  y: the head's own LPH * VK_VEC numbers of LDS.
+// Norm and turn of a lane's entries.  y: the head's own LPH * VK_VEC numbers of LDS, for rotations that are no whole vectors.
 template <int LPH, typename F>
 __device__ __forceinline__ void norm_and_turn(F (&v)[VK_VEC], const Store8Args& a, bool norm, const Turn& t, int c0, F* y) {
   if (norm) {
@@ -100,23 +100,23 @@ __device__ __forceinline__ void norm_and_turn(F (&v)[VK_VEC], const Store8Args& 
   }
   if (a.cos_t != nullptr) {
     const int h = a.rot_half;
-#pragma unroll
-    for (int e = 0; e < VK_VEC; ++e) y[c0 + e] = v[e];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
     F other[VK_VEC];
-    if (a.whole) {
-      const int at = c0 < h ? c0 + h : c0 < 2 * h ? c0 - h : c0;
+    if (a.whole) {                                      // another lane's vector
+      const int lane = threadIdx.x & 63, from = c0 < h ? lane + h / VK_VEC : c0 < 2 * h ? lane - h / VK_VEC : lane;
 #pragma unroll
-      for (int e = 0; e < VK_VEC; ++e) other[e] = y[at + e];
+      for (int e = 0; e < VK_VEC; ++e) other[e] = __shfl(v[e], from);
     } else {
 #pragma unroll
+      for (int e = 0; e < VK_VEC; ++e) y[c0 + e] = v[e];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
       for (int e = 0; e < VK_VEC; ++e) other[e] = y[c0 + e < h ? c0 + e + h : c0 + e < 2 * h ? c0 + e - h : c0 + e];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
     for (int e = 0; e < VK_VEC; ++e) v[e] = v[e] * (F)t.cs[e] + other[e] * (F)t.sn[e];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -134,11 +134,11 @@ __device__ __forceinline__ int rows_of(const Store8Args& a, int i, int& first, i
 constexpr int STORE8_TURN = 4 * 64 * VK_VEC;
 
 template <int LPH>
-__global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a, int first_block) {
+__global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a) {
   constexpr int HPW = 64 / LPH, ROWS = 4 * HPW;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ int wave_need[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPH, c0 = lane % LPH * VK_VEC, d = a.d, P = a.P, block = first_block + blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPH, c0 = lane % LPH * VK_VEC, d = a.d, P = a.P, block = blockIdx.x;
   const bool inside = c0 < d;
 
   if (block >= a.kv_blocks) {
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a,
   const int stood = exponent_of(*scale), old = off0 > 0 ? stood : CACHE8_LOWEST;
 
   double* y = reinterpret_cast<double*>(lds) + (wave * HPW + sub) * LPH * VK_VEC;
-  float* held = reinterpret_cast<float*>(lds + STORE8_TURN * sizeof(double));
+  float* held = reinterpret_cast<float*>(lds + (a.whole ? 0 : STORE8_TURN * sizeof(double)));
   // Rows i0 .. i0 + a.held - 1 into LDS: values as they are, keys normed and turned.  Returns the exponent that this lane's need.
   auto entries = [&](int i0, bool angles) {
     int need = CACHE8_LOWEST;
@@ -366,19 +366,9 @@ int vk_qkv_post8(const elem_t* qkv, int64_t row_stride, elem_t* q_out, uint8_t* 
   a.kv_blocks = (int)kv_blocks;
   // Rows that a workgroup holds in LDS: a page's, up to 32 KB, and one where every sequence has one.
   a.held = T <= S ? 1 : min(P, 32 * 1024 / 4 / d);
-  const int lds_q = STORE8_TURN * (int)sizeof(float), lds_kv = STORE8_TURN * (int)sizeof(double) + a.held * d * 4;
+  const int lds_q = a.whole ? 0 : STORE8_TURN * (int)sizeof(float), lds_kv = a.held * d * 4 + (a.whole ? 0 : STORE8_TURN * (int)sizeof(double));
   const int vecs = d / VK_VEC;
-  // Many rows: the q heads' workgroups apart, so that they do not take the LDS that the others need.
-  const bool apart = kv_blocks > 0 && q_blocks >= 2048;
-#define STORE8(L)                                                                                                                          \
-  {                                                                                                                                        \
-    if (apart) {                                                                                                                           \
-      store8_kernel<L><<<(unsigned)kv_blocks, STORE8_THREADS, lds_kv, st>>>(a, 0);                                                         \
-      store8_kernel<L><<<(unsigned)q_blocks, STORE8_THREADS, lds_q, st>>>(a, (int)kv_blocks);                                              \
-    } else {                                                                                                                               \
-      store8_kernel<L><<<(unsigned)(kv_blocks + q_blocks), STORE8_THREADS, kv_blocks > 0 ? lds_kv : lds_q, st>>>(a, 0);                    \
-    }                                                                                                                                      \
-  }
+#define STORE8(L) store8_kernel<L><<<(unsigned)(kv_blocks + q_blocks), STORE8_THREADS, kv_blocks > 0 ? lds_kv : lds_q, st>>>(a);
 #ifdef VK_BF16
   if (vecs <= 2) STORE8(2)
   else if (vecs <= 4) STORE8(4)
