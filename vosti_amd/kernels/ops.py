@@ -391,12 +391,21 @@ class Kernels:
         return out
 
     # ------------------------------------------------ caches of 8 bits, drafted tokens
-    def _here(self, *tensors) -> None:
-        """The launch goes to the current device: what lies on another one is refused."""
-        here = torch.cuda.current_device()
-        for t in tensors:
-            if t is not None and t.get_device() != here:
-                raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{here}")
+    @staticmethod
+    def _device() -> int:
+        try:
+            return torch.cuda.current_device()
+        except (RuntimeError, AssertionError):          # no GPU: no tensor lies there
+            return -2
+
+    def _at(self, t: torch.Tensor, what: str, dtype, shape, here: int) -> int:
+        """The address of a contiguous tensor of this type and shape on the current device (``here``: a launch goes there); anything else is refused."""
+        if isinstance(t, torch.Tensor) and t.get_device() == here and t.dtype == dtype and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+        self._check(t, what, dtype)
+        if t.shape != shape:
+            raise KernelError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+        raise KernelError(f"{what} lies on {t.device}, the current device is cuda:{here}")
 
     def empty_cache8(self, pages: int, nkv: int, page_size: int, d: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Keys [pages, nkv, page_size, d], values [pages, nkv, d, page_size] (both e4m3) and scales [pages, nkv, 2] of an empty 8-bit cache."""
@@ -404,17 +413,15 @@ class Kernels:
                 torch.zeros(pages, nkv, d, page_size, dtype=CACHE8_DTYPE, device="cuda"),
                 torch.zeros(pages, nkv, 2, dtype=torch.float32, device="cuda"))
 
-    def _cache8(self, k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, nkv: int, d: int) -> tuple[int, int]:
-        """Checks the three tensors; returns (pages, page size)."""
-        self._check(k_cache, "k cache", CACHE8_DTYPE)
-        if k_cache.dim() != 4 or k_cache.shape[1] != nkv or k_cache.shape[3] != d:
-            raise KernelError(f"k cache has shape {tuple(k_cache.shape)}, expected [pages, {nkv}, page size, {d}]")
+    def _cache8(self, k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, nkv: int, d: int, here: int) -> tuple[int, int, int, int, int]:
+        """Checks the three tensors; returns (pages, page size, their addresses)."""
+        if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4:
+            raise KernelError("k cache is no tensor [pages, kv heads, page size, head size]")
         pages, _, P, _ = k_cache.shape
         if P & (P - 1) or not CACHE8_PAGES[0] <= P <= CACHE8_PAGES[1]:
             raise KernelError(f"page size {P} of an 8-bit cache is no power of two from {CACHE8_PAGES[0]} to {CACHE8_PAGES[1]}")
-        self._check(v_cache, "v cache", CACHE8_DTYPE, (pages, nkv, d, P))
-        self._check(scales, "scales", torch.float32, (pages, nkv, 2))
-        return pages, P
+        return (pages, P, self._at(k_cache, "k cache", CACHE8_DTYPE, (pages, nkv, P, d), here), self._at(v_cache, "v cache", CACHE8_DTYPE, (pages, nkv, d, P), here),
+                self._at(scales, "scales", torch.float32, (pages, nkv, 2), here))
 
     def qkv_post8(self, qkv: torch.Tensor, *, nq: int, nkv: int, d: int, k_cache: torch.Tensor | None, v_cache: torch.Tensor | None,
                   scales: torch.Tensor | None, q_w: torch.Tensor | None, k_w: torch.Tensor | None, eps: float, cos: torch.Tensor | None,
@@ -427,40 +434,37 @@ class Kernels:
         16-byte vectors.  A page's scales grow with its entries and start anew when a call writes its first place; a page that two sequences of a call write
         to is undefined.  ``max_k_len``: the host's bound on k_len, which tables and block tables cover; a sequence beyond it is left out.  Rows behind the
         last sequence's are left as they were."""
+        here = self._device()
         if qkv.dim() != 2 or nq < 0 or nkv < 0 or qkv.shape[1] != (nq + 2 * nkv) * d:
             raise KernelError(f"qkv_post8: row tensor {tuple(qkv.shape)} is not [T, (nq + 2 nkv) * d = {(nq + 2 * nkv) * d}]")
         T, W = qkv.shape
-        if not qkv.is_cuda or qkv.dtype != self.dtype or (W and qkv.stride(1) != 1):
-            raise KernelError("qkv_post8: rows must be a GPU tensor of the element type with a contiguous last axis")
+        if qkv.get_device() != here or qkv.dtype != self.dtype or (W and qkv.stride(1) != 1):
+            raise KernelError("qkv_post8: rows must be a tensor of the element type on the current GPU with a contiguous last axis")
+        qp = kcp = vcp = scp = qwp = kwp = cp = sp = None
+        pages = P = wf = half = 0
         if nq:
-            q_out = self.empty(T, nq, d) if q_out is None else q_out
-            self._elem(q_out, "q_out", T, nq, d)
-        wf = 0
-        qwp = kwp = None
+            q_out = torch.empty((T, nq, d), dtype=self.dtype, device=qkv.device) if q_out is None else q_out
+            qp = self._at(q_out, "q_out", self.dtype, (T, nq, d), here)
+        if q_w is not None and k_w is not None and q_w.dtype != k_w.dtype:
+            raise KernelError("qkv_post8: q and k norm weights must have the same type")
         if q_w is not None:
-            qwp, wf = self._weight(q_w, "q norm weight", d)
+            wf = int(q_w.dtype == torch.float32)
+            qwp = self._at(q_w, "q norm weight", torch.float32 if wf else self.dtype, (d,), here)
         if k_w is not None:
-            kwp, wf2 = self._weight(k_w, "k norm weight", d)
-            if q_w is not None and wf2 != wf:
-                raise KernelError("qkv_post8: q and k norm weights must have the same type")
-            wf = wf2
-        cp = sp = None
-        half = 0
+            wf = int(k_w.dtype == torch.float32)
+            kwp = self._at(k_w, "k norm weight", torch.float32 if wf else self.dtype, (d,), here)
         if cos is not None:
             if cos.dim() != 2 or cos.shape[0] < max_k_len:
                 raise KernelError(f"qkv_post8: tables {tuple(cos.shape)} do not cover {max_k_len} places")
             half = cos.shape[1]
-            cp, sp = self._elem(cos, "cos", *cos.shape), self._elem(sin, "sin", *cos.shape)
+            cp, sp = self._at(cos, "cos", self.dtype, cos.shape, here), self._at(sin, "sin", self.dtype, cos.shape, here)
         S, width = block_table.shape
-        tp = self._i32(block_table, "block table", S, width)
-        cup, klp = self._i32(cu_q, "cu_q", S + 1), self._i32(k_len, "k_len", S)
-        pages, P, kcp, vcp, scp = 0, 0, None, None, None
+        tp = self._at(block_table, "block table", torch.int32, (S, width), here)
+        cup, klp = self._at(cu_q, "cu_q", torch.int32, (S + 1,), here), self._at(k_len, "k_len", torch.int32, (S,), here)
         if nkv:
-            pages, P = self._cache8(k_cache, v_cache, scales, nkv, d)
-            kcp, vcp, scp = k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr()
-        self._here(qkv, q_out if nq else None, k_cache, v_cache, scales, q_w, k_w, cos, sin, block_table, cu_q, k_len)
-        self._call(self.lib.vk_qkv_post8, qkv.data_ptr(), qkv.stride(0) if T > 1 else W, q_out.data_ptr() if nq else None, kcp, vcp, scp, qwp, kwp, wf, cp, sp,
-                   half, tp, width, cup, klp, T, S, nq, nkv, d, P, pages, max_k_len, float(eps), self._stream())
+            pages, P, kcp, vcp, scp = self._cache8(k_cache, v_cache, scales, nkv, d, here)
+        self._call(self.lib.vk_qkv_post8, qkv.data_ptr(), qkv.stride(0) if T > 1 else W, qp, kcp, vcp, scp, qwp, kwp, wf, cp, sp, half, tp, width, cup, klp, T, S,
+                   nq, nkv, d, P, pages, max_k_len, eps, self._stream())
         return q_out if nq else None
 
     def attn8_scratch_floats(self, items: int, item_rows: int, nq: int, d: int, max_k_len: int) -> int:
@@ -477,26 +481,25 @@ class Kernels:
         to 16 rows (decoded tokens, drafted ones) have their keys split over workgroups, whose sums meet in ``scratch`` (``attn8_scratch_floats``;
         without it the call takes memory of its own); larger ones are for prompts.  ``max_k_len`` is the host's bound on k_len; the block table must
         cover it, and keys beyond it may be left out.  Rows that no item names are left as they were."""
+        here = self._device()
         if q.dim() != 3 or k_cache.dim() != 4:
             raise KernelError(f"attention8: q {tuple(q.shape)} is not [T, heads, size], or the k cache {tuple(k_cache.shape)} not [pages, kv heads, page size, size]")
         T, nq, d = q.shape
         nkv = k_cache.shape[1]
-        self._elem(q, "q", T, nq, d)
-        pages, P = self._cache8(k_cache, v_cache, scales, nkv, d)
         S, W = block_table.shape
-        tp = self._i32(block_table, "block table", S, W)
-        cup, klp = self._i32(cu_q, "cu_q", S + 1), self._i32(k_len, "k_len", S)
         n_items = items.shape[0]
-        ip = self._i32(items, "items", n_items, 2)
+        qp = self._at(q, "q", self.dtype, (T, nq, d), here)
+        pages, P, kcp, vcp, scp = self._cache8(k_cache, v_cache, scales, nkv, d, here)
+        tp, cup = self._at(block_table, "block table", torch.int32, (S, W), here), self._at(cu_q, "cu_q", torch.int32, (S + 1,), here)
+        klp, ip = self._at(k_len, "k_len", torch.int32, (S,), here), self._at(items, "items", torch.int32, (n_items, 2), here)
         out = torch.empty_like(q) if out is None else out
-        self._elem(out, "out", T, nq, d)
-        need = self.attn8_scratch_floats(n_items, item_rows, nq, d, max_k_len) if item_rows <= 16 else 0
-        if need and scratch is None:
-            scratch = torch.empty(need, dtype=torch.float32, device=q.device)
-        self._here(q, k_cache, v_cache, scales, block_table, cu_q, k_len, items, scratch, out)
-        self._call(self.lib.vk_paged_attention8, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), tp, W, cup, klp, ip,
-                   n_items, item_rows, self._f32(scratch, "scratch") if need else None, scratch.numel() if need else 0, T, S, nq, nkv, d, P, pages, max_k_len,
-                   int(window), float(scale), self._stream())
+        op = self._at(out, "out", self.dtype, (T, nq, d), here)
+        need, scratch_p = self.attn8_scratch_floats(n_items, item_rows, nq, d, max_k_len) if item_rows <= 16 else 0, None
+        if need:
+            scratch = torch.empty(need, dtype=torch.float32, device=q.device) if scratch is None else scratch
+            scratch_p = self._at(scratch, "scratch", torch.float32, (scratch.numel(),), here)
+        self._call(self.lib.vk_paged_attention8, op, qp, kcp, vcp, scp, tp, W, cup, klp, ip, n_items, item_rows, scratch_p, scratch.numel() if need else 0, T, S, nq, nkv, d,
+                   P, pages, max_k_len, window, scale, self._stream())
         return out
 
     def verify(self, logits: torch.Tensor, draft_ids: torch.Tensor, cu: torch.Tensor, *, draft_logits: torch.Tensor | None = None,
@@ -510,23 +513,24 @@ class Kernels:
 
         Returns (tokens [R], counts [S], accept [D]): sequence s's rows of ``tokens`` begin with counts[s] tokens (the standing ones and the drawn one) and go on
         with -1; ``accept`` is min(1, p / q) of every drafted token.  What lies behind the last sequence is not written."""
+        here = self._device()
         if logits.dim() != 2 or draft_ids.dim() != 1 or cu.dim() != 1 or cu.shape[0] < 1:
             raise KernelError(f"verify: logits {tuple(logits.shape)}, draft ids {tuple(draft_ids.shape)} and cu {tuple(cu.shape)} are not [R, V], [D], [S + 1]")
         R, V = logits.shape
         D, S = draft_ids.shape[0], cu.shape[0] - 1
-        lp, ip, cup = self._elem(logits, "logits", R, V), self._i32(draft_ids, "draft ids", D), self._i32(cu, "cu", S + 1)
-        dp = self._elem(draft_logits, "draft logits", D, V) if draft_logits is not None else None
+        lp, ip, cup = self._at(logits, "logits", self.dtype, (R, V), here), self._at(draft_ids, "draft ids", torch.int32, (D,), here), self._at(cu, "cu", torch.int32, (S + 1,), here)
+        dp = self._at(draft_logits, "draft logits", self.dtype, (D, V), here) if draft_logits is not None else None
         tp = ap = up = None
         if temps is not None:
             if accept_uniforms is None or draw_uniforms is None:
                 raise KernelError("verify: temperatures need random numbers")
-            tp, ap, up = self._f32(temps, "temps", S), self._f32(accept_uniforms, "accept uniforms", D), self._f32(draw_uniforms, "draw uniforms", S)
-        self._here(logits, draft_ids, cu, draft_logits, temps, accept_uniforms, draw_uniforms)
-        tokens = torch.empty(R, dtype=torch.int32, device=logits.device)
-        counts = torch.empty(S, dtype=torch.int32, device=logits.device)
-        accept = torch.empty(D, dtype=torch.float32, device=logits.device)
-        need = int(self.lib.vk_verify_scratch_bytes(R, D, S, V))
-        scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
+            tp, ap = self._at(temps, "temps", torch.float32, (S,), here), self._at(accept_uniforms, "accept uniforms", torch.float32, (D,), here)
+            up = self._at(draw_uniforms, "draw uniforms", torch.float32, (S,), here)
+        dev = logits.device
+        tokens, counts = torch.empty(R, dtype=torch.int32, device=dev), torch.empty(S, dtype=torch.int32, device=dev)
+        accept = torch.empty(D, dtype=torch.float32, device=dev)
+        need = self.lib.vk_verify_scratch_bytes(R, D, S, V)
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
         self._call(self.lib.vk_verify, tokens.data_ptr(), counts.data_ptr(), accept.data_ptr(), lp, ip, cup, dp, tp, ap, up, scratch.data_ptr(), need, R, D, S, V,
                    self._stream())
         return tokens, counts, accept
