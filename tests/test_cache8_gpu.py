@@ -211,6 +211,25 @@ ATTENDS = [
     ("f32", [30], [90], 4, 1, 256, 64, 20, 30),
     ("f32", [140], [140], 2, 1, 64, 64, 0, 128),
     ("f32", [25], [50], 3, 1, 128, 64, 0, 25),
+    # Columns (rows of an item times q heads of a kv head) from one tile to more than a workgroup takes at once, for every width of a head.
+    ("bf16", [8, 3], [700, 40], 8, 2, 64, 64, 0, 8),
+    ("bf16", [12, 7], [530, 1100], 8, 2, 48, 16, 90, 12),
+    ("bf16", [16, 1], [100, 600], 4, 1, 64, 32, 0, 16),
+    ("bf16", [16, 9], [620, 30], 5, 1, 32, 64, 0, 16),
+    ("bf16", [4, 2], [1040, 300], 16, 2, 128, 64, 0, 4),
+    ("bf16", [3, 3], [70, 600], 8, 1, 112, 16, 65, 3),
+    ("bf16", [5, 2], [513, 90], 8, 1, 128, 128, 0, 5),
+    ("bf16", [4], [600], 8, 1, 192, 64, 0, 4),
+    ("bf16", [7], [130], 8, 1, 144, 32, 40, 7),
+    ("bf16", [2, 2], [520, 33], 16, 1, 256, 64, 0, 2),
+    ("bf16", [11], [700], 8, 1, 208, 16, 0, 11),
+    ("bf16", [100], [140], 8, 8, 160, 64, 0, 100),
+    ("f32", [4, 1], [600, 20], 8, 1, 64, 64, 0, 4),
+    ("f32", [3], [530], 8, 1, 128, 16, 0, 3),
+    ("f32", [6], [90], 8, 1, 96, 64, 30, 6),
+    ("f32", [3], [520], 8, 1, 176, 32, 0, 3),
+    ("f32", [2, 5], [30, 513], 10, 1, 256, 64, 0, 5),
+    ("f32", [9], [65], 1, 1, 256, 256, 0, 9),
 ]
 
 
@@ -305,6 +324,76 @@ def test_a_row_is_the_same_bits_in_any_company(name):
         alone = attend(k, q[at:at + n].contiguous(), cache, table[s:s + 1], [n], keys[s:s + 1], 3, max_k_len=1500)
         assert torch.equal(got[at:at + n], alone)
         at += n
+
+
+def test_arrays_that_say_more_than_there_is():
+    """Lengths beyond the bound, rows and sequences that the arrays do not have, a table of numbers of nothing: what exists is computed, the rest left as it was."""
+    k, P, d = kernels_for("bf16"), 16, 64
+    rng = np.random.default_rng(21)
+    cache = filled(rng, 6, 1, P, d)
+    table = np.array([[0, 1, 2, 3], [4, -7, 10 ** 9, 6], [5, 5, 5, 5], [1, 1, 1, 1], [2, 2, 2, 2]])
+    for rows in (3, 30):
+        q = torch.from_numpy(rng.standard_normal((4 * rows, 2, d))).to(torch.bfloat16).cuda()
+        cu = ints([0, rows, 2 * rows, 3 * rows, 2 ** 31 - 1, -2 ** 31])
+        keys = ints([2 ** 31 - 1, 40, -2 ** 31, 9, 9])
+        out = torch.full_like(q, 7.0)
+        items = ints([(0, 0), (1, 0), (2, 0), (3, 0), (4, 0), (0, 2 ** 31 - 1), (5, 0), (-2 ** 31, 0), (2, rows - 1)])
+        k.paged_attention8(q, *cache, ints(table), cu, keys, items, item_rows=rows, scale=0.1, max_k_len=50, out=out)
+        # Sequence 0's rows stand far behind the bound and see all 50 keys below it; 1 has the keys of its one page; 2 has none; 3 and 4 do not exist.
+        kk = host(cache[0])[[0, 1, 2, 3], 0] * host(cache[2])[[0, 1, 2, 3], 0, 0][:, None, None]
+        vv = host(cache[1])[[0, 1, 2, 3], 0].swapaxes(1, 2) * host(cache[2])[[0, 1, 2, 3], 0, 1][:, None, None]
+        kk, vv = kk.reshape(-1, d)[:50], vv.reshape(-1, d)[:50]
+        w = np.exp(0.1 * host(q[:rows]) @ kk.T)
+        want = (w / w.sum(-1, keepdims=True)) @ vv
+        assert np.abs(host(out[:rows]) - want).max() <= 2.0 ** -7 * np.abs(vv).max()
+        close(out[rows:2 * rows], attention(host(q[rows:2 * rows]), *map(host, cache), table[1:2], [0, rows], [40], 0.1), "bf16", d)
+        assert not out[2 * rows:3 * rows].any() and out[3 * rows:].eq(7.0).all()
+    before = [host(t) for t in cache]
+    x = torch.ones(12, 2 * d, dtype=torch.bfloat16, device="cuda")
+    k.qkv_post8(x, nq=0, nkv=1, d=d, k_cache=cache[0], v_cache=cache[1], scales=cache[2], q_w=None, k_w=None, eps=0.0, cos=None, sin=None, block_table=ints(table),
+                cu_q=ints([0, 3, 6, 2 ** 31 - 1, -2 ** 31, -1]), k_len=ints([2 ** 31 - 1, 2, 9, 9, -2 ** 31]), max_k_len=60)
+    for a, b in zip(cache, before):
+        assert np.array_equal(host(a), b)
+
+
+def test_scales_before_the_window_do_not_matter():
+    """A page that lies before every row's window has been given to another sequence, with a scale of another size."""
+    k, P, d, window = kernels_for("bf16"), 16, 64, 20
+    rng = np.random.default_rng(22)
+    for most in (2, 24):
+        rows, keys = [most], [110]
+        table, pages = tables(rng, keys, P)
+        kc, vc, scales = filled(rng, pages, 1, P, d)
+        q = torch.from_numpy(rng.standard_normal((most, 4, d))).to(torch.bfloat16).cuda()
+        want = attend(k, q, (kc, vc, scales), table, rows, keys, most, window)
+        first = (110 - most - window + 1) // P
+        scales[table[0, :first]] = 2.0 ** 100
+        scales[table[0, 0]] = float("nan")
+        assert torch.equal(want, attend(k, q, (kc, vc, scales), table, rows, keys, most, window))
+        table[0, :first] = -1
+        assert torch.equal(want, attend(k, q, (kc, vc, scales), table, rows, keys, most, window))
+
+
+def test_on_streams_of_their_own():
+    """Two calls at once, each with its own memory, in either order."""
+    k, P, d = kernels_for("bf16"), 64, 128
+    rng = np.random.default_rng(23)
+    work = []
+    for keys in ([3000, 200], [900, 1500]):
+        table, pages = tables(rng, keys, P)
+        cache = filled(rng, pages, 2, P, d)
+        q = torch.from_numpy(rng.standard_normal((4, 8, d))).to(torch.bfloat16).cuda()
+        work.append((q, cache, table, keys, attend(k, q, cache, table, [2, 2], keys, 2)))
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for (q, cache, table, keys, _), st in zip(work, streams):
+            with torch.cuda.stream(st):
+                got.append(attend(k, q, cache, table, [2, 2], keys, 2))
+        torch.cuda.synchronize()
+        for (*_, want), g in zip(work, got):
+            assert torch.equal(want, g)
 
 
 def test_offsets_beyond_32_bits():

@@ -126,6 +126,10 @@ def test_ids_outside_the_vocabulary_and_sequences_without_rows():
             for _ in range(3):
                 check("bf16", logits, np.array(ids), cu, d, [0.9] * 6, rng.random(6), rng.random(6))
     assert kernels_for("bf16").verify(logits, ints(np.zeros(0)), ints([0]))[1].shape == (0,)
+    # Sequences that the arrays do not hold: no tokens.
+    for cu in ([0, 3, 10], [-1, 3], [0, 2 ** 31 - 1, -2 ** 31], [5, 2], [0, 9]):
+        counts = kernels_for("bf16").verify(logits, ints([1, 2, 3]), ints(cu))[1].tolist()
+        assert counts == {(0, 3, 10): [counts[0], 0]}.get(tuple(cu), [0] * (len(cu) - 1)) and 0 <= counts[0] <= 3
 
 
 def test_refusals():
@@ -251,6 +255,10 @@ def test_a_recorded_step_is_the_step(name):
         graph.replay()
         other.set(states[0], np.random.default_rng(step))
         other.forward()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+        twin.replay()                                           # the other recording shares its memory with the first, and appends what is there
+        graph.replay()
         for a, b in zip(out, want):
             assert torch.equal(a, b)
         for c, e in zip(m.caches, eager.caches):

@@ -37,7 +37,7 @@ struct A8Args {
   const float* scales;
   const int32_t *table, *cu_q, *k_len, *items;
   float *part_ml, *part_acc;   // per (item, kv head, segment, column): maximum and sum; d sums
-  int W, T, S, nq, nkv, d, P, lp, pages, group, item_rows, cols_max, window, nseg, n_items;
+  int W, T, S, nq, nkv, d, P, lp, pages, group, item_rows, cols_max, window, nseg, n_items, max_keys;
   float scale_log2;
 };
 
@@ -156,23 +156,25 @@ __device__ __forceinline__ bool a8_rows(const A8Args& a, int item, int kvh, int 
   const int first = __builtin_amdgcn_readfirstlane(a.items[2 * item + 1]);
   if ((unsigned)c.seq >= (unsigned)a.S || first < 0) return false;
   const int t0 = __builtin_amdgcn_readfirstlane(a.cu_q[c.seq]), t1 = __builtin_amdgcn_readfirstlane(a.cu_q[c.seq + 1]);
-  if (t0 < 0 || t1 > a.T) return false;
+  if (t0 < 0 || t1 > a.T || t1 <= t0 || first >= t1 - t0) return false;
   c.rows = min(a.item_rows, t1 - t0 - first);
   c.cols = c.rows * a.group;
   c.col0 = col0;
-  if (c.rows <= 0 || col0 >= c.cols) return false;
+  if (col0 >= c.cols) return false;
   c.tok0 = t0 + first;
-  c.pos0 = __builtin_amdgcn_readfirstlane(a.k_len[c.seq]) - (t1 - t0) + first;
-  const int row_first = col0 / a.group, row_last = (min(c.cols, col0 + 16 * NT) - 1) / a.group;
-  c.all_pos = c.pos0 + row_first;
-  c.wave_pos = c.pos0 + row_last;
-  c.wave_lo = a.window > 0 ? max(0, c.all_pos - a.window + 1) : 0;
-  c.all_lo = a.window > 0 ? max(0, c.wave_pos - a.window + 1) : 0;
+  c.pos0 = max(__builtin_amdgcn_readfirstlane(a.k_len[c.seq]), 0) - (t1 - t0) + first;
+  // Keys from max_keys on are not looked for, whatever k_len says: neither the table nor the launch has a place for them.
+  const int row_first = col0 / a.group, row_last = (min(c.cols, col0 + 16 * NT) - 1) / a.group, end = a.max_keys - 1;
+  c.all_pos = min(c.pos0 + row_first, end);
+  c.wave_pos = min(c.pos0 + row_last, end);
+  c.wave_lo = a.window > 0 ? max(0, c.pos0 + row_first - a.window + 1) : 0;
+  c.all_lo = a.window > 0 ? max(0, c.pos0 + row_last - a.window + 1) : 0;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int col = col0 + 16 * n + c.r;
-    c.pos[n] = col < c.cols ? c.pos0 + col / a.group : -1;
-    c.lo[n] = a.window > 0 ? max(0, c.pos[n] - a.window + 1) : 0;
+    const int pos = c.pos0 + col / a.group;
+    c.pos[n] = col < c.cols ? min(pos, end) : -1;
+    c.lo[n] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
   }
   return true;
 }
@@ -771,7 +773,7 @@ __global__ __launch_bounds__(256) void a8_join_kernel(A8Args a, int cols) {
   if (!a8_rows<1>(a, item, kvh, col, c)) return;
   const int block0 = col / cols * cols, row_first = block0 / a.group, row_last = (min(c.cols, block0 + cols) - 1) / a.group;
   int seg_first, seg_last;
-  a8_segments(a.window > 0 ? max(0, c.pos0 + row_first - a.window + 1) : 0, c.pos0 + row_last, seg_first, seg_last);
+  a8_segments(a.window > 0 ? max(0, c.pos0 + row_first - a.window + 1) : 0, min(c.pos0 + row_last, a.max_keys - 1), seg_first, seg_last);
   if (seg_first == seg_last) return;                    // the other kernel wrote the result
   const int64_t part0 = ((int64_t)item * a.nkv + kvh) * a.nseg * a.cols_max + col;
   float top = A8_NONE;
@@ -859,7 +861,7 @@ int vk_paged_attention8(elem_t* out, const elem_t* q, const uint8_t* kc, const u
   VK_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)scratch) % 16 == 0, "attention8: rows, cache and scratch have to lie on 16 bytes");
   const int group = nq / nkv, nseg = max(1, (int)(((int64_t)max_k_len + A8_SEG - 1) / A8_SEG));
   A8Args a{q, out, kc, vc, scales, table, cu_q, k_len, items, nullptr, nullptr, W, T, S, nq, nkv, d, P, 0, pages, group, item_rows, item_rows * group, window, nseg,
-           n_items, scale * 1.4426950408889634f};
+           n_items, max_k_len, scale * 1.4426950408889634f};
   while (1 << a.lp < P) ++a.lp;
   constexpr bool F32 = sizeof(elem_t) == 4;
   if (item_rows > 16) {

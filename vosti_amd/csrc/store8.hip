@@ -126,8 +126,8 @@ __device__ __forceinline__ int rows_of(const Store8Args& a, int i, int& first, i
   if (i >= a.S) return 0;
   first = a.cu_q[i];
   keys = a.k_len[i];
-  const int end = a.cu_q[i + 1], n = end - first;
-  return first >= 0 && end <= a.T && n > 0 && n <= keys && keys <= a.max_k_len ? n : 0;
+  const int end = a.cu_q[i + 1];
+  return first >= 0 && first < end && end <= a.T && end - first <= keys && keys <= a.max_k_len ? end - first : 0;
 }
 
 // LDS of a workgroup: each wave's heads while they turn, and the new entries of a page, `held` rows of d numbers, between their maximum and their rounding.

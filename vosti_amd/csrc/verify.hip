@@ -133,11 +133,11 @@ __device__ __forceinline__ int wave_min_i(int v) {
 __device__ __forceinline__ int drafts_of(const VerifyArgs& a, int base, int& first, int& draft, int& seen) {
   const int i = base + (threadIdx.x & 63);
   first = i < a.S ? a.cu[i] : 0;
-  const int rows = i < a.S ? a.cu[i + 1] - first : 0;
+  const int end = i < a.S ? a.cu[i + 1] : 0, rows = first >= 0 && first < end && end <= a.R ? end - first : 0;
   const uint64_t some = __ballot(rows > 0);
   draft = first - seen - __builtin_popcountll(some & ((1ull << (threadIdx.x & 63)) - 1));
   seen += __builtin_popcountll(some);
-  return rows > 0 && first >= 0 && first + rows <= a.R && draft >= 0 && draft + rows - 1 <= a.D ? rows - 1 : -1;
+  return rows > 0 && draft >= 0 && draft + rows - 1 <= a.D ? rows - 1 : -1;
 }
 __device__ __forceinline__ double per_temperature(const VerifyArgs& a, int seq) {        // log2(e) / T; 0: the maximum alone
   const float t = a.temps != nullptr ? a.temps[seq] : 0.f;
