@@ -374,6 +374,21 @@ def test_scales_before_the_window_do_not_matter():
         assert torch.equal(want, attend(k, q, (kc, vc, scales), table, rows, keys, most, window))
 
 
+@pytest.mark.parametrize("most", (16, 128))
+def test_a_window_longer_than_the_keys_hides_none(most):
+    """Among rows that stand before the first key, where a window's begin could leave 32 bits."""
+    k, P, d = kernels_for("bf16"), 32, 64
+    rng = np.random.default_rng(23)
+    rows, keys = [40, 3], [25, 60]
+    table, pages = tables(rng, keys, P)
+    cache = filled(rng, pages, 2, P, d)
+    q = torch.from_numpy(rng.standard_normal((43, 4, d))).to(torch.bfloat16).cuda()
+    want = attend(k, q, cache, table, rows, keys, most)
+    assert not want[:15].any() and want[15:].abs().amax(-1).gt(0).all()
+    for window in (60, 64, 2 ** 31 - 1):
+        assert torch.equal(want, attend(k, q, cache, table, rows, keys, most, window))
+
+
 def test_on_streams_of_their_own():
     """Two calls at once, each with its own memory, in either order."""
     k, P, d = kernels_for("bf16"), 64, 128
@@ -432,7 +447,7 @@ def test_refusals():
     att(), put()
     for bad in (dict(q=q.float()), dict(q=q[:, :, :32]), dict(q=q.cpu()), dict(q=q[:, :3].contiguous()), dict(kc=kc.float()), dict(vc=kc), dict(sc=sc[:, :1]), dict(table=table.long()),
                 dict(cu=ints([0])), dict(kl=ints([3, 3])), dict(it=ints([0, 0])), dict(item_rows=0), dict(item_rows=129), dict(window=-1), dict(max_k_len=33),
-                dict(out=q[:2]), dict(max_k_len=-1)):
+                dict(out=q[:2]), dict(max_k_len=-1), dict(item_rows=-1), dict(window=2 ** 32 + 5), dict(max_k_len=2 ** 32 + 5)):
         with pytest.raises(KernelError):
             att(**bad)
     small = k.empty_cache8(4, 2, 8, 64), k.empty_cache8(2, 2, 512, 64), k.empty_cache8(2, 2, 48, 64)
@@ -447,7 +462,7 @@ def test_refusals():
     put(cos=cos, sin=cos)
     for bad in (dict(x=x[:, 1:]), dict(x=x.float()), dict(x=x.t()), dict(nq=3), dict(d=24, x=x[:, :192].contiguous()), dict(cos=cos[:31], sin=cos[:31]), dict(cos=cos, sin=cos.float()),
                 dict(cos=torch.zeros(32, 33, dtype=torch.bfloat16, device="cuda"), sin=torch.zeros(32, 33, dtype=torch.bfloat16, device="cuda")), dict(q_w=x[0, :32]),
-                dict(q_w=x[0, :64].contiguous(), k_w=torch.zeros(64, device="cuda")), dict(max_k_len=33), dict(q_out=q[:2]), dict(k_cache=vc), dict(scales=sc.double())):
+                dict(q_w=x[0, :64].contiguous(), k_w=torch.zeros(64, device="cuda")), dict(max_k_len=33), dict(max_k_len=2 ** 32 + 5), dict(max_k_len=-1), dict(q_out=q[:2]), dict(k_cache=vc), dict(scales=sc.double())):
         with pytest.raises(KernelError):
             put(**bad)
     unaligned = torch.zeros(3 * 512 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(3, 512)

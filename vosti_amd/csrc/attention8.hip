@@ -477,12 +477,12 @@ struct A8Held {
 };
 
 template <int DP, int NT>
-__global__ __launch_bounds__(256, DP <= 128 && NT == 1 ? 2 : 1) void a8_few_kernel(A8Args a, int segs_each, int blocks) {
+__global__ __launch_bounds__(256, DP <= 128 && NT == 1 ? 2 : 1) void a8_few_kernel(A8Args a, int segs_each) {
   __shared__ float sums[4][DP / 16][64][4];
   __shared__ float maxima[4][16 * NT], totals[4][16 * NT];
   A8Rows<NT> c;
-  const int kvh = blockIdx.x % a.nkv, block = blockIdx.x / a.nkv % blocks, item = blockIdx.x / a.nkv / blocks, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (!a8_rows<NT>(a, item, kvh, block * 16 * NT, c)) return;
+  const int kvh = blockIdx.x % a.nkv, item = blockIdx.x / a.nkv, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (!a8_rows<NT>(a, item, kvh, 0, c)) return;
   int seg_first, seg_last;
   a8_segments(c.wave_lo, c.wave_pos, seg_first, seg_last);
   const int seg0 = max(seg_first, (int)blockIdx.y * segs_each), seg1 = min(seg_last, (int)blockIdx.y * segs_each + segs_each - 1);
@@ -834,8 +834,6 @@ static int a8_shared(const A8Args& a, hipStream_t st) {
 
 extern "C" {
 
-int vk_attn8_item_rows(void) { return A8_ITEM_ROWS; }
-
 // 32-bit words of scratch for `items` items of up to item_rows <= 16 rows: 0 for more rows, whose keys are not split, and for few keys.
 int64_t vk_attn8_scratch_floats(int items, int item_rows, int nq, int d, int max_k_len) {
   const int64_t nseg = ((int64_t)max_k_len + A8_SEG - 1) / A8_SEG;
@@ -860,8 +858,9 @@ int vk_paged_attention8(elem_t* out, const elem_t* q, const uint8_t* kc, const u
   if (n_items == 0 || T == 0 || S == 0) return 0;
   VK_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)scratch) % 16 == 0, "attention8: rows, cache and scratch have to lie on 16 bytes");
   const int group = nq / nkv, nseg = max(1, (int)(((int64_t)max_k_len + A8_SEG - 1) / A8_SEG));
-  A8Args a{q, out, kc, vc, scales, table, cu_q, k_len, items, nullptr, nullptr, W, T, S, nq, nkv, d, P, 0, pages, group, item_rows, item_rows * group, window, nseg,
-           n_items, max_k_len, scale * 1.4426950408889634f};
+  // A window as long as the keys hides none; as none it takes part in no difference that could pass 32 bits.
+  A8Args a{q, out, kc, vc, scales, table, cu_q, k_len, items, nullptr, nullptr, W, T, S, nq, nkv, d, P, 0, pages, group, item_rows, item_rows * group,
+           window >= max_k_len ? 0 : window, nseg, n_items, max_k_len, scale * 1.4426950408889634f};
   while (1 << a.lp < P) ++a.lp;
   constexpr bool F32 = sizeof(elem_t) == 4;
   if (item_rows > 16) {
@@ -875,34 +874,39 @@ int vk_paged_attention8(elem_t* out, const elem_t* q, const uint8_t* kc, const u
   a.part_ml = scratch + need / (d + 2) * d;
   const int64_t joins = (int64_t)n_items * nkv;
   VK_REQUIRE(joins < (1ll << 31) && nseg <= 65535, "attention8: %d items, %d keys: too many for one launch", n_items, max_k_len);
-  // Column tiles a wave: as many as there are columns, up to what a wave's registers hold beside a tile of the cache; more columns than that go through LDS.
-  const int most = F32 ? (d <= 64 ? 2 : 1) : d <= 64 ? 4 : d <= 128 ? 2 : 1, nt = (a.cols_max + 15) / 16;
+  // Few columns go by tiles in registers, which each wave reads and converts for itself: in bfloat16 for one tile of columns, as with more the conversion is done once for all waves'
+  // tiles in LDS and not once a wave's tile (64 sequences of 4,000 keys, 8 kv heads of 64: 70 us for 32 columns and 100 for 64, in registers 113 and 182; a single sequence of 1,000
+  // keys, which waits for its loads only, takes 16 us and took 13).  In 32 bits the products bound it, and two tiles of columns stay in registers while the cache's fit beside
+  // them, to heads of 64: 22 us against 33 for that one sequence, 237 against 225 for the 64.  The choice is made by what a row's own item is, not by how many there are: a row's
+  // result doesn't depend on its company.
+  const int most = F32 && d <= 64 ? 2 : 1, nt = (a.cols_max + 15) / 16;
   int cols;                                             // of a block
   if (nt <= most) {
     cols = 16 * nt;
-    // Workgroups of several segments where there are more than the card holds at once: what stands in front of a workgroup's first loads is then paid once.
+    // Workgroups of several segments where there are more than the card holds at once: what stands in front of a workgroup's first loads is then paid once (64 rows of 8,192 keys,
+    // calls in a row: 203 us, with a segment each 230; up to 4 or 16 instead of 8 change it by 2 %).
     const int64_t held = (nt == 1 ? 2 : 1) * vk_device_cus();
     const int each = (int)max((int64_t)1, min((int64_t)8, joins * nseg / (2 * held)));
     const dim3 grid((unsigned)joins, (nseg + each - 1) / each);
-#define FEW(D, N) a8_few_kernel<D, N><<<grid, 256, 0, st>>>(a, each, 1)
-    if (d <= 64) {
-      if (nt == 1) FEW(64, 1);
-      else if (nt == 2) FEW(64, 2);
-#ifdef VK_BF16
-      else if (nt == 3) FEW(64, 3);
-      else FEW(64, 4);
-    } else if (d <= 128 && nt == 2) {
-      FEW(128, 2);
+#define FEW(D, N) a8_few_kernel<D, N><<<grid, 256, 0, st>>>(a, each)
+#ifndef VK_BF16
+    if (nt == 2) FEW(64, 2);
+    else
 #endif
-    } else if (d <= 128) FEW(128, 1);
+    if (d <= 64) FEW(64, 1);
+    else if (d <= 128) FEW(128, 1);
     else if (d <= 192) FEW(192, 1);
     else FEW(256, 1);
 #undef FEW
     if (vk_check_launch("attention8")) return 1;
   } else {
-    const bool two = a.cols_max <= 32 && d <= 192;      // two waves; of the largest heads' tiles a wave's share of the loads would not fit its registers
+    // Two waves where they have a tile of columns each (32 columns, 64 sequences of 4,000 keys, heads of 64: 70 us against 81 with four waves; in 32 bits, heads of 128, 497 against
+    // 592); of the largest heads' tiles half would be too many loads for a wave's registers.  Two tiles of columns a wave and half the waves were no faster for 64 columns (97 us
+    // against 99 for heads of 64, 181 against 177 for 128) and slower for one sequence (19 against 16).
+    const bool two = a.cols_max <= 32 && d <= 192;
+    constexpr int SMALL = F32 ? 128 : 64;               // two tiles of columns of heads of 64 are in registers in 32 bits
     cols = two ? 32 : 64;
-    const int bad = two ? (d <= 64 ? a8_shared<64, 1, 2, true>(a, st) : d <= 128 ? a8_shared<128, 1, 2, true>(a, st) : a8_shared<192, 1, 2, true>(a, st))
+    const int bad = two ? (d <= SMALL ? a8_shared<SMALL, 1, 2, true>(a, st) : d <= 128 ? a8_shared<128, 1, 2, true>(a, st) : a8_shared<192, 1, 2, true>(a, st))
                         : (d <= 64 ? a8_shared<64, 1, 4, true>(a, st) : d <= 128 ? a8_shared<128, 1, 4, true>(a, st) : d <= 192 ? a8_shared<192, 1, 4, true>(a, st)
                                                                                                                                : a8_shared<256, 1, 4, true>(a, st));
     if (bad) return 1;

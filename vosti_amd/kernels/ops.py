@@ -458,6 +458,8 @@ class Kernels:
                 raise KernelError(f"qkv_post8: tables {tuple(cos.shape)} do not cover {max_k_len} places")
             half = cos.shape[1]
             cp, sp = self._at(cos, "cos", self.dtype, cos.shape, here), self._at(sin, "sin", self.dtype, cos.shape, here)
+        if not 0 <= max_k_len < 2**31:
+            raise KernelError(f"qkv_post8: up to {max_k_len} keys")
         S, width = block_table.shape
         tp = self._at(block_table, "block table", torch.int32, (S, width), here)
         cup, klp = self._at(cu_q, "cu_q", torch.int32, (S + 1,), here), self._at(k_len, "k_len", torch.int32, (S,), here)
@@ -478,12 +480,19 @@ class Kernels:
         """Attention of the rows named by ``items`` over an 8-bit cache (see attention8.hip).
 
         items [n, 2] = (sequence, first row): an item is up to ``item_rows`` consecutive rows of its sequence, at most ATTN_ITEM_ROWS.  Items of up
-        to 16 rows (decoded tokens, drafted ones) have their keys split over workgroups, whose sums meet in ``scratch`` (``attn8_scratch_floats``;
-        without it the call takes memory of its own); larger ones are for prompts.  ``max_k_len`` is the host's bound on k_len; the block table must
-        cover it, and keys beyond it may be left out.  Rows that no item names are left as they were."""
+        to 16 rows have their keys split over workgroups, whose sums meet in ``scratch`` (``attn8_scratch_floats``; without it the call takes memory of its own);
+        a scratch belongs to one call at a time, in recorded graphs too.  They are for decoded and drafted tokens and for a portion of few sequences (32 heads of 128,
+        one sequence of 8,192 keys: 128 rows in 50 us, as one item in 208); larger items read the cache less often and are for prompts (1,024 rows of that sequence: 209 us
+        against 278; 64 portions of 128 rows with 1,000 keys: 168 against 367).  A row's result depends on ``item_rows`` in its last bits, and not on what else is
+        in the call.  ``max_k_len`` is the host's bound on k_len; the block table must cover it, and keys beyond it may be left out.  Rows that no item
+        names are left as they were."""
         here = self._device()
         if q.dim() != 3 or k_cache.dim() != 4:
             raise KernelError(f"attention8: q {tuple(q.shape)} is not [T, heads, size], or the k cache {tuple(k_cache.shape)} not [pages, kv heads, page size, size]")
+        if not 1 <= item_rows <= ATTN_ITEM_ROWS:
+            raise KernelError(f"attention8: items of {item_rows} rows; from 1 to {ATTN_ITEM_ROWS}")
+        if not 0 <= window < 2**31 or not 0 <= max_k_len < 2**31:
+            raise KernelError(f"attention8: a window of {window}, up to {max_k_len} keys")
         T, nq, d = q.shape
         nkv = k_cache.shape[1]
         S, W = block_table.shape
@@ -507,7 +516,7 @@ class Kernels:
                draw_uniforms: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Which drafted tokens stand against the target's logits, and the token behind them (see verify.hip).
 
-        logits [R, V]: rows cu[s] .. cu[s + 1] - 1 are sequence s's, one more than its drafted tokens; draft_ids [D] are those of all sequences one after
+        logits [R, V]: rows cu[s] .. cu[s + 1] - 1 (cu[0] = 0) are sequence s's, one more than its drafted tokens; draft_ids [D] are those of all sequences one after
         the other.  ``draft_logits`` [D, V]: the draft model's, without them a draft is certain.  ``temps`` [S] for both models (without them, and at 0, the
         maximum alone), with random numbers in [0, 1): ``accept_uniforms`` [D] and ``draw_uniforms`` [S].
 
