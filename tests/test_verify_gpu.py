@@ -51,6 +51,9 @@ CASES = [
     ("f32", [4, 0, 2], 503, True),
     ("f32", [1, 6], 16385, False),
     ("f32", [3, 3], 30001, True),
+    # More pieces of sequences than a few rounds of workgroups: what stands is decided in a launch of its own.
+    ("bf16", [2, 0, 1] * 300, 5000, True),
+    ("f32", [1, 0, 17] + [1] * 300, 16385, False),
 ]
 
 
@@ -70,6 +73,21 @@ def test_tokens_are_the_definitions(case):
             ids = np.array([rng.choice(V, p=chances(host(near[i]) if drawn else host(logits[of[i]]), t[i])) for i in range(D)], dtype=int)
             check(name, logits, ids, cu, near if drawn else None, temps, rng.random(D), rng.random(S))
     check(name, logits, ids, cu, near if drawn else None)
+
+
+def test_a_sequence_is_the_same_in_any_company():
+    """Alone, and among so many that another launch decides."""
+    k, V, S = kernels_for("bf16"), 5000, 900
+    g = torch.Generator().manual_seed(3)
+    logits, near = (torch.randn(n, V, generator=g).mul(2).to(torch.bfloat16).cuda() for n in (3 * S, 2 * S))
+    ids, u, w = torch.randint(0, V, (2 * S,), generator=g, dtype=torch.int32).cuda(), torch.rand(2 * S, generator=g).mul(0.01).cuda(), torch.rand(S, generator=g).cuda()
+    run = lambda a, b: k.verify(logits[3 * a:3 * b], ids[2 * a:2 * b], ints([3 * i for i in range(b - a + 1)]), draft_logits=near[2 * a:2 * b],   # noqa: E731
+                                temps=torch.ones(b - a, device="cuda"), accept_uniforms=u[2 * a:2 * b], draw_uniforms=w[a:b])
+    tokens, counts, accept = run(0, S)
+    assert counts.unique().numel() > 1
+    for s in (0, 1, 63, 64, 500, S - 1):
+        one = run(s, s + 1)
+        assert torch.equal(one[0], tokens[3 * s:3 * s + 3]) and torch.equal(one[1], counts[s:s + 1]) and torch.equal(one[2], accept[2 * s:2 * s + 2])
 
 
 @pytest.mark.parametrize("name", ["bf16", "f32"])

@@ -16,6 +16,11 @@
 //
 // Keys that a row does not see weigh 0, whatever is stored: their scores are never used, and values outside what the wave's rows see, or NaN, are
 // taken out of the second product of a tile that not all rows see whole; a row that does see a NaN gets it back through a product of its own.
+//
+// What bounds it (MI355X, bfloat16, heads of 128, 8 kv heads; reading alone reaches 6.45 TB/s here, a large bfloat16 product 1.45 PFLOP/s): 64 rows with 8,192 keys each, 32 heads, 1.08 GB
+// of cache: 189 us, 5.7 TB/s, and 5 us for the join: bytes.  13 sequences of 5 rows and some 4,000 keys, 64 heads, 73 MB: 26 us and 5: workgroups of eight tiles one after
+// the other, little more than one round of them.  A prompt of 4,096 rows over itself, 32 heads, 137 GFLOP: 163 us in a row of calls, 186 alone, 0.74 to 0.84 PFLOP/s: the vector unit, which
+// turns entries into operands and scores into weights for as long as the products take.  A single row with 333 keys: 10 us, loads that wait for each other.
 #include <type_traits>
 
 #include "cache8.h"
@@ -451,7 +456,8 @@ struct A8Pages {
   __device__ __forceinline__ uint64_t of_any(int lane) const { return (uint64_t)(unsigned)__shfl((int)(at >> 32), lane) << 32 | (unsigned)__shfl((int)at, lane); }
 };
 
-// ---- few columns (decoded and drafted tokens): a workgroup takes segments of 512 keys one after the other, a wave two of a segment's tiles, every fourth, for up to 16 NT columns.
+// ---- few columns (decoded tokens, small groups' drafted ones): a workgroup takes segments of 512 keys one after the other, a wave two of a segment's tiles, every fourth, for up to 16 NT
+// columns.
 // Tiles come straight into registers: a tile's keys are asked for when the last tile's have been multiplied, its values when those have, so that there is something under way at any
 // time and no load waits for another (page numbers and scales are read 64 pages ahead; a page number read in turn would wait for all loads before it).  The waves' sums meet in LDS, the
 // segments' in a8_join_kernel.
@@ -578,7 +584,7 @@ __global__ __launch_bounds__(256, DP <= 128 && NT == 1 ? 2 : 1) void a8_few_kern
   }
 }
 
-// ---- more columns (prompts, several drafted tokens): tiles pass through LDS once for all waves, each of which has 16 NT columns.  SPLIT: a workgroup takes one segment.
+// ---- more columns (prompts, drafted tokens): tiles pass through LDS once for all waves, each of which has 16 NT columns.  SPLIT: a workgroup takes one segment.
 //
 // A tile in LDS: K's row 16 i + r (the key that lane row r reads for tile i) in DP bytes, V's entry in 64; the 16-byte piece p of K's row r lies at p ^ turn(r), of V's entry
 // e at p ^ (e / 4 % 4), so that the 16 lanes that read a piece of 16 rows read 16 different quads of banks.  Pieces come by loads that go to LDS without passing registers: a load

@@ -31,7 +31,7 @@ int vk_sample_static(int32_t* out, const elem_t* logits, const float* temps, con
                      int64_t row_stride, hipStream_t st);
 
 // Drafted tokens against the target's logits (verify.hip).  logits [R, V]: rows cu[s] .. cu[s + 1] - 1 are sequence s's, one more than its drafted tokens,
-// whose ids are ids[cu[s] - s] .. of D; draft_logits [D, V] or null (the drafts are certain); temps [S] or null (0: the maxima); accept_u [D] and draw_u [S]:
+// whose ids follow those of the sequences before it in ids [D]; draft_logits [D, V] or null (the drafts are certain); temps [S] or null (0: the maxima); accept_u [D] and draw_u [S]:
 // random numbers in [0, 1).  tokens [R]: a sequence's standing tokens, the drawn one, then -1; counts [S]: how many they are (0 for a sequence without rows or
 // one that the arrays do not hold); accept [D]: min(1, p / q) of every drafted token.  What lies behind the last sequence is left as it was.  An id outside
 // [0, V) does not stand.  scratch: vk_verify_scratch_bytes bytes of device memory on 16 bytes.

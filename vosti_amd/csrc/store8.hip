@@ -13,6 +13,10 @@
 // A row of the step stands at place k_len - (rows of its sequence) + its number, in page table[sequence][place / P].  A workgroup takes
 // one (page, head, k or v) that the step writes to, so that the scale, the new entries and the old ones are one workgroup's
 // business; rows come to it by their sequence, not by slots.  The other workgroups take a token's q heads each.
+//
+// Measured (MI355X, bfloat16, 32 q and 8 kv heads of 128, pages of 64; a copy reaches 4.75 TB/s here): a prompt of 4,096 tokens, 93 MB: 33.7 us, 2.8 TB/s: a page's rows go through LDS
+// between their maximum and their rounding, and nothing else of the workgroup is under way then.  A token each of 64 sequences, 1.5 MB: 10.4 us: the sequence's lengths, then the page's
+// number, its scale and, where that grows, its entries, one load behind the other.  The 32-bit build, 2,300 tokens of 7 sequences, 16 and 8 heads of 64: 12 us.
 #include "cache8.h"
 #include "vec.h"
 
@@ -364,7 +368,7 @@ int vk_qkv_post8(const elem_t* qkv, int64_t row_stride, elem_t* q_out, uint8_t* 
   const int64_t jobs = nkv > 0 ? min((int64_t)T, (int64_t)T / P + 2 * (int64_t)S) : 0, kv_blocks = jobs * nkv * 2, q_blocks = nq > 0 ? T : 0;
   VK_REQUIRE(kv_blocks + q_blocks < (1ll << 31), "qkv_post8: %d rows of %d heads are too many for one launch", T, nq + 2 * nkv);
   a.kv_blocks = (int)kv_blocks;
-  // Rows that a workgroup holds in LDS: a page's, up to 32 KB, and one where every sequence has one.
+  // Rows that a workgroup holds in LDS: a page's, up to 32 KB (four workgroups a CU, so that some load while others round), and one where every sequence has one.
   a.held = T <= S ? 1 : min(P, 32 * 1024 / 4 / d);
   const int lds_q = a.whole ? 0 : STORE8_TURN * (int)sizeof(float), lds_kv = a.held * d * 4 + (a.whole ? 0 : STORE8_TURN * (int)sizeof(double));
   const int vecs = d / VK_VEC;
