@@ -1,13 +1,15 @@
 """The refusals of the 8-bit cache's and the verification's C entries, which come before any launch, and the 64-bit formulas that the GPU tests compare with."""
 import ctypes
 import math
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
 
 from plain_cache8 import attention, chances, e4m3, e4m3_numbers, exponent_for, store, verify
 from vosti_amd.kernels import build
-from vosti_amd.kernels.ops import Kernels
+from vosti_amd.kernels.ops import ABI_VERSION, Kernels
 
 GOOD = 1 << 20            # an address that nothing looks at
 
@@ -15,6 +17,12 @@ GOOD = 1 << 20            # an address that nothing looks at
 @pytest.fixture(scope="module", params=["bf16", "f32"])
 def kernels(request):
     return Kernels(request.param)
+
+
+def test_both_callers_ask_for_the_librarys_interface(kernels):
+    """The native engine refuses a library of another number than its own, and so does the Python package."""
+    source = (Path(build.__file__).parents[1] / "csrc" / "engine" / "gpu.cpp").read_text()
+    assert kernels.lib.vk_abi_version() == ABI_VERSION == int(re.search(r"KERNEL_ABI = (\d+);", source).group(1))
 
 
 def refused(kernels, fn, *args):

@@ -58,6 +58,8 @@ STORES = [
     ("f32", [90, 0, 31], [95, 0, 64], 4, 4, 96, 32, True, 48),
     ("f32", [21, 300], [21, 300], 2, 2, 256, 128, False, 0),
     ("f32", [5], [300], 2, 1, 16, 256, True, 8),
+    # No more rows than sequences, and yet several of one.
+    ("bf16", [21, 0, 1] + [0] * 25, [50, 7, 3] + [9] * 25, 2, 2, 64, 16, True, 64),
 ]
 
 
@@ -230,6 +232,15 @@ ATTENDS = [
     ("f32", [3], [520], 8, 1, 176, 32, 0, 3),
     ("f32", [2, 5], [30, 513], 10, 1, 256, 64, 0, 5),
     ("f32", [9], [65], 1, 1, 256, 256, 0, 9),
+    # So many sequences that a workgroup takes several segments of one, among them more than 64 pages; the last ones without a key in it.
+    ("bf16", [1] * 300, [1930 - 6 * i for i in range(300)], 4, 4, 16, 16, 0, 1),
+    ("bf16", [2] * 300, [130 + 7 * i for i in range(300)], 8, 4, 16, 32, 300, 2),
+    ("f32", [4] * 90, [1500 - 15 * i for i in range(90)], 32, 4, 32, 16, 0, 4),
+    # Prompts on more than 64 pages.
+    ("bf16", [40], [2500], 4, 1, 64, 16, 0, 128),
+    ("bf16", [140, 20], [1400, 3000], 2, 1, 128, 16, 1500, 128),
+    ("bf16", [30], [4300], 2, 2, 256, 32, 0, 64),
+    ("f32", [20], [1300], 2, 1, 64, 16, 0, 128),
 ]
 
 

@@ -178,7 +178,7 @@ struct Kernels::Fn {
   int (*attn_rel_pad)();
 };
 
-static constexpr int KERNEL_ABI = 20;
+static constexpr int KERNEL_ABI = 21;
 
 Kernels::Kernels(const std::string& lib_dir, const std::string& name) : name_(name), fn_(new Fn) {
   if (name == "bf16") dtype_ = DType::BF16;
