@@ -82,6 +82,18 @@ __device__ __forceinline__ void keys_times(u32x4 raw, float scale, const q_part 
     for (int n = 0; n < NT; ++n) s[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[n][h], s[n], 0, 0, 0);
   }
 }
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+__device__ __forceinline__ i32x8 two_pieces(u32x4 a, u32x4 b) { return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]}; }
+template <int NT>
+__device__ __forceinline__ void keys_times8(u32x4 a, u32x4 b, int k_exp, const q_part (&qa)[NT][A8_QJ], const q_part (&qb)[NT][A8_QJ], const int (&q_exp)[NT], f32x4 (&s)[NT]) {
+  const i32x8 k = two_pieces(a, b);
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      s[n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, two_pieces(__builtin_bit_cast(u32x4, qa[n][h]), __builtin_bit_cast(u32x4, qb[n][h])), s[n], 0, 0, 0, k_exp, 0,
+                                                              q_exp[n] - 5 * h);
+}
 template <int NT>
 __device__ __forceinline__ void values_times(u32x4 raw, float scale, const w_part (&w)[NT][A8_WP], f32x4 (&o)[NT]) {
 #pragma unroll
@@ -184,9 +196,55 @@ __device__ __forceinline__ bool a8_rows(const A8Args& a, int item, int kvh, int 
   return true;
 }
 
-// q of the wave's columns: entries 64 j + 16 g + .. of each.
+// q of the wave's columns: entries 64 j + 16 g + .. of each.  EIGHT: as two 8-bit numbers each, all first ones of the 16, then all second ones, with the exponent (+ 127) of what the first ones of a
+// column stand in.
 template <int DP, int NT>
-__device__ __forceinline__ void a8_load_q(const A8Args& a, const A8Rows<NT>& c, q_part (&q)[DP / 64][NT][A8_QJ]) {
+struct A8Query {
+#ifdef VK_BF16
+  static constexpr bool EIGHT = DP % 128 == 0;
+#else
+  static constexpr bool EIGHT = false;
+#endif
+  q_part q[DP / 64][NT][A8_QJ];
+  int exp[NT];
+};
+#ifdef VK_BF16
+template <int DP, int NT>
+__device__ __forceinline__ void a8_split_q(A8Query<DP, NT>& q) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf((float)q.q[j][n][e / 8][e % 8]));
+    const int e7 = max(exponent_of(over_groups_max(top)), -100) - 7;
+    q.exp[n] = e7 + 127;
+    const float by = pow2f(-e7);
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j) {
+      u32x4 hi, lo;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = (float)q.q[j][n][p / 2][4 * (p & 1) + i] * by;
+          x[i] = fabsf(v) < INFINITY ? v : NAN;
+        }
+        hi[p] = to_fp8x4(x[0], x[1], x[2], x[3]);
+        const f32x2 a = from_fp8x2<false>(hi[p], 1.f), b = from_fp8x2<true>(hi[p], 1.f);
+        lo[p] = to_fp8x4((x[0] - a.x) * 32.f, (x[1] - a.y) * 32.f, (x[2] - b.x) * 32.f, (x[3] - b.y) * 32.f);
+      }
+      q.q[j][n][0] = __builtin_bit_cast(bf16x8, hi);
+      q.q[j][n][1] = __builtin_bit_cast(bf16x8, lo);
+    }
+  }
+}
+#endif
+template <int DP, int NT>
+__device__ __forceinline__ void a8_load_q(const A8Args& a, const A8Rows<NT>& c, A8Query<DP, NT>& to) {
+  q_part (&q)[DP / 64][NT][A8_QJ] = to.q;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int col = c.col0 + 16 * n + c.r, row = min(col, c.cols - 1) / a.group, head = min(col, c.cols - 1) - row * a.group;
@@ -209,9 +267,13 @@ __device__ __forceinline__ void a8_load_q(const A8Args& a, const A8Rows<NT>& c, 
   }
 }
 
-// q has arrived: waited for in front of a loop, so that no wait for it stands inside, where it would be one for all loads under way.
+// q has arrived (and is split): waited for in front of a loop, so that no wait for it stands inside, where it would be one for all loads under way.
 template <int DP, int NT>
-__device__ __forceinline__ void a8_wait_q(q_part (&q)[DP / 64][NT][A8_QJ]) {
+__device__ __forceinline__ void a8_wait_q(A8Query<DP, NT>& to) {
+#ifdef VK_BF16
+  if constexpr (A8Query<DP, NT>::EIGHT) a8_split_q<DP, NT>(to);
+#endif
+  q_part (&q)[DP / 64][NT][A8_QJ] = to.q;
 #pragma unroll
   for (int j = 0; j < DP / 64; ++j)
 #pragma unroll
@@ -260,7 +322,7 @@ struct A8Sums {
 
 // The scores of a tile: S^T's, unscaled.  src.k(i, j): the lane's 16 bytes of K's tile i; k_scale: of the keys that they belong to.
 template <int DP, int NT, typename SRC>
-__device__ __forceinline__ void a8_scores(const SRC& src, float k_scale, const q_part (&q)[DP / 64][NT][A8_QJ], f32x4 (&s)[4][NT]) {
+__device__ __forceinline__ void a8_scores(const SRC& src, float k_scale, const A8Query<DP, NT>& q, f32x4 (&s)[4][NT]) {
   // Where two waves meet on a unit the one in front of its products goes first: they leave the other three of four cycles for its arithmetic (196 -> 186 us for a prompt of 4,096 rows).
   __builtin_amdgcn_s_setprio(1);
   // What a product reads is asked for one product ahead, and not further: the scheduler would take all of a tile first, and spill.
@@ -278,7 +340,15 @@ __device__ __forceinline__ void a8_scores(const SRC& src, float k_scale, const q
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j) keys_times<NT>(k[j], k_scale, q[j], s[i]);
+    for (int j = 0; j < DP / 64; ++j) {
+#ifdef VK_BF16
+      if constexpr (A8Query<DP, NT>::EIGHT) {
+        if (j % 2 == 0) keys_times8<NT>(k[j], k[j + 1], (int)(__builtin_bit_cast(uint32_t, k_scale) >> 23), q.q[j], q.q[j + 1], q.exp, s[i]);
+        continue;
+      }
+#endif
+      keys_times<NT>(k[j], k_scale, q.q[j], s[i]);
+    }
     asm volatile("" ::: "memory");
   }
   __builtin_amdgcn_s_setprio(0);
@@ -494,7 +564,7 @@ __global__ __launch_bounds__(256, DP <= 128 && NT == 1 ? 2 : 1) void a8_few_kern
   const int seg0 = max(seg_first, (int)blockIdx.y * segs_each), seg1 = min(seg_last, (int)blockIdx.y * segs_each + segs_each - 1);
   if (seg0 > seg1) return;
   const int kb0 = seg0 * A8_SEG + wave * A8_TILE, pos = min(c.wave_pos, seg1 * A8_SEG + A8_SEG - 1);
-  q_part q[DP / 64][NT][A8_QJ];
+  A8Query<DP, NT> q;
   a8_load_q<DP, NT>(a, c, q);
   A8Pages pages;
   pages.fill(a, c, seg0 * A8_SEG >> a.lp, pos);
@@ -688,7 +758,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
     c.seq = all.seq;
     c.kvh = kvh;
   }
-  q_part q[DP / 64][NT][A8_QJ];
+  A8Query<DP, NT> q;
   if (mine) a8_load_q<DP, NT>(a, c, q);
   A8Sums<DP, NT> o;
   o.clear();
