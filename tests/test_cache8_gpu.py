@@ -385,6 +385,35 @@ def test_scales_before_the_window_do_not_matter():
         assert torch.equal(want, attend(k, q, (kc, vc, scales), table, rows, keys, most, window))
 
 
+@pytest.mark.parametrize("d", (64, 128, 256))
+@pytest.mark.parametrize("rows", (1, 5, 20))
+def test_heads_of_small_and_large_entries(d, rows):
+    """q whose entries lie far apart, the largest against keys that are 0 there.  Heads of 128 and 256 are held by two numbers of four digits: entries below 2^-14 of the largest's power of two are off by
+    up to 2^-22 of it, which moves a score by that times the sum of |k|, and a result by twice that (numerator and denominator) of the mean of |v - out|, at most that of |v| and |out|."""
+    k, P, nq, nkv, keys = kernels_for("bf16"), 64, 4, 2, 150
+    rng = np.random.default_rng(d + rows)
+    table, pages = tables(rng, [keys], P)
+    kc, vc, scales = filled(rng, pages, nkv, P, d, -9, -6)
+    kc[..., 3] = 0
+    q = rng.standard_normal((rows, nq, d)) * 2.0 ** rng.integers(-16, 2, (rows, nq, d))
+    for at, size in enumerate((2.0 ** 9, 2.0 ** 14, 2.0 ** 40, 0.0)):
+        q[:, at, 3] = size
+    q = torch.from_numpy(q).to(torch.bfloat16).cuda()
+    got = host(attend(k, q, (kc, vc, scales), table, [rows], [keys], 16 if rows < 16 else 128))
+    out, weighted, most, flushed = attention(host(q), *map(host, (kc, vc, scales)), table, [0, rows], [keys], d ** -0.5)
+    power = 2.0 ** np.floor(np.log2(np.abs(host(q)).max(-1, keepdims=True)))
+    size = (np.abs(host(kc)).sum(-1) * host(scales)[:, :, None, 0]).max() * d ** -0.5
+    moved = 2.0 ** -22 * power * size + 2 * (d + 16) * 2.0 ** -24 * most + 2.0 ** -20
+    bound = 2.0 ** -8 * 1.01 * np.abs(out) + (weighted + np.abs(out)) * (2.0 ** -11 + 2 * moved) + 2.0 ** -25 * flushed + 1e-30
+    assert (np.abs(got - out) <= bound)[:, [0, 1, 3]].all()
+    assert np.isfinite(got[:, 2]).all() and np.abs(got[:, 2]).max() <= np.abs(host(vc) * host(scales)[:, :, 1, None, None]).max() * 1.01
+    q[0, 1, d - 1] = float("nan")
+    more = host(attend(k, q, (kc, vc, scales), table, [rows], [keys], 16 if rows < 16 else 128))
+    assert np.isnan(more[0, 1]).all()
+    more[0, 1] = got[0, 1]
+    assert np.array_equal(more, got)
+
+
 @pytest.mark.parametrize("most", (16, 128))
 def test_a_window_longer_than_the_keys_hides_none(most):
     """Among rows that stand before the first key, where a window's begin could leave 32 bits."""

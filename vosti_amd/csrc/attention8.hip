@@ -8,7 +8,10 @@
 // 16 (r / 4) + 4 t + r % 4 for t = 0..3, of V the keys 16 g .. 16 g + 15 of entry 16 dt + r.  K's rows are taken in that order so that the scores that a lane ends with
 // (rows 4 g + i of S^T's tile t) are those of the keys 16 g + 4 t + i: the lane's own 16 keys of V, and no weight has to change lanes between the products.
 //
-// Arithmetic.  A key's entry times its scale is exact in the element type, so the first product takes q as it is and 32-bit sums.  Weights are at most 1 (2^8
+// Arithmetic.  A key's entry times its scale is exact in the element type, so the first product takes q as it is and 32-bit sums.  For heads of 128 and 256 it takes the keys as they are
+// stored, and q as two e4m3 numbers of four digits each in units of the head's largest entry: they hold its eight digits where it is 2^-14 of the largest's power of two or more, and are off by
+// 2^-22 of that power at most elsewhere; products of twice the rate make up for there being two, and no key has to be turned into an operand (a prompt of 4,096 rows 186 -> 163 us; of heads of 64 the
+// product, 128 entries long, would be half empty).  Weights are at most 1 (2^8
 // where a reference maximum is kept) and go into the second product in 16-bit floating point with eleven digits, against values without their scale, which
 // they hold to the bit: bfloat16 weights, with eight, would double the squared error of the result.  Values' scales that differ within a product stand in its
 // entries relative to the largest of them.  The 32-bit build takes everything in 32 bits.  The sum of the weights comes from the matrix
@@ -18,9 +21,9 @@
 // taken out of the second product of a tile that not all rows see whole; a row that does see a NaN gets it back through a product of its own.
 //
 // What bounds it (MI355X, bfloat16, heads of 128, 8 kv heads; reading alone reaches 6.45 TB/s here, a large bfloat16 product 1.45 PFLOP/s): 64 rows with 8,192 keys each, 32 heads, 1.08 GB
-// of cache: 189 us, 5.7 TB/s, and 5 us for the join: bytes.  13 sequences of 5 rows and some 4,000 keys, 64 heads, 73 MB: 26 us and 5: workgroups of eight tiles one after
-// the other, little more than one round of them.  A prompt of 4,096 rows over itself, 32 heads, 137 GFLOP: 163 us in a row of calls, 186 alone, 0.74 to 0.84 PFLOP/s: the vector unit, which
-// turns entries into operands and scores into weights for as long as the products take.  A single row with 333 keys: 10 us, loads that wait for each other.
+// of cache: 189 us, 5.7 TB/s, and 5 us for the join: bytes.  13 sequences of 5 rows and some 4,000 keys, 64 heads, 73 MB: 24 us and 5: workgroups of eight tiles one after
+// the other, little more than one round of them.  A prompt of 4,096 rows over itself, 32 heads, 137 GFLOP: 157 us, 0.87 PFLOP/s: a wave's products
+// and the exponentials behind them follow each other, and its registers leave room for two waves a unit.  A single row with 333 keys: 10 us, loads that wait for each other.
 #include <type_traits>
 
 #include "cache8.h"
@@ -323,8 +326,6 @@ struct A8Sums {
 // The scores of a tile: S^T's, unscaled.  src.k(i, j): the lane's 16 bytes of K's tile i; k_scale: of the keys that they belong to.
 template <int DP, int NT, typename SRC>
 __device__ __forceinline__ void a8_scores(const SRC& src, float k_scale, const A8Query<DP, NT>& q, f32x4 (&s)[4][NT]) {
-  // Where two waves meet on a unit the one in front of its products goes first: they leave the other three of four cycles for its arithmetic (196 -> 186 us for a prompt of 4,096 rows).
-  __builtin_amdgcn_s_setprio(1);
   // What a product reads is asked for one product ahead, and not further: the scheduler would take all of a tile first, and spill.
   u32x4 next[DP / 64];
 #pragma unroll
@@ -351,7 +352,6 @@ __device__ __forceinline__ void a8_scores(const SRC& src, float k_scale, const A
     }
     asm volatile("" ::: "memory");
   }
-  __builtin_amdgcn_s_setprio(0);
 }
 
 // A tile's scores and values onto the wave's sums.  src.v(dt): the lane's 16 bytes of V's entries 16 dt + r; v_exp: of the 16 keys that they belong to, -256: none of them is there;
@@ -360,7 +360,7 @@ __device__ __forceinline__ void a8_scores(const SRC& src, float k_scale, const A
 // A column's reference maximum follows its maximum only where that is more than 2^8 above: weights are 2^8 at most then (their sums are 32-bit, and 2^8 is nothing to
 // sixteen bits), and the sums are scaled in few tiles.  Which columns move is each column's own business; whether any does is the wave's.
 // WHOLE: 1: every column that stands for a row sees every key; 0: not so; 2: unknown, and found out for the values.  (What is only done under a condition must not touch scores and sums:
-// where the ways meet again they would be copied, and held twice.  A loop for each kind of tile in place of a condition: 225 -> 196 us for that prompt.)
+// where the ways meet again they would be copied, and held twice.  A loop for each kind of tile in place of a condition: 225 -> 196 us for a prompt of 4,096 rows.)
 template <int WHOLE, int DP, int NT, typename SRC>
 __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, int kb, const SRC& src, f32x4 (&s)[4][NT], int v_exp, int top_exp, A8Sums<DP, NT>& o) {
   const bool there = v_exp > -256;
@@ -419,6 +419,8 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
     for (int x = 0; x < 16; ++x) p[x] = exp2_fast(__builtin_fmaf(s[x / 4][n][x % 4], a.scale_log2, -o.m[n]));
     set_weights(p, w[n]);
   }
+  // Where two waves meet on a unit the one in front of these products goes first: they leave most cycles for the other's arithmetic (179 -> 161 us for a prompt of
+  // 4,096 rows; 165 with the scores' products too).
   __builtin_amdgcn_s_setprio(1);
   ones_times<NT>(w, o.l);
   // Values that no column sees are taken out; so are NaN, which some may not see: those that do get it back through a product of ones.
@@ -503,7 +505,7 @@ struct A8Pages {
   uint64_t at;               // where its block of the kv head begins, in keys and in values alike (the first page's, for a page that is none)
   float k_scale;
   int v_exp;
-  uint64_t good;             // which of them there are
+  bool clean;                // all of them that hold keys up to the last one are there
   template <int NT>
   __device__ __forceinline__ void fill(const A8Args& a, const A8Rows<NT>& c, int first, int pos) {
     base = first;
@@ -515,7 +517,7 @@ struct A8Pages {
     unsigned lo = (unsigned)(block * a.P * a.d), hi = (unsigned)((uint64_t)(block * a.P * a.d) >> 32);
     k_scale = there ? ks : 1.f;
     v_exp = there ? exponent_of(vs) : -256;
-    good = __ballot(there);
+    clean = __ballot(i <= pos >> a.lp && !there) == 0;
     // Waited for here: a wait where they are used would be one for every load that is under way there.
     asm volatile("" : "+v"(lo), "+v"(hi), "+v"(k_scale), "+v"(v_exp));
     at = (uint64_t)hi << 32 | lo;
@@ -698,14 +700,14 @@ struct A8Offsets {
   }
 };
 
-template <int DP, int WAVES>
-__device__ __forceinline__ void a8_ask(const A8Args& a, const A8Pages& pg, const A8Offsets<DP, WAVES>& off, int wave, int kb, unsigned lds) {
+// Asks for a tile, whose first page is the wave's lane `first` of pg and whose first key stands at `within` of it.  WIDE: a tile lies in one page.
+template <bool WIDE, int DP, int WAVES>
+__device__ __forceinline__ void a8_ask(const A8Args& a, const A8Pages& pg, const A8Offsets<DP, WAVES>& off, int first, int within, unsigned lds) {
   typedef A8Stage<DP, WAVES> ST;
-  const int first = (kb >> a.lp) - pg.base;
-  const unsigned to = __builtin_amdgcn_readfirstlane(lds + wave * 1024);
-  if (a.P >= A8_TILE) {
+  const unsigned to = __builtin_amdgcn_readfirstlane(lds);
+  if (WIDE) {
     const uint64_t at = pg.of_lane(first);
-    const uint8_t *kp = a8_scalar(a.kc + at + (kb & (a.P - 1)) * a.d), *vp = a8_scalar(a.vc + at + (kb & (a.P - 1)));
+    const uint8_t *kp = a8_scalar(a.kc + at + within * a.d), *vp = a8_scalar(a.vc + at + within);
 #pragma unroll
     for (int i = 0; i < ST::LOADS; ++i) pipe_load_to_lds16_sv(kp, off.k[i], to + i * WAVES * 1024);
 #pragma unroll
@@ -729,7 +731,7 @@ struct A8Shared {
   __device__ __forceinline__ u32x4 v(int dt) const { return *reinterpret_cast<const u32x4*>(tile + A8_TILE * DP + (16 * dt + r) * 64 + ((g ^ (r >> 2)) << 4)); }
 };
 
-template <int DP, int NT, int WAVES, bool SPLIT>
+template <int DP, int NT, int WAVES, bool SPLIT, bool WIDE>
 __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kernel(A8Args a, int blocks) {
   typedef A8Stage<DP, WAVES> ST;
   extern __shared__ __attribute__((aligned(1024))) uint8_t stages[];      // A8_STAGES tiles
@@ -769,23 +771,30 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
   A8Pages ahead, now;                                                     // of the tiles that are asked for, of those that are computed
   A8Offsets<DP, WAVES> off;
   off.set(a, wave, threadIdx.x & 63);
-  if (tiles > 0) ahead.fill(a, c, lo >> a.lp, pos);
-  now = ahead;
+  // Tiles from which on the 64 pages that were read are used up.
+  int ahead_end = 0, now_end = 0;
+  auto fill = [&](A8Pages& pages, int& end, int i) {
+    const int kb = lo + i * A8_TILE;
+    pages.fill(a, c, kb >> a.lp, pos);
+    end = __builtin_amdgcn_readfirstlane(i + (((64 << a.lp) - (kb & (a.P - 1))) >> 6));
+  };
+  if (tiles > 0) {
+    fill(ahead, ahead_end, 0);
+    now = ahead;
+    now_end = ahead_end;
+  }
+  // Stages in bytes: of the tile that is computed, of the one that is asked for.
+  unsigned stage = 0, stage_to = 0;
+  auto turned = [](unsigned at) { return at + ST::BYTES == A8_STAGES * ST::BYTES ? 0u : at + ST::BYTES; };
   auto ask = [&](int tile) {
     const int i = __builtin_amdgcn_readfirstlane(tile), kb = lo + i * A8_TILE;
-    if ((kb >> a.lp) - ahead.base >= 64) ahead.fill(a, c, kb >> a.lp, pos);
-    a8_ask<DP, WAVES>(a, ahead, off, wave, kb, lds + (unsigned)(i % A8_STAGES) * ST::BYTES);
+    if (i >= ahead_end) fill(ahead, ahead_end, i);
+    a8_ask<WIDE, DP, WAVES>(a, ahead, off, (kb >> a.lp) - ahead.base, kb & (a.P - 1), lds + wave * 1024 + stage_to);
+    stage_to = turned(stage_to);
   };
-  if (tiles > 0) ask(0);
-  if (tiles > 1) ask(1);
-  // Whether all of the wave's rows see all of tile i.
-  auto whole = [&](int tile) {
-    const int kb = lo + __builtin_amdgcn_readfirstlane(tile) * A8_TILE;
-    if (!mine || kb < c.all_lo || kb + A8_TILE - 1 > c.all_pos) return false;
-    if ((kb >> a.lp) - now.base >= 64) now.fill(a, c, kb >> a.lp, pos);
-    const uint64_t pages = a.P >= A8_TILE ? 1 : (1ull << (A8_TILE >> a.lp)) - 1;
-    return __builtin_amdgcn_readfirstlane((int)((now.good >> ((kb >> a.lp) - now.base) & pages) == pages)) != 0;
-  };
+  for (int i = 0; i < min(tiles, A8_STAGES - 1); ++i) ask(i);
+  // Tiles that all of the wave's rows see whole, where no page is missing.
+  const int whole0 = mine ? (max(c.all_lo - lo, 0) + A8_TILE - 1) >> 6 : 0, whole1 = mine ? min(tiles, (c.all_pos + 1 - lo) >> 6) : 0;
   auto step = [&](int tile, auto all_see) {
     const int i = __builtin_amdgcn_readfirstlane(tile), kb = lo + i * A8_TILE;
     // Tile i has arrived (at most the next one's loads are under way), this wave has what it read of tile i - 1; behind the barrier that holds for all.
@@ -795,12 +804,14 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (i + 2 < tiles) ask(i + 2);
+    const A8Shared<DP, WAVES> src{stages + stage, c.r, c.g};
+    stage = turned(stage);
     if (!all_see.value && (!mine || kb > c.wave_pos || kb + A8_TILE <= c.wave_lo)) return;
-    if ((kb >> a.lp) - now.base >= 64) now.fill(a, c, kb >> a.lp, pos);
+    if (i >= now_end) fill(now, now_end, i);
     const int key = kb + 16 * c.g;
     float k_scale;
     int v_exp, top_exp;
-    if (a.P >= A8_TILE) {
+    if (WIDE) {
       const int l = (kb >> a.lp) - now.base;
       k_scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.k_scale), l));
       v_exp = top_exp = __builtin_amdgcn_readlane(now.v_exp, l);
@@ -811,14 +822,13 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
       top_exp = __builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp));
     }
     if (!all_see.value) v_exp = key <= c.wave_pos && key + 15 >= c.wave_lo ? v_exp : -256;
-    const A8Shared<DP, WAVES> src{stages + (i % A8_STAGES) * ST::BYTES, c.r, c.g};
     f32x4 s[4][NT];
     a8_scores<DP, NT>(src, k_scale, q, s);
     a8_weigh<all_see.value, DP, NT>(a, c, kb, src, s, v_exp, top_exp, o);
   };
   for (int i = 0; i < tiles;) {
-    for (; i < tiles && !whole(i); ++i) step(i, std::integral_constant<int, 0>());
-    for (; i < tiles && whole(i); ++i) step(i, std::integral_constant<int, 1>());
+    for (; i < tiles && !(i >= whole0 && i < whole1 && i < now_end && now.clean); ++i) step(i, std::integral_constant<int, 0>());
+    for (; i < whole1 && i < now_end && now.clean; ++i) step(i, std::integral_constant<int, 1>());
   }
   if (!mine) return;
 #pragma unroll
@@ -897,15 +907,21 @@ __global__ __launch_bounds__(256) void a8_join_kernel(A8Args a, int cols) {
     }
 }
 
-template <int DP, int NT, int WAVES, bool SPLIT>
-static int a8_shared(const A8Args& a, hipStream_t st) {
+template <int DP, int NT, int WAVES, bool SPLIT, bool WIDE>
+static int a8_shared_as(const A8Args& a, hipStream_t st) {
   const int blocks = (a.cols_max + 16 * NT * WAVES - 1) / (16 * NT * WAVES);
   const int64_t units = (int64_t)a.n_items * a.nkv * blocks * (SPLIT ? a.nseg : 1);
   VK_REQUIRE(units < (1ll << 31), "attention8: %d items of %d rows, %d heads: too many for one launch", a.n_items, a.item_rows, a.nq);
   const int lds = A8_STAGES * A8Stage<DP, WAVES>::BYTES;
-  if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)a8_shared_kernel<DP, NT, WAVES, SPLIT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  a8_shared_kernel<DP, NT, WAVES, SPLIT><<<(unsigned)units, 64 * WAVES, lds, st>>>(a, blocks);
+  if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)a8_shared_kernel<DP, NT, WAVES, SPLIT, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  a8_shared_kernel<DP, NT, WAVES, SPLIT, WIDE><<<(unsigned)units, 64 * WAVES, lds, st>>>(a, blocks);
   return vk_check_launch("attention8");
+}
+template <int DP, int NT, int WAVES, bool SPLIT>
+static int a8_shared(const A8Args& a, hipStream_t st) {
+  // Tiles of one page in kernels of their own: what is the same for a wave stays in scalar registers, and the loop has no branch (2,048 rows of heads of 64 over themselves 49 -> 44 us, 4,096 of 128
+  // 161 -> 157).
+  return a.P >= A8_TILE ? a8_shared_as<DP, NT, WAVES, SPLIT, true>(a, st) : a8_shared_as<DP, NT, WAVES, SPLIT, false>(a, st);
 }
 
 extern "C" {
