@@ -21,8 +21,8 @@
 // taken out of the second product of a tile that not all rows see whole; a row that does see a NaN gets it back through a product of its own.
 //
 // What bounds it (MI355X, bfloat16, heads of 128, 8 kv heads; reading alone reaches 6.45 TB/s here, a large bfloat16 product 1.45 PFLOP/s): 64 rows with 8,192 keys each, 32 heads, 1.08 GB
-// of cache: 189 us, 5.7 TB/s, and 5 us for the join: bytes.  13 sequences of 5 rows and some 4,000 keys, 64 heads, 73 MB: 24 us and 5: workgroups of eight tiles one after
-// the other, little more than one round of them.  A prompt of 4,096 rows over itself, 32 heads, 137 GFLOP: 157 us, 0.87 PFLOP/s: a wave's products
+// of cache: 187 us, 5.75 TB/s, and 5 us for the join: bytes.  13 sequences of 5 rows and some 4,000 keys, 64 heads, 73 MB: 26 us and 5: workgroups of eight tiles one after
+// the other, little more than one round of them.  A prompt of 4,096 rows over itself, 32 heads, 137 GFLOP: 154 us, 137 in a row of calls, 0.89 to 1.0 PFLOP/s: a wave's products
 // and the exponentials behind them follow each other, and its registers leave room for two waves a unit.  A single row with 333 keys: 10 us, loads that wait for each other.
 #include <type_traits>
 
@@ -35,7 +35,8 @@
 #define A8_SEG 512               // keys that are summed up apart where a row's keys are split over workgroups
 #define A8_STEP 8.0f             // a column's reference maximum moves where the tile's exceeds it by more (log2)
 #define A8_NONE -3.0e38f          // the reference maximum of a column that has seen no key: finite, so that differences with it are numbers
-#define A8_STAGES 3              // tiles in LDS: one is computed, the next has arrived or is arriving, one is being asked for
+#define A8_STAGES 2               // tiles in LDS: one is computed, the next is arriving.  A third changed nothing for prompts (155 us for 4,096 rows both ways) and keeps workgroups of split keys from
+                                  // the CU (5 rows each, 32 heads of 128, 32 sequences of 4,000 keys: 79 us against 72; 13 of 4,096 43 against 36; of unequal lengths 52 against 50)
 #define A8_ITEM_ROWS 128         // rows of an item, at most
 
 struct A8Args {
@@ -783,29 +784,25 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
     now = ahead;
     now_end = ahead_end;
   }
-  // Stages in bytes: of the tile that is computed, of the one that is asked for.
-  unsigned stage = 0, stage_to = 0;
-  auto turned = [](unsigned at) { return at + ST::BYTES == A8_STAGES * ST::BYTES ? 0u : at + ST::BYTES; };
+  unsigned stage = 0;                                   // of the tile that is asked for, in bytes
   auto ask = [&](int tile) {
     const int i = __builtin_amdgcn_readfirstlane(tile), kb = lo + i * A8_TILE;
     if (i >= ahead_end) fill(ahead, ahead_end, i);
-    a8_ask<WIDE, DP, WAVES>(a, ahead, off, (kb >> a.lp) - ahead.base, kb & (a.P - 1), lds + wave * 1024 + stage_to);
-    stage_to = turned(stage_to);
+    a8_ask<WIDE, DP, WAVES>(a, ahead, off, (kb >> a.lp) - ahead.base, kb & (a.P - 1), lds + wave * 1024 + stage);
+    stage ^= ST::BYTES;
   };
-  for (int i = 0; i < min(tiles, A8_STAGES - 1); ++i) ask(i);
+  if (tiles > 0) ask(0);
   // Tiles that all of the wave's rows see whole, where no page is missing.
   const int whole0 = mine ? (max(c.all_lo - lo, 0) + A8_TILE - 1) >> 6 : 0, whole1 = mine ? min(tiles, (c.all_pos + 1 - lo) >> 6) : 0;
   auto step = [&](int tile, auto all_see) {
     const int i = __builtin_amdgcn_readfirstlane(tile), kb = lo + i * A8_TILE;
-    // Tile i has arrived (at most the next one's loads are under way), this wave has what it read of tile i - 1; behind the barrier that holds for all.
+    // Tile i has arrived, this wave has what it read of tile i - 1; behind the barrier that holds for all.
     asm volatile("" ::: "memory");
-    if (i + 1 < tiles) __builtin_amdgcn_s_waitcnt(0x0070 | (2 * ST::LOADS & 0xF) | ((2 * ST::LOADS >> 4) << 14));
-    else __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_waitcnt(0x0070);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (i + 2 < tiles) ask(i + 2);
-    const A8Shared<DP, WAVES> src{stages + stage, c.r, c.g};
-    stage = turned(stage);
+    const A8Shared<DP, WAVES> src{stages + (stage ^ ST::BYTES), c.r, c.g};
+    if (i + 1 < tiles) ask(i + 1);
     if (!all_see.value && (!mine || kb > c.wave_pos || kb + A8_TILE <= c.wave_lo)) return;
     if (i >= now_end) fill(now, now_end, i);
     const int key = kb + 16 * c.g;
