@@ -966,7 +966,7 @@ int vk_paged_attention8(elem_t* out, const elem_t* q, const uint8_t* kc, const u
   // Few columns go by tiles in registers, which each wave reads and converts for itself: in bfloat16 for one tile of columns, as with more the conversion is done once for all waves'
   // tiles in LDS and not once a wave's tile (64 sequences of 4,000 keys, 8 kv heads of 64: 70 us for 32 columns and 100 for 64, in registers 113 and 182; a single sequence of 1,000
   // keys, which waits for its loads only, takes 16 us and took 13).  In 32 bits the products bound it, and two tiles of columns stay in registers while the cache's fit beside
-  // them, to heads of 64: 22 us against 33 for that one sequence, 237 against 225 for the 64.  The choice is made by what a row's own item is, not by how many there are: a row's
+  // them, to heads of 64: 21 us against 31 for one sequence of 4,000 keys, 39 against 51 for 8, 242 against 192 for 64.  The choice is made by what a row's own item is, not by how many there are: a row's
   // result doesn't depend on its company.
   const int most = F32 && d <= 64 ? 2 : 1, nt = (a.cols_max + 15) / 16;
   int cols;                                             // of a block

@@ -55,52 +55,72 @@ __device__ __forceinline__ double head_sum(double v) {
 __device__ __forceinline__ float one_over_root(float v) { return rsqrtf(v); }
 __device__ __forceinline__ double one_over_root(double v) { return rsqrt(v); }
 
-// What a lane reads for its VK_VEC entries of a head from entry c0 on, whatever the head: the norm's weights and the angles' cosines and sines.  Entry c turns with
-// entry c + h, c < h, and c - h, c < 2 h; others stand, with cosine 1 and sine 0.
-struct Turn {
-  float w[VK_VEC], cs[VK_VEC], sn[VK_VEC];
-};
-__device__ __forceinline__ void read_weights(const Store8Args& a, const void* w, int c0, Turn& t) {
+// Sixteen bytes of elements, as they are read; element e of them.
+__device__ __forceinline__ u32x4 read_raw(const elem_t* p, bool aligned) {
+  if (aligned) return *reinterpret_cast<const u32x4*>(p);
+  u32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+#ifdef VK_BF16
+    r[e] = (uint32_t)__builtin_bit_cast(uint16_t, p[2 * e]) | (uint32_t)__builtin_bit_cast(uint16_t, p[2 * e + 1]) << 16;
+#else
+    r[e] = __builtin_bit_cast(uint32_t, p[e]);
+#endif
+  }
+  return r;
+}
+__device__ __forceinline__ float element(u32x4 r, int e) {
+#ifdef VK_BF16
+  return __builtin_bit_cast(float, (e & 1) ? r[e / 2] & 0xffff0000u : r[e / 2] << 16);
+#else
+  return __builtin_bit_cast(float, (uint32_t)r[e]);
+#endif
+}
+
+// The norm's weights of a lane's VK_VEC entries of a head, from entry c0 on.
+__device__ __forceinline__ void read_weights(const Store8Args& a, const void* w, int c0, float (&to)[VK_VEC]) {
   const int at = min(c0, a.d - VK_VEC);                 // lanes behind the head have nothing to multiply
   if (a.whole && !a.w_is_f32) {
-    load_elems(static_cast<const elem_t*>(w) + at, t.w);
+    load_elems(static_cast<const elem_t*>(w) + at, to);
   } else {
 #pragma unroll
-    for (int e = 0; e < VK_VEC; ++e) t.w[e] = load_weight(w, a.w_is_f32, at + e);
+    for (int e = 0; e < VK_VEC; ++e) to[e] = load_weight(w, a.w_is_f32, at + e);
   }
 }
-__device__ __forceinline__ void read_angles(const Store8Args& a, int c0, int place, Turn& t) {
+// The cosines and sines that they turn by.  Entry c turns with entry c + h, c < h, and c - h, c < 2 h; others stand.
+struct Angles {
+  u32x4 cs, sn;
+};
+__device__ __forceinline__ void read_angles(const Store8Args& a, int c0, int place, Angles& t) {
   const int h = a.rot_half;
   const elem_t *cs = a.cos_t + (int64_t)place * h, *sn = a.sin_t + (int64_t)place * h;
   if (a.whole) {
     const int at = c0 < h ? c0 : c0 < 2 * h ? c0 - h : 0;
-    load_elems(cs + at, t.cs);
-    load_elems(sn + at, t.sn);
+    t.cs = read_raw(cs + at, true);
+    t.sn = read_raw(sn + at, true);
   } else {
+    elem_t c_of[VK_VEC], s_of[VK_VEC];
 #pragma unroll
     for (int e = 0; e < VK_VEC; ++e) {
       const int c = c0 + e, at = c < h ? c : c < 2 * h ? c - h : 0;
-      t.cs[e] = to_f32(cs[at]);
-      t.sn[e] = to_f32(sn[at]);
+      c_of[e] = cs[at];
+      s_of[e] = sn[at];
     }
-  }
-#pragma unroll
-  for (int e = 0; e < VK_VEC; ++e) {
-    t.cs[e] = c0 + e < 2 * h ? t.cs[e] : 1.f;
-    t.sn[e] = c0 + e < h ? -t.sn[e] : c0 + e < 2 * h ? t.sn[e] : 0.f;
+    t.cs = read_raw(c_of, false);
+    t.sn = read_raw(s_of, false);
   }
 }
 
 // Norm and turn of a lane's entries.  y: the head's own LPH * VK_VEC numbers of LDS, for rotations that are no whole vectors.
 template <int LPH, typename F>
-__device__ __forceinline__ void norm_and_turn(F (&v)[VK_VEC], const Store8Args& a, bool norm, const Turn& t, int c0, F* y) {
+__device__ __forceinline__ void norm_and_turn(F (&v)[VK_VEC], const Store8Args& a, bool norm, const float (&w)[VK_VEC], const Angles& t, int c0, F* y) {
   if (norm) {
     F part = 0;
 #pragma unroll
     for (int e = 0; e < VK_VEC; ++e) part = part + v[e] * v[e];
     const F r = one_over_root(head_sum<LPH>(part) * (F)a.per_d + (F)a.eps);
 #pragma unroll
-    for (int e = 0; e < VK_VEC; ++e) v[e] = v[e] * r * (F)t.w[e];
+    for (int e = 0; e < VK_VEC; ++e) v[e] = v[e] * r * (F)w[e];
   }
   if (a.cos_t != nullptr) {
     const int h = a.rot_half;
@@ -120,7 +140,11 @@ __device__ __forceinline__ void norm_and_turn(F (&v)[VK_VEC], const Store8Args& 
       __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
-    for (int e = 0; e < VK_VEC; ++e) v[e] = v[e] * (F)t.cs[e] + other[e] * (F)t.sn[e];
+    for (int e = 0; e < VK_VEC; ++e) {
+      const int c = c0 + e;
+      const float cs = c < 2 * h ? element(t.cs, e) : 1.f, sn = c < h ? -element(t.sn, e) : c < 2 * h ? element(t.sn, e) : 0.f;
+      v[e] = v[e] * (F)cs + other[e] * (F)sn;
+    }
   }
 }
 
@@ -133,6 +157,13 @@ __device__ __forceinline__ int rows_of(const Store8Args& a, int i, int& first, i
   const int end = a.cu_q[i + 1];
   return first >= 0 && first < end && end <= a.T && end - first <= keys && keys <= a.max_k_len ? end - first : 0;
 }
+
+// A number between its maximum and its rounding to four digits: the first eight of them, the last one set where more were lost, so that it is rounded, and compared with 448 of a scale, as it was.
+__device__ __forceinline__ uint32_t held_of(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  return u >> 16 | ((u & 0xffffu) != 0 ? 1u : 0u);
+}
+__device__ __forceinline__ float number_of(uint32_t held) { return __builtin_bit_cast(float, held << 16); }
 
 // LDS of a workgroup: each wave's heads while they turn, and the new entries of a page, `held` rows of d numbers, between their maximum and their rounding.
 constexpr int STORE8_TURN = 4 * 64 * VK_VEC;
@@ -150,15 +181,15 @@ __global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a)
     const int tok = block - a.kv_blocks;
     const elem_t* row = a.qkv + (int64_t)tok * a.row_stride + c0;
     float* y = reinterpret_cast<float*>(lds) + (wave * HPW + sub) * LPH * VK_VEC;
-    float next[VK_VEC];
+    u32x4 next;
     auto ask = [&](int h) {
-#pragma unroll
-      for (int e = 0; e < VK_VEC; ++e) next[e] = 0.f;
-      if (h + sub < a.nq && inside) load_elems(row + (h + sub) * d, next);
+      next = u32x4{0, 0, 0, 0};
+      if (h + sub < a.nq && inside) next = read_raw(row + (h + sub) * d, true);
     };
     ask(wave * HPW);
-    Turn t;
-    if (a.q_w != nullptr) read_weights(a, a.q_w, c0, t);
+    float w[VK_VEC];
+    Angles t;
+    if (a.q_w != nullptr) read_weights(a, a.q_w, c0, w);
     int place = -1;
     for (int base = 0; base < a.S && place < 0; base += 64) {
       int first, keys;
@@ -171,9 +202,9 @@ __global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a)
     for (int h = wave * HPW; h < a.nq; h += ROWS) {
       float v[VK_VEC];
 #pragma unroll
-      for (int e = 0; e < VK_VEC; ++e) v[e] = next[e];
+      for (int e = 0; e < VK_VEC; ++e) v[e] = element(next, e);
       ask(h + ROWS);
-      norm_and_turn<LPH>(v, a, a.q_w != nullptr, t, c0, y);
+      norm_and_turn<LPH>(v, a, a.q_w != nullptr, w, t, c0, y);
       if (h + sub < a.nq && inside) store_elems(a.q_out + ((int64_t)tok * a.nq + h + sub) * d + c0, v);
     }
     return;
@@ -182,8 +213,8 @@ __global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a)
   // ---- a page's new keys or values of one head
   const int job = block / (a.nkv * 2), head = (block >> 1) % a.nkv;
   const bool is_v = block & 1;
-  Turn t;
-  if (!is_v && a.k_w != nullptr) read_weights(a, a.k_w, c0, t);
+  float w[VK_VEC];
+  if (!is_v && a.k_w != nullptr) read_weights(a, a.k_w, c0, w);
   int seq = -1, tok0 = 0, off0 = 0, m = 0, pidx = 0;
   for (int base = 0, run = 0; base < a.S; base += 64) {
     int first, keys;
@@ -212,15 +243,17 @@ __global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a)
   }
   if (seq < 0 || pidx >= a.W) return;
   const elem_t* rows = a.qkv + (int64_t)tok0 * a.row_stride + (a.nq + head + (is_v ? a.nkv : 0)) * d + c0;
-  float next[VK_VEC];
+  const int place0 = (pidx << a.lp) + off0;
+  // A row's entries and its angles, asked for one row of the lane's ahead.
+  const bool turns = !is_v && a.cos_t != nullptr;
+  u32x4 next;
+  Angles next_t;
   auto ask = [&](int i) {
-#pragma unroll
-    for (int e = 0; e < VK_VEC; ++e) next[e] = 0.f;
-    if (i < m && inside) load_elems(rows + (int64_t)i * a.row_stride, next);
+    next = u32x4{0, 0, 0, 0};
+    if (i < m && inside) next = read_raw(rows + (int64_t)i * a.row_stride, true);
+    if (turns) read_angles(a, c0, place0 + min(i, m - 1), next_t);
   };
   ask(wave * HPW + sub);
-  const int place0 = (pidx << a.lp) + off0;
-  if (!is_v && a.cos_t != nullptr) read_angles(a, c0, place0 + min(wave * HPW + sub, m - 1), t);
   const int page = a.table[(int64_t)seq * a.W + pidx];
   if ((unsigned)page >= (unsigned)a.pages) return;    // a sequence whose rows are not to be kept
   const int64_t head_page = (int64_t)page * a.nkv + head;
@@ -228,41 +261,44 @@ __global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a)
   const int stood = exponent_of(*scale), old = off0 > 0 ? stood : CACHE8_LOWEST;
 
   double* y = reinterpret_cast<double*>(lds) + (wave * HPW + sub) * LPH * VK_VEC;
-  float* held = reinterpret_cast<float*>(lds + (a.whole ? 0 : STORE8_TURN * sizeof(double)));
+  uint16_t* held = reinterpret_cast<uint16_t*>(lds + (a.whole ? 0 : STORE8_TURN * sizeof(double)));
   // Rows i0 .. i0 + a.held - 1 into LDS: values as they are, keys normed and turned.  Returns the exponent that this lane's need.
-  auto entries = [&](int i0, bool angles) {
+  auto entries = [&](int i0) {
     int need = CACHE8_LOWEST;
     const int end = min(m, i0 + a.held);
     for (int r0 = i0; r0 < end; r0 += ROWS) {
       const int i = r0 + wave * HPW + sub;
       float v[VK_VEC];
 #pragma unroll
-      for (int e = 0; e < VK_VEC; ++e) v[e] = next[e];
+      for (int e = 0; e < VK_VEC; ++e) v[e] = element(next, e);
+      const Angles t = next_t;
       ask(i + ROWS);
       if (!is_v) {
         double k[VK_VEC];
 #pragma unroll
         for (int e = 0; e < VK_VEC; ++e) k[e] = (double)v[e];
-        if (a.cos_t != nullptr && (angles || r0 > i0)) read_angles(a, c0, place0 + min(i, m - 1), t);
-        norm_and_turn<LPH>(k, a, a.k_w != nullptr, t, c0, y);
+        norm_and_turn<LPH>(k, a, a.k_w != nullptr, w, t, c0, y);
 #pragma unroll
         for (int e = 0; e < VK_VEC; ++e) v[e] = round_to_odd(k[e]);
       }
       if (i < end && inside) {
+        uint32_t pair[VK_VEC / 2];
 #pragma unroll
-        for (int e = 0; e < VK_VEC; ++e) {
-          need = max(need, least_exponent(v[e]));
-          held[(i - i0) * d + c0 + e] = v[e];
-        }
+        for (int e = 0; e < VK_VEC; ++e) need = max(need, least_exponent(v[e]));
+#pragma unroll
+        for (int e = 0; e < VK_VEC; e += 2) pair[e / 2] = held_of(v[e]) | held_of(v[e + 1]) << 16;
+        uint32_t* to = reinterpret_cast<uint32_t*>(held + (i - i0) * d + c0);
+#pragma unroll
+        for (int e = 0; e < VK_VEC / 2; ++e) to[e] = pair[e];
       }
     }
     return need;
   };
-  int need = entries(0, false);
+  int need = entries(0);
   for (int i0 = a.held; i0 < m; i0 += a.held) {       // more rows than LDS holds: their maximum first, and once more for their entries
     __syncthreads();
     ask(i0 + wave * HPW + sub);
-    need = max(need, entries(i0, true));
+    need = max(need, entries(i0));
   }
   need = (int)wave_max_xor((float)need);
   if (lane == 0) wave_need[wave] = need;
@@ -276,15 +312,17 @@ __global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a)
     if (m > a.held) {
       __syncthreads();
       ask(i0 + wave * HPW + sub);
-      (void)entries(i0, true);
+      (void)entries(i0);
       __syncthreads();
     }
     if (!is_v) {
       for (int x = threadIdx.x; x < n * d / 16; x += STORE8_THREADS) {
-        const float* from = held + x * 16;
+        const u32x4 lo = *reinterpret_cast<const u32x4*>(held + x * 16), hi = *reinterpret_cast<const u32x4*>(held + x * 16 + 8);
+        const uint32_t from[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         u32x4 b;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) b[e] = to_fp8x4(entry_of(from[4 * e], now), entry_of(from[4 * e + 1], now), entry_of(from[4 * e + 2], now), entry_of(from[4 * e + 3], now));
+        for (int e = 0; e < 4; ++e)
+          b[e] = to_fp8x4(entry_of(number_of(from[2 * e]), now), entry_of(number_of(from[2 * e] >> 16), now), entry_of(number_of(from[2 * e + 1]), now), entry_of(number_of(from[2 * e + 1] >> 16), now));
         *reinterpret_cast<u32x4*>(kp + at * d + x * 16) = b;
       }
     } else {
@@ -295,14 +333,15 @@ __global__ __launch_bounds__(STORE8_THREADS, 4) void store8_kernel(Store8Args a)
       for (int x = threadIdx.x / WIDE; x < (c < d ? chunks : 0); x += STORE8_THREADS / WIDE) {
         const int o = o0 + (x << 4);
         if (o >= at && o + 16 <= at + n) {
-          const float* from = held + (o - at) * d + c;
+          const uint16_t* from = held + (o - at) * d + c;
           u32x4 b;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            b[e] = to_fp8x4(entry_of(from[4 * e * d], now), entry_of(from[(4 * e + 1) * d], now), entry_of(from[(4 * e + 2) * d], now), entry_of(from[(4 * e + 3) * d], now));
+            b[e] = to_fp8x4(entry_of(number_of(from[4 * e * d]), now), entry_of(number_of(from[(4 * e + 1) * d]), now), entry_of(number_of(from[(4 * e + 2) * d]), now),
+                            entry_of(number_of(from[(4 * e + 3) * d]), now));
           *reinterpret_cast<u32x4*>(vp + c * P + o) = b;
         } else {
-          for (int b = max(at, o); b < min(at + n, o + 16); ++b) vp[c * P + b] = (uint8_t)to_fp8x4(entry_of(held[(b - at) * d + c], now), 0.f, 0.f, 0.f);
+          for (int b = max(at, o); b < min(at + n, o + 16); ++b) vp[c * P + b] = (uint8_t)to_fp8x4(entry_of(number_of(held[(b - at) * d + c]), now), 0.f, 0.f, 0.f);
         }
       }
     }
@@ -369,8 +408,8 @@ int vk_qkv_post8(const elem_t* qkv, int64_t row_stride, elem_t* q_out, uint8_t* 
   VK_REQUIRE(kv_blocks + q_blocks < (1ll << 31), "qkv_post8: %d rows of %d heads are too many for one launch", T, nq + 2 * nkv);
   a.kv_blocks = (int)kv_blocks;
   // Rows that a workgroup holds in LDS: a page's, up to 32 KB (four workgroups a CU, so that some load while others round), and one where every sequence has one.
-  a.held = T <= S ? 1 : min(P, 32 * 1024 / 4 / d);
-  const int lds_q = a.whole ? 0 : STORE8_TURN * (int)sizeof(float), lds_kv = a.held * d * 4 + (a.whole ? 0 : STORE8_TURN * (int)sizeof(double));
+  a.held = T <= S ? 1 : min(P, 32 * 1024 / 2 / d);
+  const int lds_q = a.whole ? 0 : STORE8_TURN * (int)sizeof(float), lds_kv = a.held * d * 2 + (a.whole ? 0 : STORE8_TURN * (int)sizeof(double));
   const int vecs = d / VK_VEC;
 #define STORE8(L) store8_kernel<L><<<(unsigned)(kv_blocks + q_blocks), STORE8_THREADS, kv_blocks > 0 ? lds_kv : lds_q, st>>>(a);
 #ifdef VK_BF16
