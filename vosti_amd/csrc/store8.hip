@@ -8,15 +8,16 @@
 //   entry   x / 2^e to the nearest e4m3, half to even; the page's other entries are rounded once more where e has grown
 //
 // q is computed in 32-bit and rounded to the element type once.  k is computed in 64-bit: its entries keep four digits, and which ones they keep is decided by
-// the formula and not by the last bits of its evaluation (the vector unit's 64-bit additions and products are as fast as its 32-bit ones).
+// the formula and not by the last bits of its evaluation; in between they are rounded to odd, to 32 and to 16 bits, which changes no rounding to four digits (the vector unit's 64-bit additions and products are as fast as its 32-bit ones).
 //
 // A row of the step stands at place k_len - (rows of its sequence) + its number, in page table[sequence][place / P].  A workgroup takes
 // one (page, head, k or v) that the step writes to, so that the scale, the new entries and the old ones are one workgroup's
 // business; rows come to it by their sequence, not by slots.  The other workgroups take a token's q heads each.
 //
-// Measured (MI355X, bfloat16, 32 q and 8 kv heads of 128, pages of 64; a copy reaches 4.75 TB/s here): a prompt of 4,096 tokens, 93 MB: 33.7 us, 2.8 TB/s: a page's rows go through LDS
-// between their maximum and their rounding, and nothing else of the workgroup is under way then.  A token each of 64 sequences, 1.5 MB: 10.4 us: the sequence's lengths, then the page's
-// number, its scale and, where that grows, its entries, one load behind the other.  The 32-bit build, 2,300 tokens of 7 sequences, 16 and 8 heads of 64: 12 us.
+// Measured (MI355X, bfloat16, 32 q and 8 kv heads of 128, pages of 64; a copy reaches 4.75 TB/s here): a prompt of 4,096 tokens, 93 MB: 31 us, 28.6 in a row of calls, 3.0 to 3.3 TB/s: four
+// workgroups a CU is what the 64-bit norm's registers leave (five or six spill: 38 -> 50 us with nothing in the caches), and a page's rows wait for their maximum.  Rows and angles that are read one row ahead, as
+// they are stored, took 3 us off it and 2 off a step of 64 tokens.  A token each of 64 sequences, 1.5 MB: 8.8 us: the sequence's lengths, then the page's number, its scale and, where that grows,
+// its entries, one load behind the other.  The 32-bit build, 2,300 tokens of 7 sequences, 16 and 8 heads of 64: 13 us.
 #include "cache8.h"
 #include "vec.h"
 
@@ -407,7 +408,7 @@ int vk_qkv_post8(const elem_t* qkv, int64_t row_stride, elem_t* q_out, uint8_t* 
   const int64_t jobs = nkv > 0 ? min((int64_t)T, (int64_t)T / P + 2 * (int64_t)S) : 0, kv_blocks = jobs * nkv * 2, q_blocks = nq > 0 ? T : 0;
   VK_REQUIRE(kv_blocks + q_blocks < (1ll << 31), "qkv_post8: %d rows of %d heads are too many for one launch", T, nq + 2 * nkv);
   a.kv_blocks = (int)kv_blocks;
-  // Rows that a workgroup holds in LDS: a page's, up to 32 KB (four workgroups a CU, so that some load while others round), and one where every sequence has one.
+  // Rows that a workgroup holds in LDS: a page's, up to 32 KB (four workgroups a CU), and one where every sequence has one.
   a.held = T <= S ? 1 : min(P, 32 * 1024 / 2 / d);
   const int lds_q = a.whole ? 0 : STORE8_TURN * (int)sizeof(float), lds_kv = a.held * d * 2 + (a.whole ? 0 : STORE8_TURN * (int)sizeof(double));
   const int vecs = d / VK_VEC;
