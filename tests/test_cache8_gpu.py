@@ -414,6 +414,32 @@ def test_heads_of_small_and_large_entries(d, rows):
     assert np.array_equal(more, got)
 
 
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", (1, 9, 20))
+@pytest.mark.parametrize("d", (64, 128))
+def test_scores_that_32_bits_hold_to_a_hundred(name, rows, d):
+    """Scores of 2^30 and more: a weight is what 32 bits make of it, but no more than 1 beside the largest, so that a result lies among the values; and where one key is ahead by far it is that key's."""
+    k, P, nq, nkv, keys = kernels_for(name), 64, 4, 2, 700
+    rng = np.random.default_rng(rows + d)
+    table, pages = tables(rng, [keys], P)
+    kc, vc, scales = filled(rng, pages, nkv, P, d)
+    scales[..., 0] = 2.0 ** 12
+    q = torch.from_numpy(rng.standard_normal((rows, nq, d)) * 2.0 ** 14).to(TYPES[name]).cuda()
+    most = 16 if rows < 16 else 128
+    got = host(attend(k, q, (kc, vc, scales), table, [rows], [keys], most))
+    vv = host(vc) * host(scales)[:, :, 1, None, None]
+    assert np.isfinite(got).all() and np.abs(got).max() <= np.abs(vv).max() * (1 + 2.0 ** -8)
+    # Place 5 of the sequence along q's first row's heads, its other places across them.
+    kc[:] = torch.zeros((), device="cuda").to(E4M3)
+    page = int(table[0, 0])
+    q[:] = 0
+    q[..., 0] = 2.0 ** 14
+    kc[page, :, 5, 0] = torch.tensor(256.0, device="cuda").to(E4M3)
+    got = host(attend(k, q, (kc, vc, scales), table, [rows], [keys], most))
+    want = vv[page, :, :, 5].repeat(nq // nkv, 0)[None]
+    assert (np.abs(got - want) <= torch.finfo(TYPES[name]).eps / 2 * np.abs(want) + 2.0 ** -20 * np.abs(want).max()).all()
+
+
 @pytest.mark.parametrize("most", (16, 128))
 def test_a_window_longer_than_the_keys_hides_none(most):
     """Among rows that stand before the first key, where a window's begin could leave 32 bits."""

@@ -385,7 +385,7 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
     }
     m_tile[n] = over_groups_max(top) * a.scale_log2;
   }
-  bool moves = false;
+  bool moves = false, far = false;
   float by[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -394,6 +394,7 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
     by[n] = exp2_fast(o.m[n] - to);
     o.m[n] = to;
     moves = moves || move;
+    far = far || (fabsf(m_tile[n]) >= 67108864.f && (WHOLE == 1 || m_tile[n] != -INFINITY));      // 2^26; -inf: no key
   }
 #ifdef VK_BF16
   // The unit never falls, so that sums are scaled down only: what a smaller page adds is then in units of a larger one's.
@@ -404,12 +405,25 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
 #else
   const float to_unit = 1.f, v_scale = there ? pow2f(v_exp) : 1.f;
 #endif
-  if (__any(moves)) {
+  float from[NT];                                       // what is taken from the scores
+#pragma unroll
+  for (int n = 0; n < NT; ++n) from[n] = o.m[n];
+  if (__any(moves || far)) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       o.l[n] = o.l[n] * by[n];
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt) o.acc[n][dt] = o.acc[n][dt] * (by[n] * to_unit);
+    }
+    // The reference maximum was rounded and a score times the scale is not, before it is taken away: half a step of the maximum is a factor of all weights of the column.  From 2^26 on it could be 2^4
+    // and more, to 2^64 and beyond: there the score is rounded as the maximum was.
+    if (__any(far)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[x / 4][n][x % 4] = (s[x / 4][n][x % 4] * a.scale_log2 - from[n]) / a.scale_log2;
+        from[n] = 0.f;
+      }
     }
   }
   w_part w[NT][A8_WP];
@@ -417,7 +431,7 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
   for (int n = 0; n < NT; ++n) {
     float p[16];
 #pragma unroll
-    for (int x = 0; x < 16; ++x) p[x] = exp2_fast(__builtin_fmaf(s[x / 4][n][x % 4], a.scale_log2, -o.m[n]));
+    for (int x = 0; x < 16; ++x) p[x] = exp2_fast(__builtin_fmaf(s[x / 4][n][x % 4], a.scale_log2, -from[n]));
     set_weights(p, w[n]);
   }
   // Where two waves meet on a unit the one in front of these products goes first: they leave most cycles for the other's arithmetic (179 -> 161 us for a prompt of
@@ -910,7 +924,7 @@ static int a8_shared_as(const A8Args& a, hipStream_t st) {
   const int64_t units = (int64_t)a.n_items * a.nkv * blocks * (SPLIT ? a.nseg : 1);
   VK_REQUIRE(units < (1ll << 31), "attention8: %d items of %d rows, %d heads: too many for one launch", a.n_items, a.item_rows, a.nq);
   const int lds = A8_STAGES * A8Stage<DP, WAVES>::BYTES;
-  if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)a8_shared_kernel<DP, NT, WAVES, SPLIT, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  static_assert(A8_STAGES * A8Stage<DP, WAVES>::BYTES <= 64 * 1024, "what a launch may ask for");
   a8_shared_kernel<DP, NT, WAVES, SPLIT, WIDE><<<(unsigned)units, 64 * WAVES, lds, st>>>(a, blocks);
   return vk_check_launch("attention8");
 }
