@@ -429,6 +429,11 @@ def test_scores_that_32_bits_hold_to_a_hundred(name, rows, d):
     got = host(attend(k, q, (kc, vc, scales), table, [rows], [keys], most))
     vv = host(vc) * host(scales)[:, :, 1, None, None]
     assert np.isfinite(got).all() and np.abs(got).max() <= np.abs(vv).max() * (1 + 2.0 ** -8)
+    # Beside such heads another one is what it is beside small ones.
+    small = torch.from_numpy(rng.standard_normal((rows, nq, d)) * 2.0 ** -16).to(TYPES[name]).cuda()
+    beside = q.clone()
+    beside[:, 1] = small[:, 1]
+    assert torch.equal(attend(k, beside, (kc, vc, scales), table, [rows], [keys], most)[:, 1], attend(k, small, (kc, vc, scales), table, [rows], [keys], most)[:, 1])
     # Place 5 of the sequence along q's first row's heads, its other places across them.
     kc[:] = torch.zeros((), device="cuda").to(E4M3)
     page = int(table[0, 0])

@@ -385,6 +385,7 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
     }
     m_tile[n] = over_groups_max(top) * a.scale_log2;
   }
+  auto is_far = [&](int n) { return fabsf(m_tile[n]) >= 67108864.f && (WHOLE == 1 || m_tile[n] != -INFINITY); };      // 2^26; -inf: no key
   bool moves = false, far = false;
   float by[NT];
 #pragma unroll
@@ -394,7 +395,7 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
     by[n] = exp2_fast(o.m[n] - to);
     o.m[n] = to;
     moves = moves || move;
-    far = far || (fabsf(m_tile[n]) >= 67108864.f && (WHOLE == 1 || m_tile[n] != -INFINITY));      // 2^26; -inf: no key
+    far = far || is_far(n);
   }
 #ifdef VK_BF16
   // The unit never falls, so that sums are scaled down only: what a smaller page adds is then in units of a larger one's.
@@ -421,8 +422,8 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int x = 0; x < 16; ++x) s[x / 4][n][x % 4] = (s[x / 4][n][x % 4] * a.scale_log2 - from[n]) / a.scale_log2;
-        from[n] = 0.f;
+        for (int x = 0; x < 16; ++x) s[x / 4][n][x % 4] = is_far(n) ? (s[x / 4][n][x % 4] * a.scale_log2 - from[n]) / a.scale_log2 : s[x / 4][n][x % 4];
+        from[n] = is_far(n) ? 0.f : from[n];
       }
     }
   }
