@@ -21,8 +21,8 @@
 // taken out of the second product of a tile that not all rows see whole; a row that does see a NaN gets it back through a product of its own.
 //
 // What bounds it (MI355X, bfloat16, heads of 128, 8 kv heads; reading alone reaches 6.45 TB/s here, a large bfloat16 product 1.45 PFLOP/s): 64 rows with 8,192 keys each, 32 heads, 1.08 GB
-// of cache: 187 us, 5.75 TB/s, and 5 us for the join: bytes.  13 sequences of 5 rows and some 4,000 keys, 64 heads, 73 MB: 26 us and 5: workgroups of eight tiles one after
-// the other, little more than one round of them.  A prompt of 4,096 rows over itself, 32 heads, 137 GFLOP: 154 us, 137 in a row of calls, 0.89 to 1.0 PFLOP/s: a wave's products
+// of cache: 188 us, 5.7 TB/s, and 5 us for the join: bytes.  13 sequences of 5 rows and some 4,000 keys, 64 heads, 73 MB: 26 us and 5: workgroups of eight tiles one after
+// the other, little more than one round of them.  A prompt of 4,096 rows over itself, 32 heads, 137 GFLOP: 158 us, 138 to 144 in a row of calls, 0.87 to 0.99 PFLOP/s: a wave's products
 // and the exponentials behind them follow each other, and its registers leave room for two waves a unit.  A single row with 333 keys: 10 us, loads that wait for each other.
 #include <type_traits>
 
