@@ -16,7 +16,7 @@
 // search for the maximum), 8 to decide, 19 for the pieces, 8 to draw.  One sequence: 5.5, 7.2 and 6.5 us, launches and loads that wait for each other.
 //
 // Four launches: maximum and sum of pieces of every row, a wave each; which tokens stand, and the distributions behind them; what the pieces of those weigh; the piece and
-// the token in it.  Pieces have the same borders and their sums the same order whatever else is in the call.
+// the token in it (the second and third as one where there are few pieces).  Pieces have the same borders and their sums the same order whatever else is in the call.
 #include "common.h"
 #include "sampling.h"
 
