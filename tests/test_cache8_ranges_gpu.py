@@ -1,0 +1,82 @@
+"""Attention over an 8-bit cache (attention8.hip) where numbers lie far apart: scales of neighbouring pages, weights of neighbouring keys."""
+import numpy as np
+import pytest
+import torch
+
+from plain_cache8 import attention
+from test_cache8_gpu import TYPES, attend, close, filled, host, tables
+from vosti_amd.kernels import kernels_for
+
+pytestmark = pytest.mark.gpu
+
+
+def case(name, d, P, rows, keys, seed, nq=4, nkv=2, size=1.0):
+    rng = np.random.default_rng(seed)
+    table, pages = tables(rng, [keys], P)
+    q = torch.from_numpy(rng.standard_normal((rows, nq, d)) * size).to(TYPES[name]).cuda()
+    return table, filled(rng, pages, nkv, P, d, -6, -4), q
+
+
+def check(name, q, cache, table, rows, keys, window=0, without=()):
+    """The bounds of `close`, which hold each row to the values that it sees itself; `without`: pages of the sequence that weigh nothing and are none to the plain form and its bounds."""
+    got = attend(kernels_for(name), q, cache, table, [rows], [keys], 16 if rows <= 16 else 128, window)
+    seen = table.copy()
+    seen[0, list(without)] = -1
+    close(got, attention(host(q), *map(host, cache), seen, [0, rows], [keys], q.shape[2] ** -0.5, window), name, q.shape[2])
+
+
+@pytest.mark.parametrize("up", (15, 16, 30, 60))
+@pytest.mark.parametrize("P", (16, 64))
+@pytest.mark.parametrize("name,d,rows", [("bf16", 64, 5), ("bf16", 64, 20), ("bf16", 128, 5), ("bf16", 128, 11), ("bf16", 128, 20), ("bf16", 256, 20), ("f32", 64, 5), ("f32", 64, 20)])
+def test_a_large_page_that_one_row_sees_leaves_the_others(name, d, rows, P, up):
+    """A page whose values stand 2^up above the others': seen by the first row alone, the window of the next ones beginning behind it; and by the last row alone, which stands in its first place."""
+    window, at = 70, 6
+    keys = P * at + P - 1 + window - 1 + rows                  # row 0 sees the last place of page `at`
+    table, (kc, vc, scales), q = case(name, d, P, rows, keys, d + rows + P + up)
+    scales[..., 1] = 2.0 ** -5
+    scales[int(table[0, at]), :, 1] = 2.0 ** (up - 5)
+    check(name, q, (kc, vc, scales), table, rows, keys, window)
+    keys = P * at + 1                                          # the last row sees the first place of page `at`
+    scales[..., 1] = 2.0 ** -5
+    scales[int(table[0, at]), :, 1] = 2.0 ** (up - 5)
+    check(name, q, (kc, vc, scales), table, rows, keys)
+
+
+@pytest.mark.parametrize("up", (15, 30))
+@pytest.mark.parametrize("P", (16, 32, 64))
+@pytest.mark.parametrize("name,d,rows", [("bf16", 64, 1), ("bf16", 64, 20), ("bf16", 128, 1), ("bf16", 128, 9), ("bf16", 128, 20), ("bf16", 192, 9), ("f32", 128, 9)])
+def test_a_large_page_of_no_weight_leaves_the_others(name, d, rows, P, up):
+    """Pages 2^up above the others in whose keys every score is some 90 powers of two behind, which leaves 2^-40 of nothing: the first, one in the middle, the last but one."""
+    keys = 300
+    table, (kc, vc, scales), q = case(name, d, P, rows, keys, d + rows + P + up)
+    scales[..., 0], scales[..., 1] = 2.0 ** -6, 2.0 ** -5
+    kf = kc.float()
+    kf[..., 0] = 0.0
+    q[..., 0] = 8.0
+    used = -(-keys // P)
+    large = (0, used // 2, used - 2)
+    for at in large:
+        page = int(table[0, at])
+        kf[page] = 0.0
+        kf[page, ..., 0] = -round(90 * np.log(2) * d ** 0.5 / 8 * 2 ** 2)
+        scales[page, :, 0], scales[page, :, 1] = 2.0 ** -2, 2.0 ** (up - 5)
+    assert kf.abs().max() <= 448
+    check(name, q, (kf.to(kc.dtype), vc, scales), table, rows, keys, without=large)
+
+
+def test_a_small_page_beside_large_ones_is_exact():
+    """The smallest entries there are, in pages of every distance from the one in front of them that another row sees: one key's value, to the bit."""
+    k, d, P = kernels_for("bf16"), 64, 16
+    for rows in (2, 20):
+        for down in (1, 8, 14, 15, 16, 17, 22, 40):
+            keys = 32 + rows - 1
+            table, (kc, vc, scales), q = case("bf16", d, P, rows, keys, down)
+            window = rows - 1                                 # the last row sees keys 32 .. 30 + rows, the first one 33 - rows .. 31
+            scales[..., 1] = 1.0
+            scales[table[0, 2:].tolist(), :, 1] = 2.0 ** -down
+            kc[:] = torch.zeros((), device="cuda").to(kc.dtype)
+            least = torch.full(vc.shape, 2.0 ** -9, device="cuda")
+            least[:, :, ::2] *= 3
+            vc = least.to(vc.dtype)
+            got = host(attend(k, q, (kc, vc, scales), table, [rows], [keys], 16 if rows <= 16 else 128, window))[-1]
+            assert np.array_equal(got, np.broadcast_to(host(least)[0, 0, :, 0] * 2.0 ** -down, got.shape)), (rows, down)

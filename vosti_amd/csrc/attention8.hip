@@ -13,8 +13,9 @@
 // 2^-22 of that power at most elsewhere; products of twice the rate make up for there being two, and no key has to be turned into an operand (a prompt of 4,096 rows 186 -> 163 us; of heads of 64 the
 // product, 128 entries long, would be half empty).  Weights are at most 1 (2^8
 // where a reference maximum is kept) and go into the second product in 16-bit floating point with eleven digits, against values without their scale, which
-// they hold to the bit: bfloat16 weights, with eight, would double the squared error of the result.  Values' scales that differ within a product stand in its
-// entries relative to the largest of them.  The 32-bit build takes everything in 32 bits.  The sum of the weights comes from the matrix
+// they hold to the bit: bfloat16 weights, with eight, would double the squared error of the result.  Values' scales stand in the product's entries relative to a unit of the wave's sums
+// that follows the tile's (A8_UNIT_DOWN); pages of scales 2^11 apart and more in one tile are multiplied one after the other.  So a row's values keep their digits whatever stands in other
+// pages, up to scales 2^75 below the largest that the wave's columns see.  The 32-bit build takes everything in 32 bits.  The sum of the weights comes from the matrix
 // unit too, a product with ones: it is that of the very weights that the values are multiplied by, and the vector unit has enough to do.
 //
 // Keys that a row does not see weigh 0, whatever is stored: their scores are never used, and values outside what the wave's rows see, or NaN, are
@@ -35,6 +36,13 @@
 #define A8_SEG 512               // keys that are summed up apart where a row's keys are split over workgroups
 #define A8_STEP 8.0f             // a column's reference maximum moves where the tile's exceeds it by more (log2)
 #define A8_NONE -3.0e38f          // the reference maximum of a column that has seen no key: finite, so that differences with it are numbers
+// Values go into their product in 16-bit floating point, in units of 2^unit, and an e4m3 number is a whole multiple of 2^-9 of its scale, 448 of it at most: of scales from 2^-15 to 2^6 of the unit it
+// is held to the bit (2^-24 is the least such number).  The unit stays while a tile's largest scale is from 2^-4 to 2^6 of it, so that scales 2^11 apart need no second pass; it falls by
+// 2^60 at most, so that sums in larger units remain numbers in smaller ones.
+#define A8_UNIT_UP 6
+#define A8_UNIT_STAYS 4
+#define A8_UNIT_DOWN 15
+#define A8_UNIT_FALLS 60
 #define A8_STAGES 2               // tiles in LDS: one is computed, the next is arriving.  A third changed nothing for prompts (155 us for 4,096 rows both ways) and keeps workgroups of split keys from
                                   // the CU (5 rows each, 32 heads of 128, 32 sequences of 4,000 keys: 79 us against 72; 13 of 4,096 43 against 36; of unequal lengths 52 against 50)
 #define A8_ITEM_ROWS 128         // rows of an item, at most
@@ -296,9 +304,9 @@ struct A8Sums {
   f32x4 l[NT];                 // the same number in all four
   f32x4 acc[NT][DP / 16];
   typename std::conditional<(DP > 128), uint64_t, uint32_t>::type bad[NT];     // bit 4 dt + i: acc[n][dt][i] is NaN, by a value that is (where tiles are in registers; else it is set so)
-  int unit;
+  int unit, least_unit;
   __device__ __forceinline__ void clear() {
-    unit = -256;
+    unit = least_unit = -256;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n] = A8_NONE;
@@ -322,6 +330,17 @@ struct A8Sums {
     return 1.f;
 #endif
   }
+  // For values whose largest scale is 2^top (-256: there are none): the unit that suits them, and the least exponent that goes with it.  What lies below it takes a pass of its own.
+#ifdef VK_BF16
+  __device__ __forceinline__ int next_unit(int top) const {
+    const int to = unit == -256 || top > unit + A8_UNIT_UP ? top : top == -256 || top >= unit - A8_UNIT_STAYS ? unit : max(top, least_unit);
+    return __builtin_amdgcn_readfirstlane(to);
+  }
+  __device__ __forceinline__ static int least_exponent(int next, int top) { return top < next - A8_UNIT_DOWN ? -255 : next - A8_UNIT_DOWN; }
+#else
+  __device__ __forceinline__ int next_unit(int) const { return 0; }
+  __device__ __forceinline__ static int least_exponent(int, int) { return -255; }
+#endif
 };
 
 // The scores of a tile: S^T's, unscaled.  src.k(i, j): the lane's 16 bytes of K's tile i; k_scale: of the keys that they belong to.
@@ -356,14 +375,14 @@ __device__ __forceinline__ void a8_scores(const SRC& src, float k_scale, const A
 }
 
 // A tile's scores and values onto the wave's sums.  src.v(dt): the lane's 16 bytes of V's entries 16 dt + r; v_exp: of the 16 keys that they belong to, -256: none of them is there;
-// top_exp: the wave's largest.
+// unit: next_unit() of the wave's largest.
 //
 // A column's reference maximum follows its maximum only where that is more than 2^8 above: weights are 2^8 at most then (their sums are 32-bit, and 2^8 is nothing to
 // sixteen bits), and the sums are scaled in few tiles.  Which columns move is each column's own business; whether any does is the wave's.
 // WHOLE: 1: every column that stands for a row sees every key; 0: not so; 2: unknown, and found out for the values.  (What is only done under a condition must not touch scores and sums:
 // where the ways meet again they would be copied, and held twice.  A loop for each kind of tile in place of a condition: 225 -> 196 us for a prompt of 4,096 rows.)
 template <int WHOLE, int DP, int NT, typename SRC>
-__device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, int kb, const SRC& src, f32x4 (&s)[4][NT], int v_exp, int top_exp, A8Sums<DP, NT>& o) {
+__device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, int kb, const SRC& src, f32x4 (&s)[4][NT], int v_exp, int unit, A8Sums<DP, NT>& o) {
   const bool there = v_exp > -256;
   const bool full = WHOLE == 1 || (WHOLE == 2 && kb >= c.all_lo && kb + A8_TILE - 1 <= c.all_pos && __all(there));
   const int first = kb + 16 * c.g;
@@ -398,11 +417,10 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
     far = far || is_far(n);
   }
 #ifdef VK_BF16
-  // The unit never falls, so that sums are scaled down only: what a smaller page adds is then in units of a larger one's.
-  const int unit = max(o.unit, top_exp);
   const float to_unit = o.unit - unit < -126 ? 0.f : pow2f(o.unit - unit), v_scale = pow2f(max(-126, v_exp - unit));
   moves = moves || unit != o.unit;
   o.unit = unit;
+  o.least_unit = max(o.least_unit, unit - A8_UNIT_FALLS);
 #else
   const float to_unit = 1.f, v_scale = there ? pow2f(v_exp) : 1.f;
 #endif
@@ -624,17 +642,24 @@ __global__ __launch_bounds__(256, DP <= 128 && NT == 1 ? 2 : 1) void a8_few_kern
   a8_wait_q<DP, NT>(q);
   A8Sums<DP, NT> o;
   o.clear();
-  for (int kb = kb0; (kb & ~(A8_SEG - 1)) <= seg1 * A8_SEG; kb += A8_SEG / 2) {
+  int below = 256;                                      // scales of this and more have been taken, in the tile's passes before this one
+  for (int kb = kb0; (kb & ~(A8_SEG - 1)) <= seg1 * A8_SEG;) {
     const bool mine = kb <= pos && kb + A8_TILE > c.wave_lo;
-    const int exp_now = v_exp, top_now = __builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp));
+    const int exp_now = v_exp < below ? v_exp : -256, top = __builtin_amdgcn_readfirstlane((int)over_groups_max((float)exp_now));
+    const int unit = o.next_unit(top), least = o.least_exponent(unit, top);
+    const bool more = mine && __any(exp_now > -256 && exp_now < least);
     f32x4 s[4][NT];
     if (mine) a8_scores<DP, NT>(t, k_scale, q, s);
-    ask_k(kb + A8_SEG / 2);
-    if (mine) a8_weigh<2, DP, NT>(a, c, kb, t, s, exp_now, top_now, o);
+    ask_k(more ? kb : kb + A8_SEG / 2);
+    if (mine) a8_weigh<2, DP, NT>(a, c, kb, t, s, exp_now >= least ? exp_now : -256, unit, o);
     ask_v();
-    if ((kb & (A8_SEG / 2)) == 0) continue;
-    // Both tiles of the segment.
+    below = more ? least : 256;
+    if (more) continue;
+    const bool second = (kb & (A8_SEG / 2)) != 0;
     const int seg = kb / A8_SEG;
+    kb += A8_SEG / 2;
+    if (!second) continue;
+    // Both tiles of the segment.
 #pragma unroll
     for (int n = 0; n < NT; ++n)
       if (c.g == 0) {
@@ -684,6 +709,12 @@ struct A8Stage {
   static constexpr int PIECES = DP / 16;                                       // of a row of K
   __device__ static __forceinline__ int turn(int r) { return DP == 128 ? r >> 1 & 7 : DP == 256 ? r : r >> 2 & 3; }
 };
+
+#ifdef VK_BF16
+constexpr bool EXPONENTS = true;         // values' scales go into a unit of the sums
+#else
+constexpr bool EXPONENTS = false;
+#endif
 
 // What stands in scalar registers for an instruction written out, said to the compiler next to it: it may have moved the arithmetic to vector registers.
 __device__ __forceinline__ const uint8_t* a8_scalar(const uint8_t* p) {
@@ -792,6 +823,11 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
   auto fill = [&](A8Pages& pages, int& end, int i) {
     const int kb = lo + i * A8_TILE;
     pages.fill(a, c, kb >> a.lp, pos);
+    // and their values' scales are within 2^5 of the first one's, so that no tile of several pages needs a second pass (the whole spread, by two reductions: portions in pages of 16 keys 93 us for 90).
+    if (!WIDE && EXPONENTS) {
+      const int off = pages.v_exp - __builtin_amdgcn_readfirstlane(pages.v_exp);
+      pages.clean = pages.clean && __ballot(pages.v_exp > -256 && abs(off) > (A8_UNIT_DOWN - A8_UNIT_STAYS) / 2) == 0;
+    }
     end = __builtin_amdgcn_readfirstlane(i + (((64 << a.lp) - (kb & (a.P - 1))) >> 6));
   };
   if (tiles > 0) {
@@ -822,21 +858,37 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
     if (i >= now_end) fill(now, now_end, i);
     const int key = kb + 16 * c.g;
     float k_scale;
-    int v_exp, top_exp;
+    int v_exp;
     if (WIDE) {
       const int l = (kb >> a.lp) - now.base;
       k_scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.k_scale), l));
-      v_exp = top_exp = __builtin_amdgcn_readlane(now.v_exp, l);
-    } else {
-      k_scale = __shfl(now.k_scale, ((kb + 16 * (c.r >> 2)) >> a.lp) - now.base);
-      v_exp = __shfl(now.v_exp, (key >> a.lp) - now.base);
-      if (!all_see.value) v_exp = key <= c.wave_pos && key + 15 >= c.wave_lo ? v_exp : -256;
-      top_exp = __builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp));
+      const int exp = __builtin_amdgcn_readlane(now.v_exp, l), unit = o.next_unit(exp);
+      v_exp = all_see.value || (key <= c.wave_pos && key + 15 >= c.wave_lo) ? exp : -256;
+      f32x4 s[4][NT];
+      a8_scores<DP, NT>(src, k_scale, q, s);
+      a8_weigh<all_see.value, DP, NT>(a, c, kb, src, s, v_exp, unit, o);
+      return;
     }
+    k_scale = __shfl(now.k_scale, ((kb + 16 * (c.r >> 2)) >> a.lp) - now.base);
+    v_exp = __shfl(now.v_exp, (key >> a.lp) - now.base);
     if (!all_see.value) v_exp = key <= c.wave_pos && key + 15 >= c.wave_lo ? v_exp : -256;
-    f32x4 s[4][NT];
-    a8_scores<DP, NT>(src, k_scale, q, s);
-    a8_weigh<all_see.value, DP, NT>(a, c, kb, src, s, v_exp, top_exp, o);
+    if (all_see.value) {
+      const int unit = o.next_unit(__builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp)));
+      f32x4 s[4][NT];
+      a8_scores<DP, NT>(src, k_scale, q, s);
+      a8_weigh<all_see.value, DP, NT>(a, c, kb, src, s, v_exp, unit, o);
+      return;
+    }
+    for (bool more = true; more;) {
+      const int top = __builtin_amdgcn_readfirstlane((int)over_groups_max((float)v_exp)), unit = o.next_unit(top), least = o.least_exponent(unit, top);
+      more = __any(v_exp > -256 && v_exp < least);
+      int from = kb;
+      asm volatile("" : "+s"(from));                    // or every comparison with it would be made before the loop and held in scalar registers that there are not
+      f32x4 s[4][NT];
+      a8_scores<DP, NT>(src, k_scale, q, s);
+      a8_weigh<0, DP, NT>(a, c, from, src, s, v_exp >= least ? v_exp : -256, unit, o);
+      v_exp = v_exp >= least ? -256 : v_exp;
+    }
   };
   for (int i = 0; i < tiles;) {
     for (; i < tiles && !(i >= whole0 && i < whole1 && i < now_end && now.clean); ++i) step(i, std::integral_constant<int, 0>());

@@ -484,7 +484,7 @@ class Kernels:
         a scratch belongs to one call at a time, in recorded graphs too.  They are for decoded and drafted tokens and for a portion of few sequences (32 heads of 128,
         one sequence of 8,192 keys: 128 rows in 50 us, as one item in 208); larger items read the cache less often and are for prompts (1,024 rows of that sequence: 209 us
         against 278; 64 portions of 128 rows with 1,000 keys: 168 against 367).  A row's last bits depend on its item (``item_rows``, the item's other
-        rows) and on nothing else in the call.  ``max_k_len`` is the host's bound on k_len; the block table must cover it, and keys beyond it may be left out.  Rows that no item
+        rows) and on nothing else in the call.  In bfloat16, values of pages whose scale is 2^75 below that of another page that the same item sees may count as 0.  ``max_k_len`` is the host's bound on k_len; the block table must cover it, and keys beyond it may be left out.  Rows that no item
         names are left as they were."""
         here = self._device()
         if q.dim() != 3 or k_cache.dim() != 4:
