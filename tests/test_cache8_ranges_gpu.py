@@ -80,3 +80,27 @@ def test_a_small_page_beside_large_ones_is_exact():
             vc = least.to(vc.dtype)
             got = host(attend(k, q, (kc, vc, scales), table, [rows], [keys], 16 if rows <= 16 else 128, window))[-1]
             assert np.array_equal(got, np.broadcast_to(host(least)[0, 0, :, 0] * 2.0 ** -down, got.shape)), (rows, down)
+
+
+@pytest.mark.parametrize("behind", (20, 25, 29))
+@pytest.mark.parametrize("name,d,P,rows,keys", [("bf16", 64, 64, 20, 4096), ("bf16", 64, 16, 20, 4000), ("bf16", 128, 64, 33, 2100), ("bf16", 256, 64, 17, 700), ("bf16", 128, 64, 1, 3000),
+                                                ("bf16", 128, 64, 12, 1500), ("f32", 64, 64, 20, 4096)])
+def test_weights_far_behind_one_key_of_no_value(name, d, P, rows, keys, behind):
+    """The first key is 2^behind ahead of all others and its value is 0: what is left of the result is theirs.  A weight is off by 2^-11 of itself, or by 2^-32 of the largest (half of 2^-24 where the largest
+    is 2^7 or more); otherwise the bounds are those of `close`."""
+    table, (kc, vc, scales), q = case(name, d, P, rows, keys, d + keys + behind, size=0.25)
+    scales[..., 0] = 2.0 ** -6
+    scales[int(table[0, 0]), :, 0] = 1.0                       # (its other keys are zeros)
+    kf, vf = kc.float(), vc.float().abs()
+    kf[..., 0], q[..., 0] = 0.0, 8.0
+    kf[int(table[0, 0])] = 0.0
+    kf[int(table[0, 0]), :, 0, 0] = round(behind * np.log(2) * d ** 0.5 / 8)
+    vf[int(table[0, 0]), :, :, 0] = 0.0
+    kc, vc = kf.to(kc.dtype), vf.to(vc.dtype)
+    got = host(attend(kernels_for(name), q, (kc, vc, scales), table, [rows], [keys], 16 if rows <= 16 else 128))
+    out, weighted, most, flushed = attention(host(q), *map(host, (kc, vc, scales)), table, [0, rows], [keys], d ** -0.5)
+    weights = 2.0 ** -11 if name == "bf16" else 2.0 ** -20
+    score = 2 * (d + 16) * 2.0 ** -24 * most + 2.0 ** -20
+    bound = torch.finfo(TYPES[name]).eps / 2 * out * 1.01 + (weighted + out) * weights + weighted * score + (2.0 ** -32 if name == "bf16" else 0.0) * flushed
+    assert (np.abs(got - out) <= bound).all(), (np.abs(got - out) / bound).max()
+    assert behind > 25 or (bound < 0.1 * out).all()            # the bounds say something

@@ -11,8 +11,8 @@
 // Arithmetic.  A key's entry times its scale is exact in the element type, so the first product takes q as it is and 32-bit sums.  For heads of 128 and 256 it takes the keys as they are
 // stored, and q as two e4m3 numbers of four digits each in units of the head's largest entry: they hold its eight digits where it is 2^-14 of the largest's power of two or more, and are off by
 // 2^-22 of that power at most elsewhere; products of twice the rate make up for there being two, and no key has to be turned into an operand (a prompt of 4,096 rows 186 -> 163 us; of heads of 64 the
-// product, 128 entries long, would be half empty).  Weights are at most 1 (2^8
-// where a reference maximum is kept) and go into the second product in 16-bit floating point with eleven digits, against values without their scale, which
+// product, 128 entries long, would be half empty).  Weights go into the
+// second product in 16-bit floating point with eleven digits down to 2^-21 of the column's largest, and off by 2^-32 of that at most below (A8_LOW), against values without their scale, which
 // they hold to the bit: bfloat16 weights, with eight, would double the squared error of the result.  Values' scales stand in the product's entries relative to a unit of the wave's sums
 // that follows the tile's (A8_UNIT_DOWN); pages of scales 2^11 apart and more in one tile are multiplied one after the other.  So a row's values keep their digits whatever stands in other
 // pages, up to scales 2^75 below the largest that the wave's columns see.  The 32-bit build takes everything in 32 bits.  The sum of the weights comes from the matrix
@@ -34,7 +34,18 @@
 
 #define A8_TILE 64
 #define A8_SEG 512               // keys that are summed up apart where a row's keys are split over workgroups
-#define A8_STEP 8.0f             // a column's reference maximum moves where the tile's exceeds it by more (log2)
+// A column's reference, log2: A8_LOW below the maximum that set it, and it moves where a tile's maximum stands more than A8_STEP above it, 8 above the one that set it.  Weights of 16 bits are then 2^15 at
+// most (and no more than 2^15.2 with the rounding of a maximum below 2^22); they hold eleven digits down to 2^-21 of the largest and are off by half of 2^-24, 2^-32 of the largest, below that.  With references that
+// are the maximum itself it was 2^-25: 4,096 keys that stand that far behind one whose value is 0 gave a result off by 2 % and more.
+#ifdef VK_BF16
+#define A8_LOW 7.0f
+#define A8_STEP 15.0f
+#define A8_FAR 4194304.0f         // 2^22
+#else
+#define A8_LOW 0.0f
+#define A8_STEP 8.0f
+#define A8_FAR 67108864.0f        // 2^26
+#endif
 #define A8_NONE -3.0e38f          // the reference maximum of a column that has seen no key: finite, so that differences with it are numbers
 // Values go into their product in 16-bit floating point, in units of 2^unit, and an e4m3 number is a whole multiple of 2^-9 of its scale, 448 of it at most: of scales from 2^-15 to 2^6 of the unit it
 // is held to the bit (2^-24 is the least such number).  The unit stays while a tile's largest scale is from 2^-4 to 2^6 of it, so that scales 2^11 apart need no second pass; it falls by
@@ -377,8 +388,7 @@ __device__ __forceinline__ void a8_scores(const SRC& src, float k_scale, const A
 // A tile's scores and values onto the wave's sums.  src.v(dt): the lane's 16 bytes of V's entries 16 dt + r; v_exp: of the 16 keys that they belong to, -256: none of them is there;
 // unit: next_unit() of the wave's largest.
 //
-// A column's reference maximum follows its maximum only where that is more than 2^8 above: weights are 2^8 at most then (their sums are 32-bit, and 2^8 is nothing to
-// sixteen bits), and the sums are scaled in few tiles.  Which columns move is each column's own business; whether any does is the wave's.
+// A column's reference follows its maximum only where that is more than 2^8 above the one that set it (A8_STEP): the sums are scaled in few tiles.  Which columns move is each column's own business; whether any does is the wave's.
 // WHOLE: 1: every column that stands for a row sees every key; 0: not so; 2: unknown, and found out for the values.  (What is only done under a condition must not touch scores and sums:
 // where the ways meet again they would be copied, and held twice.  A loop for each kind of tile in place of a condition: 225 -> 196 us for a prompt of 4,096 rows.)
 template <int WHOLE, int DP, int NT, typename SRC>
@@ -404,13 +414,13 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
     }
     m_tile[n] = over_groups_max(top) * a.scale_log2;
   }
-  auto is_far = [&](int n) { return fabsf(m_tile[n]) >= 67108864.f && (WHOLE == 1 || m_tile[n] != -INFINITY); };      // 2^26; -inf: no key
+  auto is_far = [&](int n) { return fabsf(m_tile[n]) >= A8_FAR && (WHOLE == 1 || m_tile[n] != -INFINITY); };      // -inf: no key
   bool moves = false, far = false;
   float by[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const bool move = m_tile[n] > o.m[n] + A8_STEP;
-    const float to = move ? m_tile[n] : o.m[n];
+    const bool move = m_tile[n] - o.m[n] > A8_STEP;      // (the difference of neighbours is exact, a sum with the step is not)
+    const float to = move ? m_tile[n] - A8_LOW : o.m[n];
     by[n] = exp2_fast(o.m[n] - to);
     o.m[n] = to;
     moves = moves || move;
@@ -434,8 +444,8 @@ __device__ __forceinline__ void a8_weigh(const A8Args& a, const A8Rows<NT>& c, i
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt) o.acc[n][dt] = o.acc[n][dt] * (by[n] * to_unit);
     }
-    // The reference maximum was rounded and a score times the scale is not, before it is taken away: half a step of the maximum is a factor of all weights of the column.  From 2^26 on it could be 2^4
-    // and more, to 2^64 and beyond: there the score is rounded as the maximum was.
+    // The reference maximum was rounded and a score times the scale is not, before it is taken away: half a step of the maximum is a factor of all weights of the column.  From A8_FAR on it could take
+    // a weight beyond sixteen bits, and then to 2^64 and more: there the score is rounded as the maximum was.
     if (__any(far)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
