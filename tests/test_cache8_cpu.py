@@ -129,3 +129,13 @@ def test_verified_tokens_are_the_targets_distribution():
         seen[verify(p, ids[i:i + 1], [0, 2], q, [1.0], u[i:i + 1], w[i:i + 1])[0][0]] += 1
     want = chances(p[0], 1.0)
     assert (np.abs(seen / N - want) <= 5 * np.sqrt(want * (1 - want) / N)).all()
+
+
+@pytest.mark.parametrize("window,rows,segments", [(1, 1, 1), (2, 1, 2), (1, 2, 2), (512, 1, 2), (513, 1, 2), (514, 1, 3), (510, 4, 2), (512, 16, 3), (1024, 5, 4), (5000, 1, 10), (4999, 1, 10), (0, 1, 10)])
+def test_scratch_of_attention_with_a_window(kernels, window, rows, segments):
+    """So many segments of 512 as that many neighbouring keys touch, of a bound of 5,000."""
+    keys = window + rows - 1
+    if 0 < window < 5000:
+        touched = max((a + keys - 1) // 512 - a // 512 + 1 for a in range(1024))
+        assert segments == min(touched, 10)
+    assert kernels.attn8_scratch_floats(3, rows, 8, 64, 5000, window) == (3 * rows * 8 * 66 * segments if segments > 1 else 0)

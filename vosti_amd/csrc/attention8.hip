@@ -64,7 +64,7 @@ struct A8Args {
   const uint8_t *kc, *vc;
   const float* scales;
   const int32_t *table, *cu_q, *k_len, *items;
-  float *part_ml, *part_acc;   // per (item, kv head, segment, column): maximum and sum; d sums
+  float *part_ml, *part_acc;   // per (item, kv head, segment of the column's block from its first on, column): reference and sum; d sums
   int W, T, S, nq, nkv, d, P, lp, pages, group, item_rows, cols_max, window, nseg, n_items, max_keys;
   float scale_log2;
 };
@@ -607,7 +607,7 @@ __global__ __launch_bounds__(256, DP <= 128 && NT == 1 ? 2 : 1) void a8_few_kern
   if (!a8_rows<NT>(a, item, kvh, 0, c)) return;
   int seg_first, seg_last;
   a8_segments(c.wave_lo, c.wave_pos, seg_first, seg_last);
-  const int seg0 = max(seg_first, (int)blockIdx.y * segs_each), seg1 = min(seg_last, (int)blockIdx.y * segs_each + segs_each - 1);
+  const int seg0 = seg_first + (int)blockIdx.y * segs_each, seg1 = min(seg_last, seg0 + segs_each - 1);
   if (seg0 > seg1) return;
   const int kb0 = seg0 * A8_SEG + wave * A8_TILE, pos = min(c.wave_pos, seg1 * A8_SEG + A8_SEG - 1);
   A8Query<DP, NT> q;
@@ -688,7 +688,7 @@ __global__ __launch_bounds__(256, DP <= 128 && NT == 1 ? 2 : 1) void a8_few_kern
       for (int dt = 0; dt < DP / 16; ++dt) *reinterpret_cast<f32x4*>(sums[wave][dt][lane]) = o.times(n, dt, by);
       __syncthreads();
       if (col < c.cols) {
-        const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg) * a.cols_max + col;
+        const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg - seg_first) * a.cols_max + col;
 #pragma unroll
         for (int x = 0; x < DP / 64; ++x) {
           const int dt = 4 * x + wave;
@@ -799,7 +799,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
   int unit = blockIdx.x;
   const int kvh = unit % a.nkv;
   unit /= a.nkv;
-  const int seg = SPLIT ? unit % a.nseg : 0;
+  const int seg_at = SPLIT ? unit % a.nseg : 0;
   if (SPLIT) unit /= a.nseg;
   const int block = unit % blocks, item = SPLIT ? unit / blocks : a.n_items - 1 - unit / blocks;     // a prompt's last rows, which see most keys, first
   A8Rows<NT> c;
@@ -809,7 +809,8 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
   int lo = all.wave_lo, pos = all.wave_pos, seg_first = 0, seg_last = 0;
   if (SPLIT) {
     a8_segments(lo, pos, seg_first, seg_last);
-    if (seg < seg_first || seg > seg_last) return;
+    const int seg = seg_first + seg_at;
+    if (seg > seg_last) return;
     lo = max(lo, seg * A8_SEG);
     pos = min(pos, seg * A8_SEG + A8_SEG - 1);
   }
@@ -911,7 +912,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
     const float l = o.l[n][0];
     if (col >= c.cols) continue;
     if (SPLIT && seg_first != seg_last) {
-      const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg) * a.cols_max + col;
+      const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg_at) * a.cols_max + col;
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt)
         if (16 * dt < a.d) *reinterpret_cast<f32x4*>(a.part_acc + part * a.d + 16 * dt + 4 * c.g) = o.times(n, dt, o.scale());
@@ -936,19 +937,20 @@ __global__ __launch_bounds__(256) void a8_join_kernel(A8Args a, int cols) {
   a8_segments(a.window > 0 ? max(0, c.pos0 + row_first - a.window + 1) : 0, min(c.pos0 + row_last, a.max_keys - 1), seg_first, seg_last);
   if (seg_first == seg_last) return;                    // the other kernel wrote the result
   const int64_t part0 = ((int64_t)item * a.nkv + kvh) * a.nseg * a.cols_max + col;
+  const int segs = seg_last - seg_first + 1;
   float top = A8_NONE;
-  for (int s = seg_first + lane; s <= seg_last; s += 64) top = fmaxf(top, a.part_ml[2 * (part0 + (int64_t)s * a.cols_max)]);
+  for (int s = lane; s < segs; s += 64) top = fmaxf(top, a.part_ml[2 * (part0 + (int64_t)s * a.cols_max)]);
   top = wave_max_xor(top);
   float total = 0.f;
   f32x2 o[2] = {{0.f, 0.f}, {0.f, 0.f}};
-  for (int s0 = seg_first; s0 <= seg_last; s0 += 64) {
+  for (int s0 = 0; s0 < segs; s0 += 64) {
     float by = 0.f;
-    if (s0 + lane <= seg_last) {
+    if (s0 + lane < segs) {
       const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * (part0 + (int64_t)(s0 + lane) * a.cols_max));
       by = exp2_fast(ml.x - top);
       total = __builtin_fmaf(ml.y, by, total);
     }
-    const int n = min(64, seg_last - s0 + 1);
+    const int n = min(64, segs - s0);
     const float* p = a.part_acc + (part0 + (int64_t)s0 * a.cols_max) * a.d + 2 * lane;
     for (int s = 0; s < n; s += 8) {
       f32x2 v[8][2];
@@ -1000,9 +1002,15 @@ static int a8_shared(const A8Args& a, hipStream_t st) {
 
 extern "C" {
 
-// 32-bit words of scratch for `items` items of up to item_rows <= 16 rows: 0 for more rows, whose keys are not split, and for few keys.
-int64_t vk_attn8_scratch_floats(int items, int item_rows, int nq, int d, int max_k_len) {
-  const int64_t nseg = ((int64_t)max_k_len + A8_SEG - 1) / A8_SEG;
+// Segments that the rows of an item may have keys in: those of the bound, and of a window no more than its keys and the rows' other places touch.
+static int64_t a8_most_segments(int item_rows, int max_k_len, int window) {
+  const int64_t all = ((int64_t)max_k_len + A8_SEG - 1) / A8_SEG, keys = (int64_t)window + item_rows - 1;
+  return window > 0 && window < max_k_len ? min(all, (keys + A8_SEG - 2) / A8_SEG + 1) : all;
+}
+
+// 32-bit words of scratch for `items` items of up to item_rows <= 16 rows: 0 for more rows, whose keys are not split, and for few keys.  window: 0, or that of the call.
+int64_t vk_attn8_scratch_floats(int items, int item_rows, int nq, int d, int max_k_len, int window) {
+  const int64_t nseg = a8_most_segments(item_rows, max_k_len, window);
   if (item_rows > 16 || nseg <= 1) return 0;
   return (int64_t)items * item_rows * nq * nseg * (d + 2);
 }
@@ -1023,7 +1031,7 @@ int vk_paged_attention8(elem_t* out, const elem_t* q, const uint8_t* kc, const u
   VK_REQUIRE(scale > 0.f && scale < INFINITY, "attention8: scale %g is no positive number", (double)scale);
   if (n_items == 0 || T == 0 || S == 0) return 0;
   VK_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)scratch) % 16 == 0, "attention8: rows, cache and scratch have to lie on 16 bytes");
-  const int group = nq / nkv, nseg = max(1, (int)(((int64_t)max_k_len + A8_SEG - 1) / A8_SEG));
+  const int group = nq / nkv, nseg = max(1, (int)a8_most_segments(item_rows, max_k_len, window));
   // A window as long as the keys hides none; as none it takes part in no difference that could pass 32 bits.
   A8Args a{q, out, kc, vc, scales, table, cu_q, k_len, items, nullptr, nullptr, W, T, S, nq, nkv, d, P, 0, pages, group, item_rows, item_rows * group,
            window >= max_k_len ? 0 : window, nseg, n_items, max_k_len, scale * 1.4426950408889634f};
@@ -1034,7 +1042,7 @@ int vk_paged_attention8(elem_t* out, const elem_t* q, const uint8_t* kc, const u
     return d <= 64 ? a8_shared<64, NT, 4, false>(a, st) : d <= 128 ? a8_shared<128, NT, 4, false>(a, st) : d <= 192 ? a8_shared<192, NT, 4, false>(a, st)
                                                                                                                    : a8_shared<256, NT, 4, false>(a, st);
   }
-  const int64_t need = vk_attn8_scratch_floats(n_items, item_rows, nq, d, max_k_len);
+  const int64_t need = vk_attn8_scratch_floats(n_items, item_rows, nq, d, max_k_len, window);
   VK_REQUIRE(need == 0 || (scratch != nullptr && scratch_floats >= need), "attention8: scratch of %lld floats needed", (long long)need);
   a.part_acc = scratch;
   a.part_ml = scratch + need / (d + 2) * d;

@@ -178,7 +178,7 @@ struct Kernels::Fn {
   int (*attn_rel_pad)();
 };
 
-static constexpr int KERNEL_ABI = 21;
+static constexpr int KERNEL_ABI = 22;
 
 Kernels::Kernels(const std::string& lib_dir, const std::string& name) : name_(name), fn_(new Fn) {
   if (name == "bf16") dtype_ = DType::BF16;

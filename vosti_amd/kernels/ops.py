@@ -15,7 +15,7 @@ import torch
 
 from . import build
 
-ABI_VERSION = 21
+ABI_VERSION = 22
 SEGMENT_KEYS = 256
 ATTN_ITEM_ROWS = 128      # rows of one prompt item of paged_attention, and of any item of paged_attention8
 CACHE8_DTYPE = torch.float8_e4m3fn
@@ -87,7 +87,7 @@ class Kernels:
         lib.vk_attn_item_rows.restype = c_int
         _sig(lib.vk_qkv_post8, P, L, P, P, P, P, P, P, I, P, P, I, P, I, P, P, I, I, I, I, I, I, I, I, c_double, P)
         _sig(lib.vk_paged_attention8, P, P, P, P, P, P, I, P, P, P, I, I, P, L, I, I, I, I, I, I, I, I, I, F, P)
-        lib.vk_attn8_scratch_floats.argtypes = [I, I, I, I, I]
+        lib.vk_attn8_scratch_floats.argtypes = [I, I, I, I, I, I]
         lib.vk_attn8_scratch_floats.restype = c_int64
         _sig(lib.vk_verify, P, P, P, P, P, P, P, P, P, P, P, L, I, I, I, I, P)
         lib.vk_verify_scratch_bytes.argtypes = [I, I, I, I]
@@ -469,9 +469,11 @@ class Kernels:
                    nq, nkv, d, P, pages, max_k_len, eps, self._stream())
         return q_out if nq else None
 
-    def attn8_scratch_floats(self, items: int, item_rows: int, nq: int, d: int, max_k_len: int) -> int:
-        """float32 elements of scratch that ``paged_attention8`` needs for ``items`` items of up to ``item_rows`` rows."""
-        return int(self.lib.vk_attn8_scratch_floats(items, item_rows, nq, d, max_k_len))
+    def attn8_scratch_floats(self, items: int, item_rows: int, nq: int, d: int, max_k_len: int, window: int = 0) -> int:
+        """float32 elements of scratch that ``paged_attention8`` needs for ``items`` items of up to ``item_rows`` rows: items * item_rows * nq * (d + 2) for each segment of 512 keys, those of
+        the bound or, with a window, those that window + item_rows - 1 neighbouring keys can touch.  (64 items of 5 rows, 64 heads of 128: 10.6 MB a segment, and 2.7 GB for a bound of 131,072
+        keys without a window.)"""
+        return int(self.lib.vk_attn8_scratch_floats(items, item_rows, nq, d, max_k_len, window))
 
     def paged_attention8(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor,
                          block_table: torch.Tensor, cu_q: torch.Tensor, k_len: torch.Tensor, items: torch.Tensor,
@@ -503,7 +505,7 @@ class Kernels:
         klp, ip = self._at(k_len, "k_len", torch.int32, (S,), here), self._at(items, "items", torch.int32, (n_items, 2), here)
         out = torch.empty_like(q) if out is None else out
         op = self._at(out, "out", self.dtype, (T, nq, d), here)
-        need, scratch_p = self.attn8_scratch_floats(n_items, item_rows, nq, d, max_k_len) if item_rows <= 16 else 0, None
+        need, scratch_p = self.attn8_scratch_floats(n_items, item_rows, nq, d, max_k_len, window) if item_rows <= 16 else 0, None
         if need:
             scratch = torch.empty(need, dtype=torch.float32, device=q.device) if scratch is None else scratch
             scratch_p = self._at(scratch, "scratch", torch.float32, (scratch.numel(),), here)
