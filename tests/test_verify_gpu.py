@@ -284,3 +284,28 @@ def test_a_recorded_step_is_the_step(name):
                 assert np.array_equal(host(a), host(b))
         states[1] = m.next(states[1], out[1], out[2])
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("drawn", (False, True))
+def test_a_sequence_beside_one_that_the_arrays_do_not_hold(drawn):
+    """Its tokens, count and chances are those of the definition, whatever the next one's rows are said to be."""
+    k, V, rng = kernels_for("bf16"), 100, np.random.default_rng(31)
+    logits = torch.from_numpy(rng.standard_normal((9, V)) * 3).to(torch.bfloat16).cuda()
+    near = torch.from_numpy(rng.standard_normal((3, V))).to(torch.bfloat16).cuda() if drawn else None
+    seen = set()
+    for again in range(12):
+        ids, u, w = rng.integers(0, V, 3), rng.random(3).astype(np.float32) * 0.02, rng.random(2).astype(np.float32)
+        want = verify(host(logits)[:3], ids[:2], [0, 3], host(near[:2]) if drawn else None, [float(np.float32(0.9))], u[:2].astype(np.float64), w[:1].astype(np.float64))
+        for cu in ([0, 3, 10], [0, 3, 2], [0, 3, 2 ** 31 - 1], [0, 3, -1]):
+            tokens, counts, accept = k.verify(logits, ints(ids), ints(cu), draft_logits=near, temps=floats([0.9, 0.9]), accept_uniforms=floats(u), draw_uniforms=floats(w))
+            assert tokens[:3].tolist() == want[0].tolist() and counts.tolist() == [want[1][0], 0]
+            assert (np.abs(accept[:2].cpu().numpy() - want[2]) <= 2.0 ** -24 * want[2] + 1e-12).all()
+        seen.add(int(want[1][0]))
+    assert len(seen) > 1
+
+
+def test_a_batch_whose_sequences_have_no_rows():
+    """No logits at all: no tokens, and no error."""
+    k = kernels_for("bf16")
+    tokens, counts, accept = k.verify(torch.zeros(0, 700, dtype=torch.bfloat16, device="cuda"), ints(np.zeros(0)), ints([0, 0, 0]))
+    assert tokens.shape == (0,) and accept.shape == (0,) and counts.tolist() == [0, 0]

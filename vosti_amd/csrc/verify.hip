@@ -484,7 +484,7 @@ int vk_verify(int32_t* tokens, int32_t* counts, float* accept, const elem_t* log
   VK_REQUIRE(R >= 0 && D >= 0 && S >= 0 && V > 0 && V < (1 << 30), "verify: bad sizes R=%d D=%d S=%d V=%d", R, D, S, V);
   VK_REQUIRE(temps == nullptr || (draw_u != nullptr && (accept_u != nullptr || D == 0)), "verify: temperatures need random numbers");
   if (S == 0) return 0;
-  VK_REQUIRE(tokens != nullptr && counts != nullptr && logits != nullptr && cu != nullptr && (D == 0 || (ids != nullptr && accept != nullptr)), "verify: an array is missing");
+  VK_REQUIRE(counts != nullptr && cu != nullptr && (R == 0 || (tokens != nullptr && logits != nullptr)) && (D == 0 || (ids != nullptr && accept != nullptr)), "verify: an array is missing");
   VK_REQUIRE(scratch != nullptr && (uintptr_t)scratch % 16 == 0 && scratch_bytes >= vk_verify_scratch_bytes(R, D, S, V), "verify: %lld bytes of scratch needed, on 16 bytes",
              (long long)vk_verify_scratch_bytes(R, D, S, V));
   const int pieces = (int)verify_pieces(V);
