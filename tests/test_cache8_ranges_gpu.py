@@ -104,3 +104,17 @@ def test_weights_far_behind_one_key_of_no_value(name, d, P, rows, keys, behind):
     bound = torch.finfo(TYPES[name]).eps / 2 * out * 1.01 + (weighted + out) * weights + weighted * score + (2.0 ** -32 if name == "bf16" else 0.0) * flushed
     assert (np.abs(got - out) <= bound).all(), (np.abs(got - out) / bound).max()
     assert behind > 25 or (bound < 0.1 * out).all()            # the bounds say something
+
+
+@pytest.mark.parametrize("name,d,rows,keys", [("bf16", 64, 1, 400), ("bf16", 64, 1, 700), ("bf16", 128, 2, 1200), ("bf16", 64, 8, 700), ("bf16", 128, 16, 300), ("bf16", 128, 20, 700), ("f32", 64, 2, 700)])
+def test_values_near_the_largest_numbers(name, d, rows, keys):
+    """Values to 2^114, and a key in the second tile of a wave's whose weight is 2^7.9 times that of the keys in the first: sums of weights times values leave 32 bits where a weight may be 2^15."""
+    table, (kc, vc, scales), q = case(name, d, 64, rows, keys, d + keys)
+    scales[..., 0], scales[..., 1] = 2.0 ** -6, 2.0 ** 105
+    kf, vf = kc.float(), vc.float()
+    kf[:], q[..., 0] = 0.0, 8.0
+    page, place = int(table[0, 260 // 64]), 260 % 64
+    scales[page, :, 0] = 2.0 ** -3
+    kf[page, :, place, 0] = round(7.9 * np.log(2) * d ** 0.5)
+    vf[page, :, :, place] = 448.0
+    check(name, q, (kf.to(kc.dtype), vf.to(vc.dtype), scales), table, rows, keys)

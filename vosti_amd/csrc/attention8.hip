@@ -39,10 +39,12 @@
 // are the maximum itself it was 2^-25: 4,096 keys that stand that far behind one whose value is 0 gave a result off by 2 % and more.
 #ifdef VK_BF16
 #define A8_LOW 7.0f
+#define A8_PART 0.0078125f        // 2^-A8_LOW: of sums that meet others, which may be 32-bit numbers of the values' own size
 #define A8_STEP 15.0f
 #define A8_FAR 4194304.0f         // 2^22
 #else
 #define A8_LOW 0.0f
+#define A8_PART 1.0f
 #define A8_STEP 8.0f
 #define A8_FAR 67108864.0f        // 2^26
 #endif
@@ -680,10 +682,10 @@ __global__ __launch_bounds__(256, DP <= 128 && NT == 1 ? 2 : 1) void a8_few_kern
     for (int n = 0; n < NT; ++n) {
       __syncthreads();                                  // the maxima are there; the sums of the columns before have been read
       const int x0 = 16 * n + c.r, col = c.col0 + x0;
-      const float top = fmaxf(fmaxf(maxima[0][x0], maxima[1][x0]), fmaxf(maxima[2][x0], maxima[3][x0])), by = exp2_fast(o.m[n] - top) * o.scale();
+      const float top = fmaxf(fmaxf(maxima[0][x0], maxima[1][x0]), fmaxf(maxima[2][x0], maxima[3][x0])), by = exp2_fast(o.m[n] - top) * (o.scale() * A8_PART);
       float total = 0.f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) total = __builtin_fmaf(totals[x][x0], exp2_fast(maxima[x][x0] - top), total);
+      for (int x = 0; x < 4; ++x) total = __builtin_fmaf(totals[x][x0] * A8_PART, exp2_fast(maxima[x][x0] - top), total);
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt) *reinterpret_cast<f32x4*>(sums[wave][dt][lane]) = o.times(n, dt, by);
       __syncthreads();
@@ -915,8 +917,8 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) void a8_shared_kerne
       const int64_t part = (((int64_t)item * a.nkv + kvh) * a.nseg + seg_at) * a.cols_max + col;
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt)
-        if (16 * dt < a.d) *reinterpret_cast<f32x4*>(a.part_acc + part * a.d + 16 * dt + 4 * c.g) = o.times(n, dt, o.scale());
-      if (c.g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * part) = f32x2{o.m[n], l};
+        if (16 * dt < a.d) *reinterpret_cast<f32x4*>(a.part_acc + part * a.d + 16 * dt + 4 * c.g) = o.times(n, dt, o.scale() * A8_PART);
+      if (c.g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * part) = f32x2{o.m[n], l * A8_PART};
     } else {
       elem_t* to = a8_out<NT>(a, c, col);
       const float by = l == 0.f ? 0.f : o.scale() / l;
