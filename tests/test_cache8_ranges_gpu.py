@@ -118,3 +118,23 @@ def test_values_near_the_largest_numbers(name, d, rows, keys):
     kf[page, :, place, 0] = round(7.9 * np.log(2) * d ** 0.5)
     vf[page, :, :, place] = 448.0
     check(name, q, (kf.to(kc.dtype), vf.to(vc.dtype), scales), table, rows, keys)
+
+
+@pytest.mark.parametrize("d", (48, 64, 80, 112, 144, 192, 208))
+@pytest.mark.parametrize("rows", (1, 20))
+def test_which_heads_take_q_whole(d, rows):
+    """q with one entry far above the others, against keys that are 0 there.  Heads to 64 and of 129 to 192 entries take it whole and are held to the bounds of `close`; others hold entries below 2^-14 of the
+    largest's power of two to 2^-22 of it, which moves a score by that times the sum of |k|, and a result by twice that of the mean of |v - out|, at most that of |v| and |out|."""
+    k, keys = kernels_for("bf16"), 150
+    table, (kc, vc, scales), q = case("bf16", d, 64, rows, keys, d + rows)
+    kc[..., 3] = torch.zeros((), device="cuda").to(kc.dtype)
+    q *= torch.from_numpy(2.0 ** np.random.default_rng(d).integers(-16, 1, tuple(q.shape))).to(q.dtype).cuda()
+    q[..., 3] = torch.tensor([2.0 ** 9, 2.0 ** 14, 2.0 ** 9, 2.0 ** 14], device="cuda").to(q.dtype)
+    if not 64 < d <= 128 and d <= 192:
+        return check("bf16", q, (kc, vc, scales), table, rows, keys)
+    got = host(attend(k, q, (kc, vc, scales), table, [rows], [keys], 16 if rows <= 16 else 128))
+    out, weighted, most, flushed = attention(host(q), *map(host, (kc, vc, scales)), table, [0, rows], [keys], d ** -0.5)
+    power = 2.0 ** np.floor(np.log2(np.abs(host(q)).max(-1, keepdims=True)))
+    size = (np.abs(host(kc)).sum(-1) * host(scales)[:, :, None, 0]).max() * d ** -0.5
+    moved = 2.0 ** -22 * power * size + 2 * (d + 16) * 2.0 ** -24 * most + 2.0 ** -20
+    assert (np.abs(got - out) <= 2.0 ** -8 * 1.01 * np.abs(out) + (weighted + np.abs(out)) * (2.0 ** -11 + 2 * moved) + 2.0 ** -25 * flushed + 1e-30).all()
