@@ -8,7 +8,7 @@
 // 16 (r / 4) + 4 t + r % 4 for t = 0..3, of V the keys 16 g .. 16 g + 15 of entry 16 dt + r.  K's rows are taken in that order so that the scores that a lane ends with
 // (rows 4 g + i of S^T's tile t) are those of the keys 16 g + 4 t + i: the lane's own 16 keys of V, and no weight has to change lanes between the products.
 //
-// Arithmetic.  A key's entry times its scale is exact in the element type, so the first product takes q as it is and 32-bit sums.  For heads of 128 and 256 it takes the keys as they are
+// Arithmetic.  A key's entry times its scale is exact in the element type, so the first product takes q as it is and 32-bit sums.  Where tiles are 128 or 256 entries wide (heads of 80 to 128 and of 208 to 256) it takes the keys as they are
 // stored, and q as two e4m3 numbers of four digits each in units of the head's largest entry: they hold its eight digits where it is 2^-14 of the largest's power of two or more, and are off by
 // 2^-22 of that power at most elsewhere; products of twice the rate make up for there being two, and no key has to be turned into an operand (a prompt of 4,096 rows 186 -> 163 us; of heads of 64 the
 // product, 128 entries long, would be half empty).  Weights go into the
@@ -22,9 +22,10 @@
 // taken out of the second product of a tile that not all rows see whole; a row that does see a NaN gets it back through a product of its own.
 //
 // What bounds it (MI355X, bfloat16, heads of 128, 8 kv heads; reading alone reaches 6.45 TB/s here, a large bfloat16 product 1.45 PFLOP/s): 64 rows with 8,192 keys each, 32 heads, 1.08 GB
-// of cache: 188 us, 5.7 TB/s, and 5 us for the join: bytes.  13 sequences of 5 rows and some 4,000 keys, 64 heads, 73 MB: 26 us and 5: workgroups of eight tiles one after
-// the other, little more than one round of them.  A prompt of 4,096 rows over itself, 32 heads, 137 GFLOP: 158 us, 138 to 144 in a row of calls, 0.87 to 0.99 PFLOP/s: a wave's products
-// and the exponentials behind them follow each other, and its registers leave room for two waves a unit.  A single row with 333 keys: 10 us, loads that wait for each other.
+// of cache: 188 us, 5.7 TB/s, and 5 us for the join: bytes.  13 sequences of 5 rows and up to 4,096 keys, 64 heads, 73 MB: 26 us and 5: 592 workgroups with keys, all of them on the card at
+// once, each eight tiles one after the other.  A prompt of 4,096 rows over itself, 32 heads, 137 GFLOP: 159 us, 140 in a row of calls, 0.87 to 0.99 PFLOP/s: a wave's products
+// and the exponentials behind them follow each other, and its registers leave room for two waves a unit.  Portions of 5 prompts, 2,625 rows in all, windows of 1,024, pages of 16, 49 GFLOP: 99 us, 92 in a row:
+// 16 to 18 tiles each for 792 workgroups on 512 places, two rounds of them where one and a half are needed; pages of 64 take 3 us off it.  A single row with 333 keys: 10 us, loads that wait for each other.
 #include <type_traits>
 
 #include "cache8.h"

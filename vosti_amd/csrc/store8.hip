@@ -16,8 +16,8 @@
 //
 // Measured (MI355X, bfloat16, 32 q and 8 kv heads of 128, pages of 64; a copy reaches 4.75 TB/s here): a prompt of 4,096 tokens, 93 MB: 31 us, 28.6 in a row of calls, 3.0 to 3.3 TB/s: four
 // workgroups a CU is what the 64-bit norm's registers leave (five or six spill: 38 -> 50 us with nothing in the caches), and a page's rows wait for their maximum.  Rows and angles that are read one row ahead, as
-// they are stored, took 3 us off it and 2 off a step of 64 tokens.  A token each of 64 sequences, 1.5 MB: 8.8 us: the sequence's lengths, then the page's number, its scale and, where that grows,
-// its entries, one load behind the other.  The 32-bit build, 2,300 tokens of 7 sequences, 16 and 8 heads of 64: 13 us.
+// they are stored, took 3 us off it and 2 off a step of 64 tokens.  A token each of 64 sequences, 1.5 MB: 8.8 us where no page's scale grows: the sequence's lengths, then the page's number and
+// its scale, one load behind the other; 16.7 where a third of them do: a page's entries behind that.  The 32-bit build, 2,300 tokens of 7 sequences, 16 and 8 heads of 64: 13 us, whether scales grow or not.
 #include "cache8.h"
 #include "vec.h"
 

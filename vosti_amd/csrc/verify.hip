@@ -13,7 +13,7 @@
 // 64-bit fused multiply-adds are as fast as its 32-bit ones.
 //
 // Measured (MI355X, bfloat16 logits of 151,936, four drafted tokens): 64 sequences, 175 MB: 67 us for maximum and sum (its bytes take 27; seventeen 64-bit operations an exponential 38, beside the
-// search for the maximum), 8 to decide, 19 for the pieces, 8 to draw.  One sequence: 5.5, 7.2 and 6.5 us, launches and loads that wait for each other.
+// search for the maximum), 8 to decide, 19 for the pieces, 8 to draw.  One sequence, its token drawn: 4.8, 7.3 and 6.6 us, launches and loads that wait for each other.
 //
 // Four launches: maximum and sum of pieces of every row, a wave each; which tokens stand, and the distributions behind them; what the pieces of those weigh; the piece and
 // the token in it (the second and third as one where there are few pieces).  Pieces have the same borders and their sums the same order whatever else is in the call.

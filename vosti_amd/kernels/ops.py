@@ -486,10 +486,14 @@ class Kernels:
         items [n, 2] = (sequence, first row): an item is up to ``item_rows`` consecutive rows of its sequence, at most ATTN_ITEM_ROWS.  Items of up
         to 16 rows have their keys split over workgroups, whose sums meet in ``scratch`` (``attn8_scratch_floats``; without it the call takes memory of its own);
         a scratch belongs to one call at a time, in recorded graphs too.  They are for decoded and drafted tokens and for a portion of few sequences (32 heads of 128,
-        one sequence of 8,192 keys: 128 rows in 50 us, as one item in 208); larger items read the cache less often and are for prompts (1,024 rows of that sequence: 209 us
-        against 278; 64 portions of 128 rows with 1,000 keys: 168 against 367).  A row's last bits depend on its item (``item_rows``, the item's other
-        rows) and on nothing else in the call.  In bfloat16, values of pages whose scale is 2^75 below that of another page that the same item sees may count as 0.  ``max_k_len`` is the host's bound on k_len; the block table must cover it, and keys beyond it may be left out.  Rows that no item
-        names are left as they were."""
+        one sequence of 8,192 keys: 128 rows in 45 us, as one item in 180); larger items read the cache less often and are for prompts (1,024 rows of that sequence: 182 us
+        against 247; 64 portions of 128 rows with 1,000 keys: 156 against 334).  A row's last bits depend on its item (``item_rows``, the item's other
+        rows) and on nothing else in the call.  ``max_k_len`` is the host's bound on k_len; the block table must cover it, and keys beyond it may be left out.  Rows that no item
+        names are left as they were.
+
+        In bfloat16, weights are off by up to 2^-11 of themselves, or by 2^-32 of the row's largest where that is more; for heads of 80 to 128 and of 208 to 256 entries, entries of q below
+        2^-14 of their head's largest are off by up to 2^-22 of it (heads of other sizes take q whole); and values of pages whose scale is 2^75 below that of another page that the same
+        item sees may count as 0."""
         here = self._device()
         if q.dim() != 3 or k_cache.dim() != 4:
             raise KernelError(f"attention8: q {tuple(q.shape)} is not [T, heads, size], or the k cache {tuple(k_cache.shape)} not [pages, kv heads, page size, size]")
