@@ -138,3 +138,16 @@ def test_which_heads_take_q_whole(d, rows):
     size = (np.abs(host(kc)).sum(-1) * host(scales)[:, :, None, 0]).max() * d ** -0.5
     moved = 2.0 ** -22 * power * size + 2 * (d + 16) * 2.0 ** -24 * most + 2.0 ** -20
     assert (np.abs(got - out) <= 2.0 ** -8 * 1.01 * np.abs(out) + (weighted + np.abs(out)) * (2.0 ** -11 + 2 * moved) + 2.0 ** -25 * flushed + 1e-30).all()
+
+
+@pytest.mark.parametrize("order", ((0, -20, -40, -60), (-60, -40, -20, 0), (-20, -60, 0, -40)))
+@pytest.mark.parametrize("name,d,rows", [("bf16", 64, 2), ("bf16", 128, 12), ("bf16", 128, 70), ("bf16", 256, 16), ("bf16", 192, 100), ("f32", 64, 70)])
+def test_every_page_of_a_tile_in_a_scale_of_its_own(name, d, rows, order):
+    """Pages of 16 keys in steps of 2^20 to 2^60, and windows of a key to two pages: each row is held to the values that it sees, in as many passes as a tile has pages."""
+    for window in (1, 5, 16, 31):
+        for keys in (70, 200 + rows):
+            keys = max(keys, rows)
+            table, (kc, vc, scales), q = case(name, d, 16, rows, keys, d + rows + window)
+            for at in range(-(-keys // 16)):
+                scales[int(table[0, at]), :, 1] = 2.0 ** order[at % 4]
+            check(name, q, (kc, vc, scales), table, rows, keys, window)
